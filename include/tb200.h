@@ -299,6 +299,58 @@ extern "C"
     TB200_API tb200_status tb200_matmul(tb200_ctx* ctx, const tb200_tensor* a, const tb200_tensor* b, int32_t a_zp,
                                         int32_t b_zp, const tb200_epilogue* epilogue, tb200_tensor* output);
 
+    /* ---- feed-forward operators -------------------------------------------------------------------
+     * The block behind a decoder's attention: two projections of the same rows, one through an activation, multiplied.
+     * TOSA has no operator for it (a graph spells it MATMUL, MATMUL, SIGMOID, MUL, MUL) and none for 4-bit weights; the
+     * reference has no counterpart.  All sums are taken in fp32 and results rounded once.  Every operand must be
+     * contiguous, no output may overlap an operand. */
+    typedef enum tb200_activation
+    {
+        TB200_ACT_SILU      = 0, /* x / (1 + exp(-x)) */
+        TB200_ACT_GELU      = 1, /* x * (1 + erf(x / sqrt(2))) / 2 */
+        TB200_ACT_GELU_TANH = 2, /* x * (1 + tanh(sqrt(2 / pi) * (x + 0.044715 x^3))) / 2 */
+        TB200_ACT_RELU      = 3, /* derivative at 0: 0 */
+        TB200_ACT_SIGMOID   = 4
+    } tb200_activation;
+
+    /* A [C,W] matrix of 4-bit elements, stored by output column: `data` INT8 or UINT8 [W, pitch], pitch >= (C + 1) / 2
+     * bytes, element c of a row in bits 4 * (c % 2) .. 4 * (c % 2) + 3 of byte c / 2, two's complement (-8 .. 7).  Element
+     * (c, w) stands for scale[c / group, w] * (element - zero[c / group, w]).  scale FP16, BF16 or FP32 [groups, W] with
+     * groups = ceil(C / group); zero INT8 [groups, W] with values -8 .. 7 (another value is a failed REQUIRE:
+     * TB200_UNPREDICTABLE at the next sync), or NULL for none.  group: a multiple of 32, or at least C (one scale per
+     * column).  What a row holds behind its last element is not used.  Rows whose pitch is a multiple of 16 bytes are
+     * read as they are; others are copied into scratch first. */
+    typedef struct tb200_w4
+    {
+        const tb200_tensor* data;
+        const tb200_tensor* scale;
+        const tb200_tensor* zero;
+        int32_t group;
+    } tb200_w4;
+
+    /* MATMUL with 4-bit weights: a [N,H,C] (FP16, BF16 or FP32), output [N,H,W] of a's type or FP32; the matrix is shared by
+     * the N batches.  */
+    TB200_API tb200_status tb200_matmul_w4(tb200_ctx* ctx, const tb200_tensor* a, const tb200_w4* b, tb200_tensor* output);
+
+    /* output = activation(a x gate) * (a x up), FP16, BF16 or FP32: a [N,H,C], gate and up [N,C,W], or [1,C,W] shared by the
+     * batches; output [N,H,W] of a's type or FP32.  The two projections never reach device memory in the 16-bit types. */
+    TB200_API tb200_status tb200_matmul_gated(tb200_ctx* ctx, const tb200_tensor* a, const tb200_tensor* gate,
+                                              const tb200_tensor* up, int32_t activation, tb200_tensor* output);
+
+    /* Gradients of tb200_matmul_gated's operands from its output's (grad_output, the operands' type), the projections being
+     * evaluated again: with G = a x gate, U = a x up, dG = grad_output * U * activation'(G), dU = grad_output * activation(G),
+     *   grad_a = dG x gate^T + dU x up^T, grad_gate = a^T x dG, grad_up = a^T x dU,
+     * the last two summed over the batches where the weights are shared.  Each gradient has its operand's shape, the operands'
+     * type or FP32, and may be NULL.  In the 16-bit types dG and dU are rounded to that type between the products. */
+    TB200_API tb200_status tb200_matmul_gated_backward(tb200_ctx* ctx, const tb200_tensor* a, const tb200_tensor* gate,
+                                                       const tb200_tensor* up, const tb200_tensor* grad_output,
+                                                       int32_t activation, tb200_tensor* grad_a, tb200_tensor* grad_gate,
+                                                       tb200_tensor* grad_up);
+
+    /* tb200_matmul_gated with 4-bit weights (shared by the batches, both of the same group). */
+    TB200_API tb200_status tb200_matmul_gated_w4(tb200_ctx* ctx, const tb200_tensor* a, const tb200_w4* gate,
+                                                 const tb200_w4* up, int32_t activation, tb200_tensor* output);
+
     /* RESCALE.  Replaces OpRescale<Rank,In,Out>::eval (reference_model/src/ops/type_conversion.cpp:223-422, checks
      * :71-154) with QuantUtil::apply_scale_32 / apply_scale_16 (reference_model/src/quant_util.h:45-108). */
     TB200_API tb200_status tb200_rescale(tb200_ctx* ctx, const tb200_tensor* input, const tb200_rescale_attr* attr,

@@ -13,6 +13,7 @@ from .binding import (  # noqa: F401
     Status,
     Tb200Error,
     Tensor,
+    W4,
     lib_path,
     load_library,
     npy_probe,

@@ -39,6 +39,7 @@ _NP_DTYPE = {DType.FP16: np.float16, DType.FP32: np.float32, DType.INT16: np.int
              DType.INT8: np.int8, DType.UINT16: np.uint16, DType.UINT8: np.uint8, DType.BF16: np.uint16,
              DType.FP8E4M3: np.uint8, DType.FP8E5M2: np.uint8}    # bf16 and fp8 travel as raw bit patterns
 ROUNDING = {"SINGLE_ROUND": 0, "DOUBLE_ROUND": 1, "INEXACT_ROUND": 2}
+ACTIVATION = {"SILU": 0, "GELU": 1, "GELU_TANH": 2, "RELU": 3, "SIGMOID": 4}    # tb200_activation
 
 
 class Tb200Error(RuntimeError):
@@ -60,6 +61,10 @@ class _Epilogue(ctypes.Structure):
                 ("clamp_max_f", ctypes.c_float)]
 
 
+class _W4(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("scale", ctypes.c_void_p), ("zero", ctypes.c_void_p), ("group", ctypes.c_int32)]
+
+
 def lib_path():
     return os.path.join(_HERE, "csrc", "libtb200.so")
 
@@ -79,6 +84,7 @@ EXPORTS = [
     "tb200_set_wait_limit", "tb200_set_shared_gpu", "tb200_set_launch_overlap", "tb200_const_cache_control", "tb200_const_cache_entries",
     "tb200_comm_unique_id", "tb200_comm_init", "tb200_comm_attach", "tb200_comm_destroy", "tb200_comm_rank",
     "tb200_comm_size", "tb200_gather_output",
+    "tb200_matmul_w4", "tb200_matmul_gated", "tb200_matmul_gated_backward", "tb200_matmul_gated_w4",
 ]
 
 
@@ -153,6 +159,10 @@ def load_library():
         "tb200_comm_rank": (i32, [vp]),
         "tb200_comm_size": (i32, [vp]),
         "tb200_gather_output": (i32, [vp, vp, vp]),
+        "tb200_matmul_w4": (i32, [vp, vp, ctypes.POINTER(_W4), vp]),
+        "tb200_matmul_gated": (i32, [vp, vp, vp, vp, i32, vp]),
+        "tb200_matmul_gated_backward": (i32, [vp, vp, vp, vp, vp, i32, vp, vp, vp]),
+        "tb200_matmul_gated_w4": (i32, [vp, vp, ctypes.POINTER(_W4), ctypes.POINTER(_W4), i32, vp]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)
@@ -221,6 +231,20 @@ class Epilogue:
             else:
                 self.c.clamp_min_i, self.c.clamp_max_i = int(lo), int(hi)
                 self.c.clamp_min_f, self.c.clamp_max_f = float(lo), float(hi)
+
+
+class W4:
+    """A [C,W] matrix of 4-bit weights (device Tensors): data bytes [W, pitch], element c of a row in nibble c % 2 of byte c // 2,
+    two's complement; scale and zero (or None) [ceil(C / group), W]: tb200_w4."""
+
+    def __init__(self, data, scale, zero=None, group=128):
+        self.data, self.scale, self.zero, self.group = data, scale, zero, int(group)
+        self.c = _W4(data.handle, scale.handle, zero.handle if zero is not None else None, self.group)
+        self.ref = ctypes.byref(self.c)
+
+
+def _activation(a):
+    return ACTIVATION[a] if isinstance(a, str) else int(a)
 
 
 class Tensor:
@@ -473,6 +497,26 @@ class Context:
     def matmul(self, a, b, out, a_zp=0, b_zp=0, epilogue=None, check=True):
         return self._check(self.lib.tb200_matmul(self.handle, a.handle, b.handle, int(a_zp), int(b_zp),
                                                  ctypes.byref(epilogue.c) if epilogue else None, out.handle), check)
+
+    def matmul_w4(self, a, w, out, check=True):
+        """MATMUL of a [N,H,C] with a W4 matrix [C,W]."""
+        return self._check(self.lib.tb200_matmul_w4(self.handle, a.handle, w.ref, out.handle), check)
+
+    def matmul_gated(self, a, gate, up, out, activation="SILU", check=True):
+        """out = activation(a x gate) * (a x up); gate and up [N,C,W], or [1,C,W] shared by the batches."""
+        return self._check(self.lib.tb200_matmul_gated(self.handle, a.handle, gate.handle, up.handle, _activation(activation),
+                                                       out.handle), check)
+
+    def matmul_gated_backward(self, a, gate, up, grad_out, grad_a=None, grad_gate=None, grad_up=None, activation="SILU", check=True):
+        """Gradients of matmul_gated's operands from its output's; a gradient that is None is not computed."""
+        g = [t.handle if t is not None else None for t in (grad_a, grad_gate, grad_up)]
+        return self._check(self.lib.tb200_matmul_gated_backward(self.handle, a.handle, gate.handle, up.handle, grad_out.handle,
+                                                                _activation(activation), *g), check)
+
+    def matmul_gated_w4(self, a, gate, up, out, activation="SILU", check=True):
+        """matmul_gated with two W4 matrices."""
+        return self._check(self.lib.tb200_matmul_gated_w4(self.handle, a.handle, gate.ref, up.ref, _activation(activation), out.handle),
+                           check)
 
     def rescale(self, x, attr, out, check=True):
         return self._check(self.lib.tb200_rescale(self.handle, x.handle, ctypes.byref(attr.c), out.handle), check)

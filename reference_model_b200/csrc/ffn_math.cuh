@@ -1,0 +1,122 @@
+// Activations of the gated product, their derivatives, and rounding to the output's type.
+#pragma once
+#include <cstdint>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "common.h"
+
+namespace tb200
+{
+namespace ffn
+{
+
+// Value of the activation.  The logistic forms divide by 1 + exp(-x), which neither cancels nor overflows to NaN for a finite x;
+// the Gaussian one goes through erfc, whose relative error stays small in the left tail where 1 + erf would cancel.
+template <int ACT>
+__device__ __forceinline__ float act_value(float g)
+{
+    if (ACT == TB200_ACT_SILU)
+        return g / (1.f + expf(-g));
+    if (ACT == TB200_ACT_GELU)
+        return 0.5f * g * erfcf(-0.70710678118654752f * g);
+    if (ACT == TB200_ACT_GELU_TANH)
+        return g / (1.f + expf(-1.5957691216057308f * (g + 0.044715f * g * g * g)));    // (1 + tanh(y)) / 2 = 1 / (1 + exp(-2 y))
+    if (ACT == TB200_ACT_RELU)
+        return g < 0.f ? 0.f : g;    // a NaN stays one
+    return 1.f / (1.f + expf(-g));
+}
+
+// Value and derivative.
+template <int ACT>
+__device__ __forceinline__ void act_slope(float g, float& value, float& slope)
+{
+    if (ACT == TB200_ACT_SILU || ACT == TB200_ACT_SIGMOID)
+    {
+        const float s = 1.f / (1.f + expf(-g));
+        value         = ACT == TB200_ACT_SILU ? g * s : s;
+        slope         = ACT == TB200_ACT_SILU ? s * (1.f + g * (1.f - s)) : s * (1.f - s);
+    }
+    else if (ACT == TB200_ACT_GELU)
+    {
+        const float p = 0.5f * erfcf(-0.70710678118654752f * g);
+        value         = g * p;
+        slope         = p + g * (0.39894228040143268f * expf(-0.5f * g * g));
+    }
+    else if (ACT == TB200_ACT_GELU_TANH)
+    {
+        const float s = 1.f / (1.f + expf(-1.5957691216057308f * (g + 0.044715f * g * g * g)));
+        value         = g * s;
+        slope         = s + g * s * (1.f - s) * 1.5957691216057308f * (1.f + 0.134145f * g * g);
+    }
+    else
+    {
+        value = g < 0.f ? 0.f : g;
+        slope = g > 0.f ? 1.f : g <= 0.f ? 0.f : g;
+    }
+}
+
+__device__ __forceinline__ float act_value(int act, float g)
+{
+    switch (act)
+    {
+        case TB200_ACT_SILU: return act_value<TB200_ACT_SILU>(g);
+        case TB200_ACT_GELU: return act_value<TB200_ACT_GELU>(g);
+        case TB200_ACT_GELU_TANH: return act_value<TB200_ACT_GELU_TANH>(g);
+        case TB200_ACT_RELU: return act_value<TB200_ACT_RELU>(g);
+        default: return act_value<TB200_ACT_SIGMOID>(g);
+    }
+}
+
+__device__ __forceinline__ void act_slope(int act, float g, float& value, float& slope)
+{
+    switch (act)
+    {
+        case TB200_ACT_SILU: act_slope<TB200_ACT_SILU>(g, value, slope); break;
+        case TB200_ACT_GELU: act_slope<TB200_ACT_GELU>(g, value, slope); break;
+        case TB200_ACT_GELU_TANH: act_slope<TB200_ACT_GELU_TANH>(g, value, slope); break;
+        case TB200_ACT_RELU: act_slope<TB200_ACT_RELU>(g, value, slope); break;
+        default: act_slope<TB200_ACT_SIGMOID>(g, value, slope); break;
+    }
+}
+
+__device__ __forceinline__ float load_fp(const void* p, int64_t i, tb200_dtype dt)
+{
+    if (dt == TB200_FP32)
+        return reinterpret_cast<const float*>(p)[i];
+    if (dt == TB200_FP16)
+        return __half2float(reinterpret_cast<const __half*>(p)[i]);
+    return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p)[i]);
+}
+
+// Results are rounded once, to nearest, where they are stored.
+__device__ __forceinline__ void store_fp(void* p, int64_t i, tb200_dtype dt, float v)
+{
+    if (dt == TB200_FP32)
+        reinterpret_cast<float*>(p)[i] = v;
+    else if (dt == TB200_FP16)
+        reinterpret_cast<__half*>(p)[i] = __float2half_rn(v);
+    else
+        reinterpret_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+}
+
+__device__ __forceinline__ uint32_t pack2(float lo, float hi, bool bf16)
+{
+    if (bf16)
+    {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&v);
+    }
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+__device__ __forceinline__ float2 unpack2(uint32_t w, bool bf16)
+{
+    if (bf16)
+        return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w));
+    return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+
+}    // namespace ffn
+}    // namespace tb200
