@@ -26,6 +26,338 @@ tb200_status guarded(tb200_ctx* ctx, F body)
     }
 }
 
+// Carves a call's workspace out of the context's scratch: first the sizes, then the addresses.
+struct Carver
+{
+    uint8_t* base = nullptr;
+    size_t used   = 0;
+    void* take(size_t bytes)
+    {
+        void* p = base ? base + used : nullptr;
+        used += (bytes + 255) & ~(size_t)255;
+        return p;
+    }
+};
+
+int64_t round_up(int64_t v, int64_t to)
+{
+    return (v + to - 1) / to * to;
+}
+
+// A 16-bit operand as the tensor maps want it, rows a multiple of 16 bytes apart: as it lies, or copied into `pad`.
+Matrix operand(const void* data, int64_t inner, int64_t outer, int64_t batches, void* pad)
+{
+    Matrix m = { data, inner, outer, batches, inner };
+    if (inner % 8 != 0)
+    {
+        m.data  = pad;
+        m.pitch = round_up(inner, 8);
+    }
+    return m;
+}
+
+size_t pad_bytes(int64_t inner, int64_t rows)
+{
+    return inner % 8 != 0 ? (size_t)rows * round_up(inner, 8) * 2 : 0;
+}
+
+tb200_status pad(tb200_ctx* ctx, const void* data, const Matrix& m)
+{
+    if (m.data == data)
+        return TB200_OK;
+    return pitch_copy_launch(ctx, data, const_cast<void*>(m.data), m.outer * m.batches, m.inner, m.pitch);
+}
+
+#define TB200_TRY(expr)                     \
+    do                                      \
+    {                                       \
+        const tb200_status st__ = (expr);   \
+        if (st__ != TB200_OK)               \
+            return st__;                    \
+    } while (0)
+
+// Rows up to which the kernels that stream the weights past a few rows serve.
+constexpr int64_t kFewRows = 64;
+
+// 16-bit gated product on the tensor cores
+tb200_status gated_pair(tb200_ctx* ctx, const GatedProblem& q)
+{
+    Carver size, at;
+    for (int pass = 0; pass < 2; pass++)
+    {
+        Carver& c     = pass ? at : size;
+        void* const a = c.take(pad_bytes(q.C, q.NB * q.H));
+        void* const g = c.take(pad_bytes(q.W, (int64_t)q.NB * q.C));
+        void* const u = c.take(pad_bytes(q.W, (int64_t)q.NB * q.C));
+        if (!pass)
+        {
+            if (size.used)
+                TB200_TRY(ensure_scratch(ctx, size.used));
+            at.base = reinterpret_cast<uint8_t*>(ctx->scratch);
+            continue;
+        }
+        PairProduct k;
+        memset(&k, 0, sizeof(k));
+        k.dt   = q.dt;
+        k.kind = PAIR_GATED;
+        k.b_mn = true;
+        k.a    = operand(q.a, q.C, q.H, q.NB, a);
+        k.b[0] = operand(q.gate, q.W, q.C, q.NB, g);
+        k.b[1] = operand(q.up, q.W, q.C, q.NB, u);
+        TB200_TRY(pad(ctx, q.a, k.a));
+        TB200_TRY(pad(ctx, q.gate, k.b[0]));
+        TB200_TRY(pad(ctx, q.up, k.b[1]));
+        k.rows      = (int)q.H;
+        k.cols      = q.W;
+        k.K         = q.C;
+        k.phases    = 1;
+        k.NB        = q.NB;
+        k.results   = 1;
+        k.act       = q.act;
+        k.out[0]    = q.out;
+        k.out_dt[0] = k.out_dt[1] = q.out_dt;
+        k.ld        = q.W;
+        k.name      = "gated_pair_f16";
+        TB200_TRY(q.H <= kFewRows ? gated_rows_launch(ctx, k) : pair_launch(ctx, k));
+    }
+    return TB200_OK;
+}
+
+// Its gradients: dG and dU into scratch (rounded to the operands' type), then one product for grad_a and one for both weights'.
+tb200_status gated_backward_pair(tb200_ctx* ctx, const GatedProblem& q)
+{
+    const int64_t Wp  = round_up(q.W, 16);
+    const size_t half = (size_t)q.NB * q.H * Wp * 2;    // bytes of dG
+    Carver size, at;
+    for (int pass = 0; pass < 2; pass++)
+    {
+        Carver& c           = pass ? at : size;
+        void* const pa      = c.take(pad_bytes(q.C, q.NB * q.H));
+        void* const pg      = c.take(pad_bytes(q.W, (int64_t)q.NB * q.C));
+        void* const pu      = c.take(pad_bytes(q.W, (int64_t)q.NB * q.C));
+        uint8_t* const dg   = reinterpret_cast<uint8_t*>(c.take(2 * half));
+        if (!pass)
+        {
+            TB200_TRY(ensure_scratch(ctx, size.used));
+            at.base = reinterpret_cast<uint8_t*>(ctx->scratch);
+            continue;
+        }
+        const Matrix a = operand(q.a, q.C, q.H, q.NB, pa), gate = operand(q.gate, q.W, q.C, q.NB, pg), up = operand(q.up, q.W, q.C, q.NB, pu);
+        TB200_TRY(pad(ctx, q.a, a));
+        TB200_TRY(pad(ctx, q.gate, gate));
+        TB200_TRY(pad(ctx, q.up, up));
+        PairProduct k;
+        memset(&k, 0, sizeof(k));
+        k.dt      = q.dt;
+        k.kind    = PAIR_GRAD;
+        k.b_mn    = true;
+        k.a       = a;
+        k.b[0]    = gate;
+        k.b[1]    = up;
+        k.rows    = (int)q.H;
+        k.cols    = q.W;
+        k.K       = q.C;
+        k.phases  = 1;
+        k.NB      = q.NB;
+        k.results = 2;
+        k.act     = q.act;
+        k.dout    = q.dout;
+        k.out[0]  = dg;
+        k.out[1]  = dg + half;
+        k.out_dt[0] = k.out_dt[1] = q.dt;
+        k.ld      = Wp;
+        k.name    = "gated_backward_pair_f16";
+        TB200_TRY(pair_launch(ctx, k));
+        const Matrix d = { dg, q.W, q.H, 2 * (int64_t)q.NB, Wp };
+        if (q.da)
+        {
+            memset(&k, 0, sizeof(k));
+            k.dt        = q.dt;
+            k.kind      = PAIR_PLAIN;
+            k.a         = d;
+            k.b[0]      = gate;
+            k.b[1]      = up;
+            k.rows      = (int)q.H;
+            k.cols      = q.C;
+            k.K         = q.W;
+            k.phases    = 2;
+            k.NB        = q.NB;
+            k.results   = 1;
+            k.out[0]    = q.da;
+            k.out_dt[0] = q.da_dt;
+            k.ld        = q.C;
+            k.name      = "gated_backward_pair_f16";
+            TB200_TRY(pair_launch(ctx, k));
+        }
+        if (q.dgate || q.dup)
+        {
+            memset(&k, 0, sizeof(k));
+            k.dt      = q.dt;
+            k.kind    = PAIR_PLAIN;
+            k.a_mn    = true;
+            k.b_mn    = true;
+            k.a       = a;
+            k.b[0]    = d;
+            k.rows    = q.C;
+            k.cols    = q.W;
+            k.K       = q.H;
+            k.phases  = 1;
+            k.NB      = q.NB;
+            k.results = q.dgate && q.dup ? 2 : 1;
+            if (!q.dgate)
+                k.b[0].data = dg + half;
+            k.b[0].batches = (int64_t)q.NB * k.results;
+            k.out[0]    = q.dgate ? q.dgate : q.dup;
+            k.out_dt[0] = q.dgate ? q.dgate_dt : q.dup_dt;
+            k.out[1]    = k.results == 2 ? q.dup : nullptr;
+            k.out_dt[1] = q.dup_dt;
+            k.ld        = q.W;
+            k.name      = "gated_backward_pair_f16";
+            TB200_TRY(pair_launch(ctx, k));
+        }
+    }
+    return TB200_OK;
+}
+
+// fp32: the two projections by the fp32 product, then a pass over them
+tb200_status gated_f32(tb200_ctx* ctx, const GatedProblem& q)
+{
+    const int64_t rows = q.NB * q.H, n = rows * q.W;
+    Carver c;
+    c.take((size_t)n * 4);
+    c.take((size_t)n * 4);
+    TB200_TRY(ensure_scratch(ctx, c.used));
+    c       = Carver();
+    c.base  = reinterpret_cast<uint8_t*>(ctx->scratch);
+    float* const g = reinterpret_cast<float*>(c.take((size_t)n * 4));
+    float* const u = reinterpret_cast<float*>(c.take((size_t)n * 4));
+    const float* a = reinterpret_cast<const float*>(q.a);
+    TB200_TRY(sgemm_f32_launch(ctx, a, reinterpret_cast<const float*>(q.gate), g, q.NB, (int)q.H, q.C, q.W));
+    TB200_TRY(sgemm_f32_launch(ctx, a, reinterpret_cast<const float*>(q.up), u, q.NB, (int)q.H, q.C, q.W));
+    TB200_TRY(gate_f32_launch(ctx, g, u, reinterpret_cast<float*>(q.out), n, q.act));
+    return post_launch(ctx, "gated_f32", 0);
+}
+
+// Its gradients: the fp32 product takes its second operand as [K][columns], so what lies the other way is transposed into scratch.
+tb200_status gated_backward_f32(tb200_ctx* ctx, const GatedProblem& q)
+{
+    const int64_t rows = q.NB * q.H, n = rows * q.W, weights = (int64_t)q.C * q.W;
+    const bool weights_too = q.dgate || q.dup;
+    Carver c;
+    float *g = nullptr, *u = nullptr, *both = nullptr, *bt = nullptr, *at = nullptr;
+    for (int pass = 0; pass < 2; pass++)
+    {
+        g    = reinterpret_cast<float*>(c.take((size_t)n * 4));
+        u    = reinterpret_cast<float*>(c.take((size_t)n * 4));
+        both = reinterpret_cast<float*>(c.take(q.da ? (size_t)n * 8 : 0));
+        bt   = reinterpret_cast<float*>(c.take(q.da ? (size_t)q.NB * weights * 8 : 0));
+        at   = reinterpret_cast<float*>(c.take(weights_too ? (size_t)rows * q.C * 4 : 0));
+        if (!pass)
+        {
+            TB200_TRY(ensure_scratch(ctx, c.used));
+            c      = Carver();
+            c.base = reinterpret_cast<uint8_t*>(ctx->scratch);
+        }
+    }
+    const float *a = reinterpret_cast<const float*>(q.a), *gate = reinterpret_cast<const float*>(q.gate), *up = reinterpret_cast<const float*>(q.up);
+    TB200_TRY(sgemm_f32_launch(ctx, a, gate, g, q.NB, (int)q.H, q.C, q.W));
+    TB200_TRY(sgemm_f32_launch(ctx, a, up, u, q.NB, (int)q.H, q.C, q.W));
+    TB200_TRY(grad_f32_launch(ctx, g, u, reinterpret_cast<const float*>(q.dout), q.da ? both : nullptr, rows, q.W, q.act));
+    if (q.da)
+    {
+        TB200_TRY(transpose_f32_launch(ctx, gate, bt, q.NB, q.C, q.W, 2 * weights));
+        TB200_TRY(transpose_f32_launch(ctx, up, bt + weights, q.NB, q.C, q.W, 2 * weights));
+        TB200_TRY(sgemm_f32_launch(ctx, both, bt, reinterpret_cast<float*>(q.da), q.NB, (int)q.H, 2 * q.W, q.C));
+    }
+    if (weights_too)
+    {
+        TB200_TRY(transpose_f32_launch(ctx, a, at, q.NB, q.H, q.C, q.H * q.C));
+        if (q.dgate)
+            TB200_TRY(sgemm_f32_launch(ctx, at, g, reinterpret_cast<float*>(q.dgate), q.NB, q.C, (int)q.H, q.W));
+        if (q.dup)
+            TB200_TRY(sgemm_f32_launch(ctx, at, u, reinterpret_cast<float*>(q.dup), q.NB, q.C, (int)q.H, q.W));
+    }
+    return post_launch(ctx, "gated_backward_f32", 0);
+}
+
+// 4-bit weights: few rows read them as they are; more go through the values laid out in scratch, in a's type.
+tb200_status w4_launch(tb200_ctx* ctx, const W4Problem& q)
+{
+    const bool f32      = q.dt == TB200_FP32;
+    const int parts     = f32 ? 3 : 1;
+    const int64_t xpitch = round_up(q.C, 8);
+    const int64_t wpitch = round_up((q.C + 1) / 2, 16), dpitch = round_up(q.C, 32);
+    const bool few       = q.M * parts <= kFewRows;
+    const bool copy_x    = !f32 && q.C % 8 != 0;
+    const int64_t n      = q.M * q.W;
+    Carver c;
+    void *x = nullptr, *w[2] = {}, *proj[2] = {};
+    for (int pass = 0; pass < 2; pass++)
+    {
+        x = c.take(few && f32 ? (size_t)q.M * 3 * xpitch * 2 : copy_x ? (size_t)q.M * xpitch * 2 : 0);
+        for (int i = 0; i < q.mats; i++)
+        {
+            w[i]    = c.take(few ? (q.w[i].pitch % 16 ? (size_t)q.W * wpitch : 0) : f32 ? (size_t)q.C * q.W * 4 : (size_t)q.W * dpitch * 2);
+            proj[i] = c.take(!few && f32 && q.mats == 2 ? (size_t)n * 4 : 0);
+        }
+        if (!pass)
+        {
+            if (c.used)
+                TB200_TRY(ensure_scratch(ctx, c.used));
+            c      = Carver();
+            c.base = reinterpret_cast<uint8_t*>(ctx->scratch);
+        }
+    }
+    if (few)
+    {
+        W4Problem r = q;
+        for (int i = 0; i < q.mats; i++)
+            if (q.w[i].pitch % 16)
+            {
+                TB200_TRY(byte_copy_launch(ctx, q.w[i].data, reinterpret_cast<uint8_t*>(w[i]), q.W, (q.C + 1) / 2, q.w[i].pitch, wpitch));
+                r.w[i].data  = reinterpret_cast<const uint8_t*>(w[i]);
+                r.w[i].pitch = wpitch;
+            }
+        if (f32)
+            TB200_TRY(split_rows_launch(ctx, reinterpret_cast<const float*>(q.a), x, q.M, q.C, xpitch));
+        else if (copy_x)
+            TB200_TRY(pitch_copy_launch(ctx, q.a, x, q.M, q.C, xpitch));
+        return w4_rows_launch(ctx, r, f32 || copy_x ? x : q.a, f32 || copy_x ? xpitch : q.C, parts, f32 || q.dt == TB200_BF16);
+    }
+    for (int i = 0; i < q.mats; i++)
+        TB200_TRY(w4_dense_launch(ctx, q.w[i], q.C, q.W, q.group, q.dt, w[i], dpitch));
+    if (f32)
+    {
+        for (int i = 0; i < q.mats; i++)
+            TB200_TRY(sgemm_f32_launch(ctx, reinterpret_cast<const float*>(q.a), reinterpret_cast<const float*>(w[i]),
+                                       reinterpret_cast<float*>(q.mats == 2 ? proj[i] : q.out), 1, (int)q.M, q.C, q.W));
+        if (q.mats == 2)
+            TB200_TRY(gate_f32_launch(ctx, reinterpret_cast<const float*>(proj[0]), reinterpret_cast<const float*>(proj[1]), reinterpret_cast<float*>(q.out), n,
+                                      q.act));
+        return post_launch(ctx, q.mats == 2 ? "gated_w4_f32" : "matmul_w4_f32", 0);
+    }
+    PairProduct k;
+    memset(&k, 0, sizeof(k));
+    k.dt   = q.dt;
+    k.kind = q.mats == 2 ? PAIR_GATED : PAIR_PLAIN;
+    k.a    = operand(q.a, q.C, q.M, 1, x);
+    TB200_TRY(pad(ctx, q.a, k.a));
+    for (int i = 0; i < q.mats; i++)
+        k.b[i] = { w[i], q.C, q.W, 1, dpitch };
+    k.rows      = (int)q.M;
+    k.cols      = q.W;
+    k.K         = q.C;
+    k.phases    = 1;
+    k.NB        = 1;
+    k.results   = 1;
+    k.act       = q.act;
+    k.out[0]    = q.out;
+    k.out_dt[0] = k.out_dt[1] = q.out_dt;
+    k.ld        = q.W;
+    k.name      = q.mats == 2 ? "gated_w4_pair" : "matmul_w4_pair";
+    return pair_launch(ctx, k);
+}
+
 size_t aligned(size_t bytes)
 {
     return (bytes + 255) & ~(size_t)255;
@@ -69,7 +401,7 @@ tb200_status w4_entry(tb200_ctx* ctx, const char* op, const tb200_tensor* a, con
         q.w[i].scale_dt = mats[i]->scale->dtype;
         q.w[i].zero     = mats[i]->zero ? reinterpret_cast<const int8_t*>(mats[i]->zero->data) : nullptr;
     }
-    return w4_direct_launch(ctx, q);
+    return ctx->policy == 0 && q.C <= (1 << 30) ? w4_launch(ctx, q) : w4_direct_launch(ctx, q);
 }
 
 GatedProblem gated_problem(const tb200_tensor* a, const tb200_tensor* gate, const tb200_tensor* up, int activation)
@@ -128,6 +460,8 @@ extern "C" tb200_status tb200_matmul_gated(tb200_ctx* ctx, const tb200_tensor* a
         GatedProblem q = gated_problem(a, gate, up, activation);
         q.out          = output->data;
         q.out_dt       = output->dtype;
+        if (ctx->policy == 0)
+            return q.dt == TB200_FP32 ? gated_f32(ctx, q) : gated_pair(ctx, q);
         return gated_direct_launch(ctx, q);
     });
 }
@@ -175,6 +509,8 @@ extern "C" tb200_status tb200_matmul_gated_backward(tb200_ctx* ctx, const tb200_
             q.dup    = grad_up->data;
             q.dup_dt = grad_up->dtype;
         }
+        if (ctx->policy == 0)
+            return q.dt == TB200_FP32 ? gated_backward_f32(ctx, q) : gated_backward_pair(ctx, q);
         const size_t each     = aligned((size_t)q.NB * q.H * q.W * sizeof(float));
         const tb200_status st = ensure_scratch(ctx, 2 * each);
         if (st != TB200_OK)

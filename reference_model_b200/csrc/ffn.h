@@ -59,5 +59,61 @@ tb200_status gated_direct_launch(tb200_ctx* ctx, const GatedProblem& q);
 // dg, du: fp32 scratch [NB][H][W] each
 tb200_status gated_backward_direct_launch(tb200_ctx* ctx, const GatedProblem& q, float* dg, float* du);
 
+// ---- ffn_pair.cu: 16-bit products on CTA pairs
+// [batches][outer][inner] elements, rows `pitch` elements apart (a multiple of 8), 16-byte aligned
+struct Matrix
+{
+    const void* data;
+    int64_t inner, outer, batches, pitch;
+};
+enum PairKind : int
+{
+    PAIR_PLAIN = 0,
+    PAIR_GATED = 1,    // f(A B0) (A B1)
+    PAIR_GRAD  = 2     // dG and dU of the same from the output's gradient
+};
+struct PairProduct
+{
+    tb200_dtype dt;    // of the operands, FP16 or BF16
+    PairKind kind;
+    bool a_mn, b_mn;   // K across the operand's rows instead of along them
+    Matrix a, b[2];
+    int rows, cols;
+    int64_t K;
+    int phases;        // 2: K runs over a's first NB batches against b[0], then over the next NB against b[1]
+    int NB;
+    int results;       // PAIR_PLAIN, 2: b[0]'s batches NB .. 2 NB - 1 give out[1]
+    int act;
+    const void* dout;
+    void* out[2];
+    tb200_dtype out_dt[2];
+    int64_t ld;        // elements from one result row to the next
+    const char* name;
+};
+tb200_status pair_launch(tb200_ctx* ctx, const PairProduct& q);
+
+// ---- gated_rows.cu: PAIR_GATED with K across b's rows and few rows of a (weights read once)
+tb200_status gated_rows_launch(tb200_ctx* ctx, const PairProduct& q);
+
+// ---- w4_rows.cu: up to 64 16-bit rows against 4-bit weights
+// x: a's rows in 16 bits, `x_pitch` elements apart (a multiple of 8), 16-byte aligned; fp32 rows as three bf16 rows each (parts 3,
+// bf16).  The weights' pitch is a multiple of 16 bytes.
+tb200_status w4_rows_launch(tb200_ctx* ctx, const W4Problem& q, const void* x, int64_t x_pitch, int parts, bool bf16);
+
+// ---- ffn_small.cu: copies
+// fp32 rows to three bf16 rows each whose sum they are, rows `pitch` apart
+tb200_status split_rows_launch(tb200_ctx* ctx, const float* in, void* out, int64_t rows, int64_t inner, int64_t pitch);
+// rows of `inner` bytes, `in_pitch` apart, to rows `pitch` (a multiple of 16) apart
+tb200_status byte_copy_launch(tb200_ctx* ctx, const uint8_t* in, uint8_t* out, int64_t rows, int64_t inner, int64_t in_pitch, int64_t pitch);
+// [W][pitch] 16-bit rows of a 4-bit matrix's values, or fp32 [C][W] (dt FP32)
+tb200_status w4_dense_launch(tb200_ctx* ctx, const W4Mat& w, int C, int W, int group, tb200_dtype dt, void* out, int64_t pitch);
+tb200_status gate_f32_launch(tb200_ctx* ctx, const float* g, const float* u, float* out, int64_t n, int act);
+// g and u hold dG and dU afterwards, `both` (or null) the two side by side
+tb200_status grad_f32_launch(tb200_ctx* ctx, float* g, float* u, const float* d, float* both, int64_t rows, int W, int act);
+// [batches][R][C] to [batches][C][R], results `out_batch` elements apart
+tb200_status transpose_f32_launch(tb200_ctx* ctx, const float* in, float* out, int64_t batches, int64_t R, int64_t C, int64_t out_batch);
+// 16-bit rows of `inner` elements to rows `pitch` apart, zeros behind them
+tb200_status pitch_copy_launch(tb200_ctx* ctx, const void* in, void* out, int64_t rows, int64_t inner, int64_t pitch);
+
 }    // namespace ffn
 }    // namespace tb200

@@ -1,0 +1,605 @@
+// 16-bit products of the feed-forward operators on CTA pairs (tcgen05 cta_group::2): the gated product of two projections, the
+// gradients of its projections, and the plain products of the backward pass and of 4-bit weights laid out in 16 bits.
+//
+// A pair owns a 256-row tile of 256 accumulator columns.  Each CTA loads its own 128 rows of A and its own 128 columns of B per 64
+// elements of K; the tensor cores of both read B from both.  For the gated product the first CTA's 128 columns are the gate's and
+// the second's the same 128 columns of the up projection: one pass over A serves both, a thread of the epilogue finds G in
+// accumulator column j and U in column 128 + j of its own row, and neither projection leaves the chip.  The other products
+// take 256 neighbouring columns.  Either operand may have K along its rows (the tile's K runs are contiguous) or across them
+// (gradients of weights: a^T x dG reads both as they lie).  grad_a is one product over both projections: K runs over dG against
+// the gate, then over dU against the up projection, in the same accumulator.
+// Tiles go in groups of `group_m` rows of tiles, rows fastest: a wave's tiles then share few columns of B and the group's A stays
+// in L2 while B streams by once per group.
+// Sums are fp32 in tensor memory; results are rounded once, where they are stored.
+#include <algorithm>
+#include <cstring>
+#include <cuda.h>
+
+#include "ffn.h"
+#include "ffn_math.cuh"
+#include "ptx_sm100.cuh"
+
+namespace tb200
+{
+namespace ffn
+{
+namespace
+{
+
+constexpr int kEpiWarps  = 8;
+constexpr int kThreads   = 64 + 32 * kEpiWarps;    // TMA warp, MMA warp, epilogue
+constexpr int kMaxStages = 4;
+constexpr int kChunk     = 16384;    // 128 rows (or columns) x 64 elements of K
+constexpr int kSub       = 2;        // chunks per stage
+constexpr int kStage     = 2 * kSub * kChunk;
+constexpr int kSmem      = 3 * kStage + 1024;
+constexpr int kStages    = 3;
+constexpr int kTmemCols  = 512;
+
+enum : int
+{
+    EPI_PLAIN = 0,    // out[idx] = accumulator
+    EPI_GATED = 1,    // out = f(G) U
+    EPI_GRAD  = 2     // dG and dU from the output's gradient
+};
+
+struct Params
+{
+    CUtensorMap tmA, tmB0, tmB1;
+    int rows, cols;    // of a result matrix
+    int tiles_m, tiles_n, num_tiles, group_m;
+    int chunks, phases;    // K chunks of a phase
+    int NB;                // batches of A's and B's own
+    int act, bf16;
+    tb200_dtype out_dt;
+    uint32_t idesc;
+    uint64_t a_desc_hi, b_desc_hi;
+    void *out0, *out1;     // results [NB][rows][ld]; plain products: batch NB + n goes to out1
+    tb200_dtype out1_dt;
+    int64_t ld;
+    int vec;               // whole 16-element runs of a result's row may be stored 32 bytes at a time (2), 16 (1), or not (0)
+    const void* dout;      // [NB][rows][cols]
+    int dout_vec;          // its rows may be read 16 bytes at a time
+    long long wait_limit;
+    int* status;
+};
+
+struct Tile
+{
+    int idx, m0, n0;
+};
+
+template <int EPI>
+__device__ __forceinline__ Tile decode(const Params& p, int tile)
+{
+    const int per = p.tiles_m * p.tiles_n;
+    Tile t;
+    t.idx         = tile / per;
+    const int r   = tile - t.idx * per;
+    const int grp = r / (p.group_m * p.tiles_n), first = grp * p.group_m;
+    const int gm  = min(p.group_m, p.tiles_m - first);
+    const int rr  = r - first * p.tiles_n;
+    t.m0          = (first + rr % gm) * 256;
+    t.n0          = rr / gm * (EPI == EPI_PLAIN ? 256 : 128);
+    return t;
+}
+
+// Sixteen neighbouring results of a row.
+__device__ __forceinline__ void store_run(void* base, int64_t at, tb200_dtype dt, int n, int vec, const float (&v)[16])
+{
+    if (dt == TB200_FP32)
+    {
+        float* o = reinterpret_cast<float*>(base) + at;
+        if (n == 16 && vec == 2)
+        {
+#pragma unroll
+            for (int i = 0; i < 16; i += 8)
+                ptx::st_global_v8(o + i, __float_as_uint(v[i]), __float_as_uint(v[i + 1]), __float_as_uint(v[i + 2]), __float_as_uint(v[i + 3]),
+                                  __float_as_uint(v[i + 4]), __float_as_uint(v[i + 5]), __float_as_uint(v[i + 6]), __float_as_uint(v[i + 7]));
+        }
+        else if (n == 16 && vec == 1)
+        {
+#pragma unroll
+            for (int i = 0; i < 16; i += 4)
+                *reinterpret_cast<float4*>(o + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+        }
+        else
+        {
+#pragma unroll
+            for (int i = 0; i < 16; i++)
+                if (i < n)
+                    o[i] = v[i];
+        }
+        return;
+    }
+    uint32_t h[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+        h[i] = pack2(v[2 * i], v[2 * i + 1], dt == TB200_BF16);
+    uint16_t* o = reinterpret_cast<uint16_t*>(base) + at;
+    if (n == 16 && vec == 2)
+        ptx::st_global_v8(o, h[0], h[1], h[2], h[3], h[4], h[5], h[6], h[7]);
+    else if (n == 16 && vec == 1)
+    {
+        *reinterpret_cast<uint4*>(o)     = make_uint4(h[0], h[1], h[2], h[3]);
+        *reinterpret_cast<uint4*>(o + 8) = make_uint4(h[4], h[5], h[6], h[7]);
+    }
+    else
+    {
+#pragma unroll
+        for (int i = 0; i < 16; i++)
+            if (i < n)
+                o[i] = (uint16_t)((i & 1) ? (h[i >> 1] >> 16) : (h[i >> 1] & 0xffffu));
+    }
+}
+
+template <int ACT>
+__device__ __forceinline__ void gate_run(const uint32_t (&g)[16], const uint32_t (&u)[16], float (&o)[16])
+{
+#pragma unroll
+    for (int i = 0; i < 16; i++)
+        o[i] = act_value<ACT>(__uint_as_float(g[i])) * __uint_as_float(u[i]);
+}
+
+template <int ACT>
+__device__ __forceinline__ void grad_run(const uint32_t (&g)[16], const uint32_t (&u)[16], const float (&d)[16], float (&dg)[16], float (&du)[16])
+{
+#pragma unroll
+    for (int i = 0; i < 16; i++)
+    {
+        float value, slope;
+        act_slope<ACT>(__uint_as_float(g[i]), value, slope);
+        dg[i] = d[i] * __uint_as_float(u[i]) * slope;
+        du[i] = d[i] * value;
+    }
+}
+
+template <int EPI, bool A_MN, bool B_MN>
+__global__ void __launch_bounds__(kThreads, 1) ffn_pair_kernel(const __grid_constant__ Params p)
+{
+    extern __shared__ uint8_t smem_raw[];
+    // identical layout in both CTAs of a pair: remote signals address a barrier by its offset
+    __shared__ __align__(8) uint64_t bar_full[kMaxStages];     // used in the first CTA: bytes of both CTAs
+    __shared__ __align__(8) uint64_t bar_empty[kMaxStages];    // per CTA: stage consumed by the MMAs
+    __shared__ __align__(8) uint64_t bar_tmem_full[2];         // per CTA: accumulator buffer complete
+    __shared__ __align__(8) uint64_t bar_tmem_empty[2];        // first CTA: buffer drained by both CTAs' epilogues
+    __shared__ __align__(8) uint64_t bar_drain;                // first CTA: MMAs in flight when the issuer gives up
+    __shared__ uint32_t tmem_base_holder;
+
+    const int warp           = threadIdx.x >> 5;
+    const int lane           = threadIdx.x & 31;
+    const uint32_t rank      = ptx::cluster_ctarank();
+    const int cluster_id     = blockIdx.x >> 1;
+    const int num_clusters   = gridDim.x >> 1;
+    const uint32_t smem_base = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
+
+    if (threadIdx.x == 0)
+    {
+        for (int s = 0; s < kStages; s++)
+        {
+            ptx::mbar_init(ptx::smem_u32(&bar_full[s]), 1);
+            ptx::mbar_init(ptx::smem_u32(&bar_empty[s]), 1);
+        }
+        for (int a = 0; a < 2; a++)
+        {
+            ptx::mbar_init(ptx::smem_u32(&bar_tmem_full[a]), 1);
+            ptx::mbar_init(ptx::smem_u32(&bar_tmem_empty[a]), 2 * kEpiWarps);
+        }
+        ptx::mbar_init(ptx::smem_u32(&bar_drain), 1);
+        ptx::fence_barrier_init();
+        ptx::prefetch_tmap(&p.tmA);
+        ptx::prefetch_tmap(&p.tmB0);
+        ptx::prefetch_tmap(&p.tmB1);
+    }
+    if (warp == 1)
+    {
+        ptx::tmem_alloc_pair(ptx::smem_u32(&tmem_base_holder), kTmemCols);
+        ptx::tmem_relinquish_pair();
+    }
+    ptx::tc_fence_before_sync();
+    __syncthreads();
+    // no signal may reach the other CTA before its barriers exist
+    ptx::cluster_sync();
+    ptx::tc_fence_after_sync();
+    const uint32_t tmem_base = tmem_base_holder;
+    const int total          = p.chunks * p.phases;
+
+    if (warp == 0)
+    {
+        // ------------------------------------------------------------------ TMA producer (both CTAs)
+        if (lane == 0)
+        {
+            int stage      = 0;
+            uint32_t phase = 0;
+            bool ok        = true;
+            int64_t issued = 0;
+            for (int tile = cluster_id; tile < p.num_tiles && ok; tile += num_clusters)
+            {
+                const Tile t          = decode<EPI>(p, tile);
+                const int m0          = t.m0 + (int)rank * 128;
+                const int n0          = EPI == EPI_PLAIN ? t.n0 + (int)rank * 128 : t.n0;
+                const int batch       = t.idx < p.NB ? t.idx : t.idx - p.NB;
+                const int b_batch     = (A_MN && B_MN) ? t.idx : batch;    // gradients of weights: dG's batches, then dU's
+                for (int left = total, c = 0; left > 0; left -= kSub)
+                {
+                    if (!ptx::mbar_wait_bounded(ptx::smem_u32(&bar_empty[stage]), phase ^ 1u, p.wait_limit))
+                    {
+                        ok = false;
+                        break;
+                    }
+                    const int nch             = min(kSub, left);
+                    const uint32_t full_local = ptx::smem_u32(&bar_full[stage]);
+                    // the first CTA arms the barrier with the bytes of both CTAs; each CTA's copies report there
+                    if (rank == 0)
+                        ptx::mbar_arrive_expect_tx(full_local, (uint32_t)(nch * 4 * kChunk));
+                    const uint32_t full_first = ptx::map_to_cta(full_local, 0);
+                    const uint32_t sA         = smem_base + (uint32_t)(stage * kStage);
+                    const uint32_t sB         = sA + (uint32_t)(kSub * kChunk);
+                    for (int j = 0; j < nch; j++, c++)
+                    {
+                        const int ph      = c >= p.chunks ? 1 : 0;
+                        const int k       = (c - ph * p.chunks) * 64;
+                        const uint32_t dA = sA + (uint32_t)(j * kChunk), dB = sB + (uint32_t)(j * kChunk);
+                        if (A_MN)
+                        {
+                            ptx::tma_load_3d_pair(dA, &p.tmA, full_first, m0, k, batch);
+                            ptx::tma_load_3d_pair(dA + 8192, &p.tmA, full_first, m0 + 64, k, batch);
+                        }
+                        else
+                            ptx::tma_load_3d_pair(dA, &p.tmA, full_first, k, m0, batch + ph * p.NB);
+                        const CUtensorMap* mb = (EPI == EPI_PLAIN ? ph != 0 : rank != 0) ? &p.tmB1 : &p.tmB0;
+                        if (B_MN)
+                        {
+                            ptx::tma_load_3d_pair(dB, mb, full_first, n0, k, b_batch);
+                            ptx::tma_load_3d_pair(dB + 8192, mb, full_first, n0 + 64, k, b_batch);
+                        }
+                        else
+                            ptx::tma_load_3d_pair(dB, mb, full_first, k, n0, b_batch);
+                    }
+                    issued++;
+                    if (++stage == kStages)
+                    {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+            }
+            if (!ok)
+            {
+                atomicOr(p.status, TB200_DEV_TIMEOUT);
+                // the pair's copies in flight land before either CTA leaves (all of them report to the first CTA)
+                if (rank == 0)
+                    for (int64_t i = max((int64_t)0, issued - kStages); i < issued; i++)
+                        ptx::mbar_wait_bounded(ptx::smem_u32(&bar_full[i % kStages]), (uint32_t)(i / kStages) & 1u, p.wait_limit);
+            }
+        }
+    }
+    else if (warp == 1)
+    {
+        // ------------------------------------------------------------------ MMA issuer (first CTA of the pair)
+        if (lane == 0 && rank == 0)
+        {
+            int stage      = 0;
+            uint32_t phase = 0;
+            int acc        = 0;
+            uint32_t acc_phase = 0;
+            bool ok            = true;
+            for (int tile = cluster_id; tile < p.num_tiles && ok; tile += num_clusters)
+            {
+                if (!ptx::mbar_wait_bounded(ptx::smem_u32(&bar_tmem_empty[acc]), acc_phase ^ 1u, p.wait_limit))
+                {
+                    ok = false;
+                    break;
+                }
+                ptx::tc_fence_after_sync();
+                const uint32_t d_tmem = tmem_base + (uint32_t)(acc * 256);
+                uint32_t accum        = 0;    // the first MMA of a tile overwrites the accumulator
+                for (int left = total; left > 0; left -= kSub)
+                {
+                    if (!ptx::mbar_wait_bounded(ptx::smem_u32(&bar_full[stage]), phase, p.wait_limit))
+                    {
+                        ok = false;
+                        break;
+                    }
+                    ptx::tc_fence_after_sync();
+                    const int nch     = min(kSub, left);
+                    const uint32_t sA = smem_base + (uint32_t)(stage * kStage);
+                    const uint32_t sB = sA + (uint32_t)(kSub * kChunk);
+                    for (int j = 0; j < nch; j++)
+                    {
+                        uint64_t ad = ptx::smem_desc(p.a_desc_hi, sA + (uint32_t)(j * kChunk));
+                        uint64_t bd = ptx::smem_desc(p.b_desc_hi, sB + (uint32_t)(j * kChunk));
+#pragma unroll
+                        for (int m = 0; m < 4; m++)
+                        {
+                            ptx::mma_f16_ss_pair(d_tmem, ad, bd, p.idesc, accum);
+                            accum = 1;
+                            // sixteen elements of K: 32 bytes inside the swizzled row, or sixteen rows of 128 bytes
+                            ad += A_MN ? 128 : 2;
+                            bd += B_MN ? 128 : 2;
+                        }
+                    }
+                    // frees the stage in both CTAs once the MMAs above have read it
+                    ptx::mma_commit_pair(ptx::smem_u32(&bar_empty[stage]), 3);
+                    if (++stage == kStages)
+                    {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+                if (!ok)
+                    break;
+                ptx::mma_commit_pair(ptx::smem_u32(&bar_tmem_full[acc]), 3);
+                acc ^= 1;
+                if (acc == 0)
+                    acc_phase ^= 1u;
+            }
+            if (!ok)
+            {
+                atomicOr(p.status, TB200_DEV_TIMEOUT);
+                ptx::mma_commit_pair(ptx::smem_u32(&bar_drain), 1);
+                ptx::mbar_wait_bounded(ptx::smem_u32(&bar_drain), 0, p.wait_limit);
+            }
+        }
+    }
+    else
+    {
+        // ------------------------------------------------------------------ epilogue warps (both CTAs)
+        const int quarter = warp & 3;           // TMEM lane quarter this warp may read
+        const int slot    = (warp - 2) >> 2;    // the two warps of a quarter take 16-column runs in turn
+        const int row     = quarter * 32 + lane;
+        const uint32_t empty_first[2] = { ptx::map_to_cta(ptx::smem_u32(&bar_tmem_empty[0]), 0),
+                                          ptx::map_to_cta(ptx::smem_u32(&bar_tmem_empty[1]), 0) };
+        int acc            = 0;
+        uint32_t acc_phase = 0;
+        bool ok            = true;
+        for (int tile = cluster_id; tile < p.num_tiles; tile += num_clusters)
+        {
+            const Tile t = decode<EPI>(p, tile);
+            ok           = ptx::mbar_wait_bounded(ptx::smem_u32(&bar_tmem_full[acc]), acc_phase, p.wait_limit);
+            // the whole warp must agree before the warp-collective TMEM loads
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok)
+                break;
+            ptx::tc_fence_after_sync();
+            const int m          = t.m0 + (int)rank * 128 + row;
+            const bool row_valid = m < p.rows;
+            const int batch      = t.idx < p.NB ? t.idx : t.idx - p.NB;
+            const int64_t orow   = ((int64_t)batch * p.rows + m) * p.ld;
+            const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(acc * 256);
+            if (EPI == EPI_PLAIN)
+            {
+                void* const out      = t.idx < p.NB ? p.out0 : p.out1;
+                const tb200_dtype dt = t.idx < p.NB ? p.out_dt : p.out1_dt;
+                for (int c = slot; c < 16; c += 2)
+                {
+                    const int col = t.n0 + c * 16;
+                    if (col >= p.cols)
+                        break;
+                    uint32_t g[16];
+                    ptx::tmem_ld_32x32b_x16(taddr + (uint32_t)(c * 16), g);
+                    ptx::tmem_ld_wait_x16(g);
+                    if (!row_valid)
+                        continue;
+                    float v[16];
+#pragma unroll
+                    for (int i = 0; i < 16; i++)
+                        v[i] = __uint_as_float(g[i]);
+                    store_run(out, orow + col, dt, min(16, p.cols - col), p.vec, v);
+                }
+            }
+            else
+            {
+                for (int c = slot; c < 8; c += 2)
+                {
+                    const int col = t.n0 + c * 16;
+                    if (col >= p.cols)
+                        break;
+                    const int n = min(16, p.cols - col);
+                    uint32_t g[16], u[16];
+                    ptx::tmem_ld_32x32b_x16(taddr + (uint32_t)(c * 16), g);
+                    ptx::tmem_ld_32x32b_x16(taddr + (uint32_t)(128 + c * 16), u);
+                    float d[16];
+                    if (EPI == EPI_GRAD)
+                    {
+                        const int64_t at = ((int64_t)batch * p.rows + m) * p.cols + col;
+                        const uint16_t* s = reinterpret_cast<const uint16_t*>(p.dout) + at;
+                        if (row_valid && n == 16 && p.dout_vec)
+                        {
+                            const uint4 lo = __ldg(reinterpret_cast<const uint4*>(s)), hi = __ldg(reinterpret_cast<const uint4*>(s) + 1);
+                            const uint32_t w[8] = { lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w };
+#pragma unroll
+                            for (int i = 0; i < 8; i++)
+                            {
+                                const float2 f = unpack2(w[i], p.bf16 != 0);
+                                d[2 * i]       = f.x;
+                                d[2 * i + 1]   = f.y;
+                            }
+                        }
+                        else
+                        {
+#pragma unroll
+                            for (int i = 0; i < 16; i++)
+                                d[i] = row_valid && i < n ? unpack2(s[i], p.bf16 != 0).x : 0.f;
+                        }
+                    }
+                    ptx::tmem_ld_wait_x16(g);
+                    ptx::tmem_ld_wait_x16(u);
+                    if (!row_valid)
+                        continue;
+                    if (EPI == EPI_GATED)
+                    {
+                        float v[16];
+                        switch (p.act)
+                        {
+                            case TB200_ACT_SILU: gate_run<TB200_ACT_SILU>(g, u, v); break;
+                            case TB200_ACT_GELU: gate_run<TB200_ACT_GELU>(g, u, v); break;
+                            case TB200_ACT_GELU_TANH: gate_run<TB200_ACT_GELU_TANH>(g, u, v); break;
+                            case TB200_ACT_RELU: gate_run<TB200_ACT_RELU>(g, u, v); break;
+                            default: gate_run<TB200_ACT_SIGMOID>(g, u, v); break;
+                        }
+                        store_run(p.out0, orow + col, p.out_dt, n, p.vec, v);
+                    }
+                    else
+                    {
+                        float dg[16], du[16];
+                        switch (p.act)
+                        {
+                            case TB200_ACT_SILU: grad_run<TB200_ACT_SILU>(g, u, d, dg, du); break;
+                            case TB200_ACT_GELU: grad_run<TB200_ACT_GELU>(g, u, d, dg, du); break;
+                            case TB200_ACT_GELU_TANH: grad_run<TB200_ACT_GELU_TANH>(g, u, d, dg, du); break;
+                            case TB200_ACT_RELU: grad_run<TB200_ACT_RELU>(g, u, d, dg, du); break;
+                            default: grad_run<TB200_ACT_SIGMOID>(g, u, d, dg, du); break;
+                        }
+                        store_run(p.out0, orow + col, p.out_dt, n, p.vec, dg);
+                        store_run(p.out1, orow + col, p.out_dt, n, p.vec, du);
+                    }
+                }
+            }
+            // this warp has read its part of the buffer: one arrival per warp on the first CTA's barrier
+            ptx::tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0)
+                ptx::mbar_arrive_cluster(empty_first[acc]);
+            acc ^= 1;
+            if (acc == 0)
+                acc_phase ^= 1u;
+        }
+        if (!ok && lane == 0)
+            atomicOr(p.status, TB200_DEV_TIMEOUT);
+    }
+
+    // ---------------------------------------------------------------------- teardown
+    // Neither CTA may leave (or free its TMEM) while the other can still signal it or read its shared memory.
+    ptx::tc_fence_before_sync();
+    __syncthreads();
+    ptx::cluster_sync();
+    if (warp == 1)
+    {
+        ptx::tc_fence_after_sync();
+        ptx::tmem_dealloc_pair(tmem_base, kTmemCols);
+    }
+}
+
+typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// A [batches][outer][inner] operand of 16-bit elements with rows `pitch` elements apart: K along its rows (boxes of 64 x 128), or
+// across them (64 x 64, two for each half tile).  What lies outside reads as zero.
+tb200_status encode(tb200_ctx* ctx, CUtensorMap* m, const Matrix& x, bool bf16, bool k_inner)
+{
+    const EncodeTiled enc = reinterpret_cast<EncodeTiled>(tensor_map_encode_fn());
+    if (!enc)
+        return fail(ctx, TB200_INTERNAL, "cuTensorMapEncodeTiled is not available from the driver");
+    const cuuint64_t dims[3]    = { (cuuint64_t)x.inner, (cuuint64_t)x.outer, (cuuint64_t)x.batches };
+    const cuuint64_t strides[2] = { (cuuint64_t)x.pitch * 2, (cuuint64_t)x.pitch * (cuuint64_t)x.outer * 2 };
+    const cuuint32_t box[3]     = { 64, k_inner ? 128u : 64u, 1 };
+    const cuuint32_t estr[3]    = { 1, 1, 1 };
+    const CUresult r = enc(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(x.data), dims, strides, box,
+                           estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS)
+        return fail(ctx, TB200_INTERNAL, "tensor map of a feed-forward product rejected (CUresult %d)", (int)r);
+    return TB200_OK;
+}
+
+int run_alignment(const void* p, int64_t ld, size_t es)
+{
+    const uintptr_t bits = reinterpret_cast<uintptr_t>(p) | (uintptr_t)(ld * (int64_t)es);
+    return (bits & 31) == 0 ? 2 : (bits & 15) == 0 ? 1 : 0;
+}
+
+}    // namespace
+
+tb200_status pair_launch(tb200_ctx* ctx, const PairProduct& q)
+{
+    Params k;
+    memset(&k, 0, sizeof(k));
+    const bool bf16 = q.dt == TB200_BF16;
+    const bool gated = q.kind != PAIR_PLAIN;
+    tb200_status st  = encode(ctx, &k.tmA, q.a, bf16, !q.a_mn);
+    if (st == TB200_OK)
+        st = encode(ctx, &k.tmB0, q.b[0], bf16, !q.b_mn);
+    if (st == TB200_OK)
+        st = encode(ctx, &k.tmB1, q.b[1].data ? q.b[1] : q.b[0], bf16, !q.b_mn);
+    if (st != TB200_OK)
+        return st;
+    k.rows      = q.rows;
+    k.cols      = q.cols;
+    k.tiles_m   = (q.rows + 255) / 256;
+    k.tiles_n   = gated ? (q.cols + 127) / 128 : (q.cols + 255) / 256;
+    k.NB        = q.NB;
+    const int64_t tiles = (int64_t)k.tiles_m * k.tiles_n * q.NB * (q.results == 2 && !gated ? 2 : 1);
+    if (tiles > (1 << 30))
+        return fail(ctx, TB200_ERROR, "a feed-forward product of %lld tiles is too large", (long long)tiles);
+    k.num_tiles = (int)tiles;
+    // A's rows of a group, about 32 MB, stay in L2
+    const int64_t a_tile = 256LL * q.K * q.phases * 2;
+    k.group_m  = (int)std::max<int64_t>(1, std::min<int64_t>(k.tiles_m, (32LL << 20) / std::max<int64_t>(1, a_tile)));
+    k.chunks   = (int)((q.K + 63) / 64);
+    k.phases   = q.phases;
+    k.act      = q.act;
+    k.bf16     = bf16 ? 1 : 0;
+    k.out_dt   = q.out_dt[0];
+    k.out1_dt  = q.out_dt[1];
+    k.out0     = q.out[0];
+    k.out1     = q.out[1];
+    k.ld       = q.ld;
+    k.vec      = q.out[0] ? run_alignment(q.out[0], q.ld, dtype_size(q.out_dt[0])) : 2;
+    if (q.out[1])
+        k.vec = std::min(k.vec, run_alignment(q.out[1], q.ld, dtype_size(q.out_dt[1])));
+    k.dout     = q.dout;
+    k.dout_vec = q.dout && run_alignment(q.dout, q.cols, 2) > 0;
+    // K along the rows: 8-row groups of 128-byte swizzled rows 1024 bytes apart.  Across them: 64 columns of 64 K rows, the second
+    // half's 8192 bytes behind.
+    k.a_desc_hi  = q.a_mn ? ptx::make_smem_desc_hi(8192, 1024, 2) : ptx::make_smem_desc_hi(16, 1024, 2);
+    k.b_desc_hi  = q.b_mn ? ptx::make_smem_desc_hi(8192, 1024, 2) : ptx::make_smem_desc_hi(16, 1024, 2);
+    const uint32_t fmt = bf16 ? 1u : 0u;
+    k.idesc      = ptx::make_idesc(1u, fmt, fmt, q.a_mn ? 1u : 0u, q.b_mn ? 1u : 0u, 256u, 256u);
+    k.wait_limit = ctx->wait_limit_cycles;
+    k.status     = ctx->d_status;
+
+    void (*kern)(const Params) = nullptr;
+    int bit                    = 0;
+    if (q.kind == PAIR_GATED && !q.a_mn)
+    {
+        kern = q.b_mn ? ffn_pair_kernel<EPI_GATED, false, true> : ffn_pair_kernel<EPI_GATED, false, false>;
+        bit  = q.b_mn ? 0 : 1;
+    }
+    else if (q.kind == PAIR_GRAD && !q.a_mn && q.b_mn)
+    {
+        kern = ffn_pair_kernel<EPI_GRAD, false, true>;
+        bit  = 2;
+    }
+    else if (q.kind == PAIR_PLAIN && q.a_mn == q.b_mn)
+    {
+        kern = q.a_mn ? ffn_pair_kernel<EPI_PLAIN, true, true> : ffn_pair_kernel<EPI_PLAIN, false, false>;
+        bit  = q.a_mn ? 3 : 4;
+    }
+    if (!kern)
+        return fail(ctx, TB200_INTERNAL, "no kernel for this feed-forward product");
+    st = raise_smem_limit(ctx, 128 + bit, reinterpret_cast<const void*>(kern), kSmem);
+    if (st != TB200_OK)
+        return st;
+    cudaLaunchConfig_t cfg = {};
+    cfg.blockDim           = dim3(kThreads);
+    cfg.dynamicSmemBytes   = (size_t)kSmem;
+    cfg.stream             = ctx->stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id               = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs    = attr;
+    cfg.numAttrs = 1;
+    cfg.gridDim  = dim3((unsigned)(2 * std::max(1, std::min(k.num_tiles, ctx->num_sms / 2))));
+    timer_begin(ctx);
+    const cudaError_t le = cudaLaunchKernelEx(&cfg, kern, k);
+    timer_end(ctx);
+    if (le != cudaSuccess)
+        return fail(ctx, TB200_INTERNAL, "launch of a feed-forward product failed: %s", cudaGetErrorString(le));
+    return post_launch(ctx, q.name);
+}
+
+}    // namespace ffn
+}    // namespace tb200
