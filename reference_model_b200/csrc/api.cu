@@ -383,6 +383,8 @@ extern "C" tb200_status tb200_ctx_destroy(tb200_ctx* ctx)
         cudaFree(ctx->join_table);
     if (ctx->pair_flags)
         cudaFree(ctx->pair_flags);
+    if (ctx->ffn_count)
+        cudaFree(ctx->ffn_count);
     if (ctx->pipe.ready)
     {
         cudaStreamSynchronize(ctx->pipe.h2d);

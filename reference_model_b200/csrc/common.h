@@ -149,6 +149,8 @@ struct tb200_ctx
     uint32_t* pair_flags = nullptr;    // flags of the CTA-pair MATMUL's in-kernel zero-point sums, zeroed when allocated
     size_t pair_flag_words = 0;
     uint32_t pair_epoch  = 0;          // bumped per launch; a flag equal to it means "written in this launch"
+    int* ffn_count       = nullptr;    // arrivals at shared tiles of 4-bit products; zero whenever none runs
+    int ffn_counts       = 0;
     void* stage          = nullptr;    // grow-on-demand staging of TRANSPOSE_CONV2D (spread input, mirrored weights)
     size_t stage_bytes   = 0;
     void* io_pinned      = nullptr;    // 64 MiB pinned host buffer of the .npy loader / writer, allocated on first use

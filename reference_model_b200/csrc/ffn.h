@@ -19,6 +19,7 @@ struct W4Mat
     const void* scale;
     const int8_t* zero;    // or null
     tb200_dtype scale_dt;
+    int64_t scale_pitch, zero_pitch;    // elements from one group's to the next
 };
 
 struct W4Problem
@@ -97,8 +98,9 @@ tb200_status gated_rows_launch(tb200_ctx* ctx, const PairProduct& q);
 
 // ---- w4_rows.cu: up to 64 16-bit rows against 4-bit weights
 // x: a's rows in 16 bits, `x_pitch` elements apart (a multiple of 8), 16-byte aligned; fp32 rows as three bf16 rows each (parts 3,
-// bf16).  The weights' pitch is a multiple of 16 bytes.
-tb200_status w4_rows_launch(tb200_ctx* ctx, const W4Problem& q, const void* x, int64_t x_pitch, int parts, bool bf16);
+// bf16).  The pitches of the weights, scales and zero points are multiples of 16 bytes.
+tb200_status w4_rows_launch(tb200_ctx* ctx, const W4Problem& q, const void* x, int64_t x_pitch, int parts, bool bf16, float* partial);
+size_t w4_rows_partial_bytes(const tb200_ctx* ctx, int64_t xrows);
 
 // ---- ffn_small.cu: copies
 // fp32 rows to three bf16 rows each whose sum they are, rows `pitch` apart

@@ -60,11 +60,11 @@ template <bool BF16>
 __device__ __forceinline__ void few_mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
 {
     if (BF16)
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
     else
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -113,11 +113,11 @@ __global__ void __launch_bounds__(kFewThreads) gated_rows_kernel(const __grid_co
         if (lane == 0)
         {
             bool ok = true;
-            int i   = 0;
+            int i = 0, s = 0;
+            uint32_t phase = 0;
             for (; i < mine; i++)
             {
-                const int s = i % p.num_stages;
-                if (!ptx::mbar_wait_bounded(ptx::smem_u32(&bar_empty[s]), ((uint32_t)(i / p.num_stages) & 1u) ^ 1u, p.wait_limit))
+                if (!ptx::mbar_wait_bounded(ptx::smem_u32(&bar_empty[s]), phase ^ 1u, p.wait_limit))
                 {
                     ok = false;
                     break;
@@ -133,6 +133,11 @@ __global__ void __launch_bounds__(kFewThreads) gated_rows_kernel(const __grid_co
                     ptx::tma_load_3d(sW + (uint32_t)(j * 8192), &p.tmG, full, col0, k + j * 64, batch);
                     ptx::tma_load_3d(sW + (uint32_t)(16384 + j * 8192), &p.tmU, full, col0, k + j * 64, batch);
                     ptx::tma_load_3d(sX + (uint32_t)(j * 8 * NT * 128), &p.tmX, full, k + j * 64, row0, batch);
+                }
+                if (++s == p.num_stages)
+                {
+                    s = 0;
+                    phase ^= 1u;
                 }
             }
             if (!ok)
@@ -150,11 +155,12 @@ __global__ void __launch_bounds__(kFewThreads) gated_rows_kernel(const __grid_co
         const int q = lane >> 3, r = lane & 7;
         const uint32_t aW = (uint32_t)((warp >> 2) * 16384 + ((q >> 1) * 8 + r) * 128) + (uint32_t)(((piece0 + (q & 1)) ^ r) << 4);
         bool ok = true;
+        int s = 0;
+        uint32_t phase = 0;
         for (int i = 0; i < mine; i++)
         {
-            const int s = i % p.num_stages;
-            ok          = ptx::mbar_wait_bounded(ptx::smem_u32(&bar_full[s]), (uint32_t)(i / p.num_stages) & 1u, p.wait_limit);
-            ok          = __all_sync(0xffffffffu, ok);
+            ok = ptx::mbar_wait_bounded(ptx::smem_u32(&bar_full[s]), phase, p.wait_limit);
+            ok = __all_sync(0xffffffffu, ok);
             if (!ok)
                 break;
             const uint32_t sW = smem_base + (uint32_t)(s * p.stage_bytes), sX = sW + kFewWBytes;
@@ -185,6 +191,11 @@ __global__ void __launch_bounds__(kFewThreads) gated_rows_kernel(const __grid_co
             __syncwarp();
             if (lane == 0)
                 ptx::mbar_arrive(ptx::smem_u32(&bar_empty[s]));
+            if (++s == p.num_stages)
+            {
+                s = 0;
+                phase ^= 1u;
+            }
         }
         if (!ok && lane == 0)
         {
@@ -229,12 +240,17 @@ __global__ void __launch_bounds__(kFewThreads) gated_rows_kernel(const __grid_co
             if (p.splits > 1)
             {
                 const uint32_t local = ptx::smem_u32(at);
-                for (int r = 0; r < p.splits; r++)
+                float x[8];    // all on their way before the first is added
+#pragma unroll
+                for (int r = 0; r < 8; r++)
                 {
-                    float x;
-                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(ptx::map_to_cta(local, (uint32_t)r)) : "memory");
-                    sum += x;
+                    x[r] = 0.f;
+                    if (r < p.splits)
+                        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x[r]) : "r"(ptx::map_to_cta(local, (uint32_t)r)) : "memory");
                 }
+#pragma unroll
+                for (int r = 0; r < 8; r++)
+                    sum += x[r];
             }
             else
                 sum = *at;
@@ -304,7 +320,7 @@ tb200_status gated_rows_launch(tb200_ctx* ctx, const PairProduct& q)
     const size_t red  = (size_t)8 * nt * kFewRedLd * sizeof(float);
     const size_t smem = std::max((size_t)p.num_stages * p.stage_bytes, red) + 1024;
     const FewKern kern = bf16 ? pick<true>(nt) : pick<false>(nt);
-    st = raise_smem_limit(ctx, 160 + (nt == 8 ? 3 : nt / 2) * 2 + (bf16 ? 1 : 0), reinterpret_cast<const void*>(kern), (int)smem);
+    st = raise_smem_limit(ctx, 168 + (nt == 8 ? 3 : nt / 2) * 2 + (bf16 ? 1 : 0), reinterpret_cast<const void*>(kern), (int)smem);
     if (st != TB200_OK)
         return st;
     cudaLaunchConfig_t cfg = {};

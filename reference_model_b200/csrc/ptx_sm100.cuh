@@ -145,6 +145,18 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* m, 
         : "memory");
 }
 
+// Tiles on their way from memory to L2 (no copy to shared memory, nothing to wait for)
+__device__ __forceinline__ void prefetch_2d(const CUtensorMap* m, int c0, int c1)
+{
+    asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(reinterpret_cast<uint64_t>(m)), "r"(c0), "r"(c1) : "memory");
+}
+
+__device__ __forceinline__ void prefetch_3d(const CUtensorMap* m, int c0, int c1, int c2)
+{
+    asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global.tile [%0, {%1, %2, %3}];" ::"l"(reinterpret_cast<uint64_t>(m)), "r"(c0), "r"(c1), "r"(c2)
+                 : "memory");
+}
+
 // im2col mode, [N][H][W][C] maps: consecutive pixels of the map's box from (w, h, n) on, each displaced by the tap offsets
 __device__ __forceinline__ void tma_load_im2col_4d(uint32_t dst, const CUtensorMap* m, uint32_t bar, int c, int w, int h, int n,
                                                    uint16_t off_w, uint16_t off_h)
