@@ -26,15 +26,23 @@ namespace ffn
 namespace
 {
 
-constexpr int kEpiWarps  = 8;
-constexpr int kThreads   = 64 + 32 * kEpiWarps;    // TMA warp, MMA warp, epilogue
-constexpr int kMaxStages = 4;
-constexpr int kChunk     = 16384;    // 128 rows (or columns) x 64 elements of K
-constexpr int kSub       = 2;        // chunks per stage
-constexpr int kStage     = 2 * kSub * kChunk;
-constexpr int kSmem      = 3 * kStage + 1024;
-constexpr int kStages    = 3;
-constexpr int kTmemCols  = 512;
+constexpr int kEpiWarps = 8;
+constexpr int kThreads  = 64 + 32 * kEpiWarps;    // TMA warp, MMA warp, epilogue
+constexpr int kChunk    = 16384;                  // 128 rows (or columns) x 64 elements of K
+
+// Pairs of CTAs (PAIR) with tiles of 256 rows and 256 accumulator columns, or CTAs by themselves with 128 x 128; one CTA to an SM.
+template <bool PAIR>
+struct Shape
+{
+    static constexpr int kStages = PAIR ? 3 : 6;
+    static constexpr int kCtas = PAIR ? 2 : 1;
+    static constexpr int kRows = 128 * kCtas, kCols = PAIR ? 256 : 128;    // of a tile
+    static constexpr int kSub  = PAIR ? 2 : 1;                             // chunks per stage
+    static constexpr int kStage = 2 * kSub * kChunk;                       // each CTA holds 128 rows of A and 128 columns of B
+    static constexpr int kSmem  = kStages * kStage + 1024;
+    static constexpr int kTmemCols = 2 * kCols;
+    static constexpr int kRedLd    = kCols + 4;    // row pitch of a tile's sums in shared memory: a warp's stores meet every bank
+};
 
 enum : int
 {
@@ -49,6 +57,7 @@ struct Params
     int rows, cols;    // of a result matrix
     int tiles_m, tiles_n, num_tiles, group_m;
     int chunks, phases;    // K chunks of a phase
+    int splits;            // CTAs of a cluster that share a tile's K (CTAs by themselves only)
     int NB;                // batches of A's and B's own
     int act, bf16;
     tb200_dtype out_dt;
@@ -69,7 +78,7 @@ struct Tile
     int idx, m0, n0;
 };
 
-template <int EPI>
+template <int EPI, bool PAIR>
 __device__ __forceinline__ Tile decode(const Params& p, int tile)
 {
     const int per = p.tiles_m * p.tiles_n;
@@ -79,8 +88,8 @@ __device__ __forceinline__ Tile decode(const Params& p, int tile)
     const int grp = r / (p.group_m * p.tiles_n), first = grp * p.group_m;
     const int gm  = min(p.group_m, p.tiles_m - first);
     const int rr  = r - first * p.tiles_n;
-    t.m0          = (first + rr % gm) * 256;
-    t.n0          = rr / gm * (EPI == EPI_PLAIN ? 256 : 128);
+    t.m0          = (first + rr % gm) * Shape<PAIR>::kRows;
+    t.n0          = rr / gm * (EPI == EPI_PLAIN ? Shape<PAIR>::kCols : Shape<PAIR>::kCols / 2);
     return t;
 }
 
@@ -138,7 +147,7 @@ __device__ __forceinline__ void gate_run(const uint32_t (&g)[16], const uint32_t
 {
 #pragma unroll
     for (int i = 0; i < 16; i++)
-        o[i] = act_value<ACT>(__uint_as_float(g[i])) * __uint_as_float(u[i]);
+        o[i] = act_value_16<ACT>(__uint_as_float(g[i])) * __uint_as_float(u[i]);
 }
 
 template <int ACT>
@@ -148,30 +157,102 @@ __device__ __forceinline__ void grad_run(const uint32_t (&g)[16], const uint32_t
     for (int i = 0; i < 16; i++)
     {
         float value, slope;
-        act_slope<ACT>(__uint_as_float(g[i]), value, slope);
+        act_slope_16<ACT>(__uint_as_float(g[i]), value, slope);
         dg[i] = d[i] * __uint_as_float(u[i]) * slope;
         du[i] = d[i] * value;
     }
 }
 
-template <int EPI, bool A_MN, bool B_MN>
+// Sixteen neighbouring columns of a row of the tile, all sums there: results, activated and multiplied, or the two gradients.
+template <int EPI>
+__device__ __forceinline__ void finish_run(const Params& p, const Tile& t, int row, int run, const uint32_t (&g)[16], const uint32_t (&u)[16])
+{
+    const int m = t.m0 + row, col = t.n0 + run, n = min(16, p.cols - col);
+    if (m >= p.rows)
+        return;
+    const int batch    = t.idx < p.NB ? t.idx : t.idx - p.NB;
+    const int64_t orow = ((int64_t)batch * p.rows + m) * p.ld;
+    if (EPI == EPI_PLAIN)
+    {
+        float v[16];
+#pragma unroll
+        for (int i = 0; i < 16; i++)
+            v[i] = __uint_as_float(g[i]);
+        store_run(t.idx < p.NB ? p.out0 : p.out1, orow + col, t.idx < p.NB ? p.out_dt : p.out1_dt, n, p.vec, v);
+    }
+    else if (EPI == EPI_GATED)
+    {
+        float v[16];
+        switch (p.act)
+        {
+            case TB200_ACT_SILU: gate_run<TB200_ACT_SILU>(g, u, v); break;
+            case TB200_ACT_GELU: gate_run<TB200_ACT_GELU>(g, u, v); break;
+            case TB200_ACT_GELU_TANH: gate_run<TB200_ACT_GELU_TANH>(g, u, v); break;
+            case TB200_ACT_RELU: gate_run<TB200_ACT_RELU>(g, u, v); break;
+            default: gate_run<TB200_ACT_SIGMOID>(g, u, v); break;
+        }
+        store_run(p.out0, orow + col, p.out_dt, n, p.vec, v);
+    }
+    else
+    {
+        float d[16], dg[16], du[16];
+        const uint16_t* const s = reinterpret_cast<const uint16_t*>(p.dout) + ((int64_t)batch * p.rows + m) * p.cols + col;
+        if (n == 16 && p.dout_vec)
+        {
+            const uint4 lo = *reinterpret_cast<const uint4*>(s), hi = *(reinterpret_cast<const uint4*>(s) + 1);
+            const uint32_t w[8] = { lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w };
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+            {
+                const float2 f = unpack2(w[i], p.bf16 != 0);
+                d[2 * i]       = f.x;
+                d[2 * i + 1]   = f.y;
+            }
+        }
+        else
+        {
+#pragma unroll
+            for (int i = 0; i < 16; i++)
+                d[i] = i < n ? unpack2(s[i], p.bf16 != 0).x : 0.f;
+        }
+        switch (p.act)
+        {
+            case TB200_ACT_SILU: grad_run<TB200_ACT_SILU>(g, u, d, dg, du); break;
+            case TB200_ACT_GELU: grad_run<TB200_ACT_GELU>(g, u, d, dg, du); break;
+            case TB200_ACT_GELU_TANH: grad_run<TB200_ACT_GELU_TANH>(g, u, d, dg, du); break;
+            case TB200_ACT_RELU: grad_run<TB200_ACT_RELU>(g, u, d, dg, du); break;
+            default: grad_run<TB200_ACT_SIGMOID>(g, u, d, dg, du); break;
+        }
+        store_run(p.out0, orow + col, p.out_dt, n, p.vec, dg);
+        store_run(p.out1, orow + col, p.out_dt, n, p.vec, du);
+    }
+}
+
+template <int EPI, bool A_MN, bool B_MN, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1) ffn_pair_kernel(const __grid_constant__ Params p)
 {
+    using S               = Shape<PAIR>;
+    constexpr int kSub    = S::kSub, kStage = S::kStage, kHalf = S::kCols / 2, kStages = S::kStages;
     extern __shared__ uint8_t smem_raw[];
     // identical layout in both CTAs of a pair: remote signals address a barrier by its offset
-    __shared__ __align__(8) uint64_t bar_full[kMaxStages];     // used in the first CTA: bytes of both CTAs
-    __shared__ __align__(8) uint64_t bar_empty[kMaxStages];    // per CTA: stage consumed by the MMAs
+    __shared__ __align__(8) uint64_t bar_full[kStages];     // used in the first CTA: bytes of both CTAs
+    __shared__ __align__(8) uint64_t bar_empty[kStages];    // per CTA: stage consumed by the MMAs
     __shared__ __align__(8) uint64_t bar_tmem_full[2];         // per CTA: accumulator buffer complete
     __shared__ __align__(8) uint64_t bar_tmem_empty[2];        // first CTA: buffer drained by both CTAs' epilogues
+    __shared__ __align__(8) uint64_t bar_ready;                // first CTA: tensor memory taken in both
     __shared__ __align__(8) uint64_t bar_drain;                // first CTA: MMAs in flight when the issuer gives up
     __shared__ uint32_t tmem_base_holder;
 
     const int warp           = threadIdx.x >> 5;
     const int lane           = threadIdx.x & 31;
-    const uint32_t rank      = ptx::cluster_ctarank();
-    const int cluster_id     = blockIdx.x >> 1;
-    const int num_clusters   = gridDim.x >> 1;
+    const uint32_t rank      = PAIR ? ptx::cluster_ctarank() : 0;
+    const int cluster_id     = PAIR ? blockIdx.x / 2 : blockIdx.x / (unsigned)p.splits;
+    const int num_clusters   = PAIR ? gridDim.x / 2 : gridDim.x / (unsigned)p.splits;
+    const int share          = !PAIR && p.splits > 1 ? (int)ptx::cluster_ctarank() : 0;    // of K
+    const int chunk0         = share * (p.chunks * p.phases) / p.splits;
+    const int total          = (share + 1) * (p.chunks * p.phases) / p.splits - chunk0;    // chunks of this CTA (pair)
     const uint32_t smem_base = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
+    float* const red         = reinterpret_cast<float*>(smem_raw + (smem_base - ptx::smem_u32(smem_raw)));    // a share's sums of a tile
 
     if (threadIdx.x == 0)
     {
@@ -183,26 +264,66 @@ __global__ void __launch_bounds__(kThreads, 1) ffn_pair_kernel(const __grid_cons
         for (int a = 0; a < 2; a++)
         {
             ptx::mbar_init(ptx::smem_u32(&bar_tmem_full[a]), 1);
-            ptx::mbar_init(ptx::smem_u32(&bar_tmem_empty[a]), 2 * kEpiWarps);
+            ptx::mbar_init(ptx::smem_u32(&bar_tmem_empty[a]), S::kCtas * kEpiWarps);
         }
         ptx::mbar_init(ptx::smem_u32(&bar_drain), 1);
+        ptx::mbar_init(ptx::smem_u32(&bar_ready), S::kCtas);
         ptx::fence_barrier_init();
         ptx::prefetch_tmap(&p.tmA);
         ptx::prefetch_tmap(&p.tmB0);
         ptx::prefetch_tmap(&p.tmB1);
+        // the first weights on their way to L2, where a write by the kernel before would still find them
+        if (EPI != EPI_PLAIN && cluster_id < p.num_tiles)
+        {
+            const Tile t = decode<EPI, PAIR>(p, cluster_id);
+            for (int c = chunk0; c < min(p.chunks, chunk0 + min(total, kStages * kSub)); c++)
+                for (int m = PAIR ? (int)rank : 0; m < (PAIR ? (int)rank + 1 : 2); m++)
+                {
+                    const CUtensorMap* const b = m ? &p.tmB1 : &p.tmB0;
+                    if (!B_MN)
+                        ptx::prefetch_3d(b, c * 64, t.n0, t.idx);
+                    else
+                        for (int n = 0; n < kHalf; n += 64)
+                            ptx::prefetch_3d(b, t.n0 + n, c * 64, t.idx);
+                }
+        }
     }
-    if (warp == 1)
-    {
-        ptx::tmem_alloc_pair(ptx::smem_u32(&tmem_base_holder), kTmemCols);
-        ptx::tmem_relinquish_pair();
-    }
-    ptx::tc_fence_before_sync();
-    __syncthreads();
     // no signal may reach the other CTA before its barriers exist
-    ptx::cluster_sync();
-    ptx::tc_fence_after_sync();
-    const uint32_t tmem_base = tmem_base_holder;
-    const int total          = p.chunks * p.phases;
+    if (PAIR)
+        ptx::cluster_sync();
+    else
+        __syncthreads();
+    // Everything a kernel before this one may have written is read behind this wait, and nothing is written before it.  Tensor memory
+    // is taken behind it too, and the next kernel let in only then: neither kernel can keep the other from columns it waits for.
+    ptx::dep_launch_wait();
+    uint32_t tmem_base = 0;
+    if (warp != 0)
+    {
+        if (warp == 1)
+        {
+            if (PAIR)
+            {
+                ptx::tmem_alloc_pair(ptx::smem_u32(&tmem_base_holder), S::kTmemCols);
+                ptx::tmem_relinquish_pair();
+            }
+            else
+            {
+                ptx::tmem_alloc(ptx::smem_u32(&tmem_base_holder), S::kTmemCols);
+                ptx::tmem_relinquish();
+            }
+            if (lane == 0)
+            {
+                if (PAIR)
+                    ptx::mbar_arrive_cluster(ptx::map_to_cta(ptx::smem_u32(&bar_ready), 0));
+                ptx::dep_launch_trigger();
+            }
+        }
+        // all but the TMA warp, whose copies are on their way by now
+        ptx::tc_fence_before_sync();
+        asm volatile("bar.sync 1, %0;" ::"n"(kThreads - 32) : "memory");
+        ptx::tc_fence_after_sync();
+        tmem_base = tmem_base_holder;
+    }
 
     if (warp == 0)
     {
@@ -215,12 +336,12 @@ __global__ void __launch_bounds__(kThreads, 1) ffn_pair_kernel(const __grid_cons
             int64_t issued = 0;
             for (int tile = cluster_id; tile < p.num_tiles && ok; tile += num_clusters)
             {
-                const Tile t          = decode<EPI>(p, tile);
+                const Tile t          = decode<EPI, PAIR>(p, tile);
                 const int m0          = t.m0 + (int)rank * 128;
-                const int n0          = EPI == EPI_PLAIN ? t.n0 + (int)rank * 128 : t.n0;
+                const int n0          = EPI == EPI_PLAIN ? t.n0 + (int)rank * 128 : t.n0;    // of the CTA's 128 columns, or of each matrix's
                 const int batch       = t.idx < p.NB ? t.idx : t.idx - p.NB;
                 const int b_batch     = (A_MN && B_MN) ? t.idx : batch;    // gradients of weights: dG's batches, then dU's
-                for (int left = total, c = 0; left > 0; left -= kSub)
+                for (int left = total, c = chunk0; left > 0; left -= kSub)
                 {
                     if (!ptx::mbar_wait_bounded(ptx::smem_u32(&bar_empty[stage]), phase ^ 1u, p.wait_limit))
                     {
@@ -231,8 +352,8 @@ __global__ void __launch_bounds__(kThreads, 1) ffn_pair_kernel(const __grid_cons
                     const uint32_t full_local = ptx::smem_u32(&bar_full[stage]);
                     // the first CTA arms the barrier with the bytes of both CTAs; each CTA's copies report there
                     if (rank == 0)
-                        ptx::mbar_arrive_expect_tx(full_local, (uint32_t)(nch * 4 * kChunk));
-                    const uint32_t full_first = ptx::map_to_cta(full_local, 0);
+                        ptx::mbar_arrive_expect_tx(full_local, (uint32_t)(nch * 2 * S::kCtas * kChunk));
+                    const uint32_t full_first = PAIR ? ptx::map_to_cta(full_local, 0) : full_local;
                     const uint32_t sA         = smem_base + (uint32_t)(stage * kStage);
                     const uint32_t sB         = sA + (uint32_t)(kSub * kChunk);
                     for (int j = 0; j < nch; j++, c++)
@@ -240,21 +361,42 @@ __global__ void __launch_bounds__(kThreads, 1) ffn_pair_kernel(const __grid_cons
                         const int ph      = c >= p.chunks ? 1 : 0;
                         const int k       = (c - ph * p.chunks) * 64;
                         const uint32_t dA = sA + (uint32_t)(j * kChunk), dB = sB + (uint32_t)(j * kChunk);
+                        auto load = [&](uint32_t dst, const CUtensorMap* m, int c0, int c1, int c2) {
+                            if (PAIR)
+                                ptx::tma_load_3d_pair(dst, m, full_first, c0, c1, c2);
+                            else
+                                ptx::tma_load_3d(dst, m, full_first, c0, c1, c2);
+                        };
                         if (A_MN)
                         {
-                            ptx::tma_load_3d_pair(dA, &p.tmA, full_first, m0, k, batch);
-                            ptx::tma_load_3d_pair(dA + 8192, &p.tmA, full_first, m0 + 64, k, batch);
+                            load(dA, &p.tmA, m0, k, batch);
+                            load(dA + 8192, &p.tmA, m0 + 64, k, batch);
                         }
                         else
-                            ptx::tma_load_3d_pair(dA, &p.tmA, full_first, k, m0, batch + ph * p.NB);
+                            load(dA, &p.tmA, k, m0, batch + ph * p.NB);
+                        if (EPI != EPI_PLAIN && !PAIR)
+                        {
+                            // one CTA holds 64 columns of each matrix
+                            if (B_MN)
+                            {
+                                load(dB, &p.tmB0, n0, k, b_batch);
+                                load(dB + 8192, &p.tmB1, n0, k, b_batch);
+                            }
+                            else
+                            {
+                                load(dB, &p.tmB0, k, n0, b_batch);
+                                load(dB + 8192, &p.tmB1, k, n0, b_batch);
+                            }
+                            continue;
+                        }
                         const CUtensorMap* mb = (EPI == EPI_PLAIN ? ph != 0 : rank != 0) ? &p.tmB1 : &p.tmB0;
                         if (B_MN)
                         {
-                            ptx::tma_load_3d_pair(dB, mb, full_first, n0, k, b_batch);
-                            ptx::tma_load_3d_pair(dB + 8192, mb, full_first, n0 + 64, k, b_batch);
+                            load(dB, mb, n0, k, b_batch);
+                            load(dB + 8192, mb, n0 + 64, k, b_batch);
                         }
                         else
-                            ptx::tma_load_3d_pair(dB, mb, full_first, k, n0, b_batch);
+                            load(dB, mb, k, n0, b_batch);
                     }
                     issued++;
                     if (++stage == kStages)
@@ -284,6 +426,16 @@ __global__ void __launch_bounds__(kThreads, 1) ffn_pair_kernel(const __grid_cons
             int acc        = 0;
             uint32_t acc_phase = 0;
             bool ok            = true;
+            // arrives in every CTA of the tile once the MMAs so far are done
+            auto commit = [&](uint32_t bar) {
+                if (PAIR)
+                    ptx::mma_commit_pair(bar, 3);
+                else
+                    ptx::mma_commit(bar);
+            };
+            // the MMAs write both CTAs' tensor memory
+            if (PAIR)
+                ok = ptx::mbar_wait_bounded(ptx::smem_u32(&bar_ready), 0, p.wait_limit);
             for (int tile = cluster_id; tile < p.num_tiles && ok; tile += num_clusters)
             {
                 if (!ptx::mbar_wait_bounded(ptx::smem_u32(&bar_tmem_empty[acc]), acc_phase ^ 1u, p.wait_limit))
@@ -292,7 +444,7 @@ __global__ void __launch_bounds__(kThreads, 1) ffn_pair_kernel(const __grid_cons
                     break;
                 }
                 ptx::tc_fence_after_sync();
-                const uint32_t d_tmem = tmem_base + (uint32_t)(acc * 256);
+                const uint32_t d_tmem = tmem_base + (uint32_t)(acc * S::kCols);
                 uint32_t accum        = 0;    // the first MMA of a tile overwrites the accumulator
                 for (int left = total; left > 0; left -= kSub)
                 {
@@ -312,7 +464,10 @@ __global__ void __launch_bounds__(kThreads, 1) ffn_pair_kernel(const __grid_cons
 #pragma unroll
                         for (int m = 0; m < 4; m++)
                         {
-                            ptx::mma_f16_ss_pair(d_tmem, ad, bd, p.idesc, accum);
+                            if (PAIR)
+                                ptx::mma_f16_ss_pair(d_tmem, ad, bd, p.idesc, accum);
+                            else
+                                ptx::mma_f16_ss(d_tmem, ad, bd, p.idesc, accum);
                             accum = 1;
                             // sixteen elements of K: 32 bytes inside the swizzled row, or sixteen rows of 128 bytes
                             ad += A_MN ? 128 : 2;
@@ -320,7 +475,7 @@ __global__ void __launch_bounds__(kThreads, 1) ffn_pair_kernel(const __grid_cons
                         }
                     }
                     // frees the stage in both CTAs once the MMAs above have read it
-                    ptx::mma_commit_pair(ptx::smem_u32(&bar_empty[stage]), 3);
+                    commit(ptx::smem_u32(&bar_empty[stage]));
                     if (++stage == kStages)
                     {
                         stage = 0;
@@ -329,7 +484,7 @@ __global__ void __launch_bounds__(kThreads, 1) ffn_pair_kernel(const __grid_cons
                 }
                 if (!ok)
                     break;
-                ptx::mma_commit_pair(ptx::smem_u32(&bar_tmem_full[acc]), 3);
+                commit(ptx::smem_u32(&bar_tmem_full[acc]));
                 acc ^= 1;
                 if (acc == 0)
                     acc_phase ^= 1u;
@@ -337,7 +492,10 @@ __global__ void __launch_bounds__(kThreads, 1) ffn_pair_kernel(const __grid_cons
             if (!ok)
             {
                 atomicOr(p.status, TB200_DEV_TIMEOUT);
-                ptx::mma_commit_pair(ptx::smem_u32(&bar_drain), 1);
+                if (PAIR)
+                    ptx::mma_commit_pair(ptx::smem_u32(&bar_drain), 1);
+                else
+                    ptx::mma_commit(ptx::smem_u32(&bar_drain));
                 ptx::mbar_wait_bounded(ptx::smem_u32(&bar_drain), 0, p.wait_limit);
             }
         }
@@ -348,119 +506,71 @@ __global__ void __launch_bounds__(kThreads, 1) ffn_pair_kernel(const __grid_cons
         const int quarter = warp & 3;           // TMEM lane quarter this warp may read
         const int slot    = (warp - 2) >> 2;    // the two warps of a quarter take 16-column runs in turn
         const int row     = quarter * 32 + lane;
-        const uint32_t empty_first[2] = { ptx::map_to_cta(ptx::smem_u32(&bar_tmem_empty[0]), 0),
-                                          ptx::map_to_cta(ptx::smem_u32(&bar_tmem_empty[1]), 0) };
+        const uint32_t empty_first[2] = { PAIR ? ptx::map_to_cta(ptx::smem_u32(&bar_tmem_empty[0]), 0) : ptx::smem_u32(&bar_tmem_empty[0]),
+                                          PAIR ? ptx::map_to_cta(ptx::smem_u32(&bar_tmem_empty[1]), 0) : ptx::smem_u32(&bar_tmem_empty[1]) };
         int acc            = 0;
         uint32_t acc_phase = 0;
         bool ok            = true;
         for (int tile = cluster_id; tile < p.num_tiles; tile += num_clusters)
         {
-            const Tile t = decode<EPI>(p, tile);
+            const Tile t = decode<EPI, PAIR>(p, tile);
             ok           = ptx::mbar_wait_bounded(ptx::smem_u32(&bar_tmem_full[acc]), acc_phase, p.wait_limit);
             // the whole warp must agree before the warp-collective TMEM loads
             ok = __all_sync(0xffffffffu, ok);
             if (!ok)
                 break;
             ptx::tc_fence_after_sync();
-            const int m          = t.m0 + (int)rank * 128 + row;
-            const bool row_valid = m < p.rows;
-            const int batch      = t.idx < p.NB ? t.idx : t.idx - p.NB;
-            const int64_t orow   = ((int64_t)batch * p.rows + m) * p.ld;
-            const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(acc * 256);
-            if (EPI == EPI_PLAIN)
+            const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(acc * S::kCols);
+            if (!PAIR && p.splits > 1)
             {
-                void* const out      = t.idx < p.NB ? p.out0 : p.out1;
-                const tb200_dtype dt = t.idx < p.NB ? p.out_dt : p.out1_dt;
-                for (int c = slot; c < 16; c += 2)
+                // this share's sums to shared memory, over the ring (its copies have landed and been multiplied)
+                for (int c = slot; c < S::kCols / 16; c += 2)
                 {
-                    const int col = t.n0 + c * 16;
-                    if (col >= p.cols)
+                    uint32_t v[16];
+                    ptx::tmem_ld_32x32b_x16(taddr + (uint32_t)(c * 16), v);
+                    ptx::tmem_ld_wait_x16(v);
+                    uint4* const to = reinterpret_cast<uint4*>(red + row * S::kRedLd + c * 16);
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        to[i] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+                }
+            }
+            else if (EPI == EPI_PLAIN)
+            {
+                for (int c = slot; c < S::kCols / 16; c += 2)
+                {
+                    if (t.n0 + c * 16 >= p.cols)
                         break;
                     uint32_t g[16];
                     ptx::tmem_ld_32x32b_x16(taddr + (uint32_t)(c * 16), g);
                     ptx::tmem_ld_wait_x16(g);
-                    if (!row_valid)
-                        continue;
-                    float v[16];
-#pragma unroll
-                    for (int i = 0; i < 16; i++)
-                        v[i] = __uint_as_float(g[i]);
-                    store_run(out, orow + col, dt, min(16, p.cols - col), p.vec, v);
+                    finish_run<EPI>(p, t, (int)rank * 128 + row, c * 16, g, g);
                 }
             }
             else
             {
-                for (int c = slot; c < 8; c += 2)
+                for (int c = slot; c < kHalf / 16; c += 2)
                 {
-                    const int col = t.n0 + c * 16;
-                    if (col >= p.cols)
+                    if (t.n0 + c * 16 >= p.cols)
                         break;
-                    const int n = min(16, p.cols - col);
                     uint32_t g[16], u[16];
                     ptx::tmem_ld_32x32b_x16(taddr + (uint32_t)(c * 16), g);
-                    ptx::tmem_ld_32x32b_x16(taddr + (uint32_t)(128 + c * 16), u);
-                    float d[16];
-                    if (EPI == EPI_GRAD)
-                    {
-                        const int64_t at = ((int64_t)batch * p.rows + m) * p.cols + col;
-                        const uint16_t* s = reinterpret_cast<const uint16_t*>(p.dout) + at;
-                        if (row_valid && n == 16 && p.dout_vec)
-                        {
-                            const uint4 lo = __ldg(reinterpret_cast<const uint4*>(s)), hi = __ldg(reinterpret_cast<const uint4*>(s) + 1);
-                            const uint32_t w[8] = { lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w };
-#pragma unroll
-                            for (int i = 0; i < 8; i++)
-                            {
-                                const float2 f = unpack2(w[i], p.bf16 != 0);
-                                d[2 * i]       = f.x;
-                                d[2 * i + 1]   = f.y;
-                            }
-                        }
-                        else
-                        {
-#pragma unroll
-                            for (int i = 0; i < 16; i++)
-                                d[i] = row_valid && i < n ? unpack2(s[i], p.bf16 != 0).x : 0.f;
-                        }
-                    }
+                    ptx::tmem_ld_32x32b_x16(taddr + (uint32_t)(kHalf + c * 16), u);
                     ptx::tmem_ld_wait_x16(g);
                     ptx::tmem_ld_wait_x16(u);
-                    if (!row_valid)
-                        continue;
-                    if (EPI == EPI_GATED)
-                    {
-                        float v[16];
-                        switch (p.act)
-                        {
-                            case TB200_ACT_SILU: gate_run<TB200_ACT_SILU>(g, u, v); break;
-                            case TB200_ACT_GELU: gate_run<TB200_ACT_GELU>(g, u, v); break;
-                            case TB200_ACT_GELU_TANH: gate_run<TB200_ACT_GELU_TANH>(g, u, v); break;
-                            case TB200_ACT_RELU: gate_run<TB200_ACT_RELU>(g, u, v); break;
-                            default: gate_run<TB200_ACT_SIGMOID>(g, u, v); break;
-                        }
-                        store_run(p.out0, orow + col, p.out_dt, n, p.vec, v);
-                    }
-                    else
-                    {
-                        float dg[16], du[16];
-                        switch (p.act)
-                        {
-                            case TB200_ACT_SILU: grad_run<TB200_ACT_SILU>(g, u, d, dg, du); break;
-                            case TB200_ACT_GELU: grad_run<TB200_ACT_GELU>(g, u, d, dg, du); break;
-                            case TB200_ACT_GELU_TANH: grad_run<TB200_ACT_GELU_TANH>(g, u, d, dg, du); break;
-                            case TB200_ACT_RELU: grad_run<TB200_ACT_RELU>(g, u, d, dg, du); break;
-                            default: grad_run<TB200_ACT_SIGMOID>(g, u, d, dg, du); break;
-                        }
-                        store_run(p.out0, orow + col, p.out_dt, n, p.vec, dg);
-                        store_run(p.out1, orow + col, p.out_dt, n, p.vec, du);
-                    }
+                    finish_run<EPI>(p, t, (int)rank * 128 + row, c * 16, g, u);
                 }
             }
             // this warp has read its part of the buffer: one arrival per warp on the first CTA's barrier
             ptx::tc_fence_before_sync();
             __syncwarp();
             if (lane == 0)
-                ptx::mbar_arrive_cluster(empty_first[acc]);
+            {
+                if (PAIR)
+                    ptx::mbar_arrive_cluster(empty_first[acc]);
+                else
+                    ptx::mbar_arrive(empty_first[acc]);
+            }
             acc ^= 1;
             if (acc == 0)
                 acc_phase ^= 1u;
@@ -469,15 +579,75 @@ __global__ void __launch_bounds__(kThreads, 1) ffn_pair_kernel(const __grid_cons
             atomicOr(p.status, TB200_DEV_TIMEOUT);
     }
 
+    if (!PAIR && p.splits > 1)
+    {
+        // ------------------------------------------------------------------ the shares' sums meet, in order (one tile to a cluster)
+        // A share whose wait gave up holds sums that do not count; every share reaches both barriers.
+        ptx::cluster_sync();
+        const Tile t         = decode<EPI, PAIR>(p, cluster_id);
+        constexpr int kRuns  = (EPI == EPI_PLAIN ? S::kCols : kHalf) / 16;    // of a row
+        const uint32_t local = ptx::smem_u32(red);
+        for (int e = share * kThreads + (int)threadIdx.x; e < 128 * kRuns; e += p.splits * kThreads)
+        {
+            const int r = e / kRuns, run = e % kRuns * 16;
+            if (t.m0 + r >= p.rows || t.n0 + run >= p.cols)
+                continue;
+            uint32_t g[16], u[16];
+            auto sum = [&](int col, uint32_t (&v)[16]) {
+                float total[16];
+#pragma unroll
+                for (int i = 0; i < 16; i++)
+                    total[i] = 0.f;
+                for (int k = 0; k < p.splits; k++)
+                {
+                    const uint32_t at = ptx::map_to_cta(local + (uint32_t)((r * S::kRedLd + col) * 4), (uint32_t)k);
+                    float4 x[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                                     : "=f"(x[i].x), "=f"(x[i].y), "=f"(x[i].z), "=f"(x[i].w)
+                                     : "r"(at + (uint32_t)(16 * i))
+                                     : "memory");
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                    {
+                        total[4 * i] += x[i].x;
+                        total[4 * i + 1] += x[i].y;
+                        total[4 * i + 2] += x[i].z;
+                        total[4 * i + 3] += x[i].w;
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 16; i++)
+                    v[i] = __float_as_uint(total[i]);
+            };
+            sum(run, g);
+            if (EPI != EPI_PLAIN)
+                sum(kHalf + run, u);
+            else
+            {
+#pragma unroll
+                for (int i = 0; i < 16; i++)
+                    u[i] = 0;
+            }
+            finish_run<EPI>(p, t, r, run, g, u);
+        }
+        ptx::cluster_sync();    // nobody leaves while another share may still read its sums
+    }
+
     // ---------------------------------------------------------------------- teardown
     // Neither CTA may leave (or free its TMEM) while the other can still signal it or read its shared memory.
     ptx::tc_fence_before_sync();
     __syncthreads();
-    ptx::cluster_sync();
+    if (PAIR)
+        ptx::cluster_sync();
     if (warp == 1)
     {
         ptx::tc_fence_after_sync();
-        ptx::tmem_dealloc_pair(tmem_base, kTmemCols);
+        if (PAIR)
+            ptx::tmem_dealloc_pair(tmem_base, S::kTmemCols);
+        else
+            ptx::tmem_dealloc(tmem_base, S::kTmemCols);
     }
 }
 
@@ -486,14 +656,14 @@ typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, v
 
 // A [batches][outer][inner] operand of 16-bit elements with rows `pitch` elements apart: K along its rows (boxes of 64 x 128), or
 // across them (64 x 64, two for each half tile).  What lies outside reads as zero.
-tb200_status encode(tb200_ctx* ctx, CUtensorMap* m, const Matrix& x, bool bf16, bool k_inner)
+tb200_status encode(tb200_ctx* ctx, CUtensorMap* m, const Matrix& x, bool bf16, bool k_inner, uint32_t lines = 128)
 {
     const EncodeTiled enc = reinterpret_cast<EncodeTiled>(tensor_map_encode_fn());
     if (!enc)
         return fail(ctx, TB200_INTERNAL, "cuTensorMapEncodeTiled is not available from the driver");
     const cuuint64_t dims[3]    = { (cuuint64_t)x.inner, (cuuint64_t)x.outer, (cuuint64_t)x.batches };
     const cuuint64_t strides[2] = { (cuuint64_t)x.pitch * 2, (cuuint64_t)x.pitch * (cuuint64_t)x.outer * 2 };
-    const cuuint32_t box[3]     = { 64, k_inner ? 128u : 64u, 1 };
+    const cuuint32_t box[3]     = { 64, k_inner ? lines : 64u, 1 };
     const cuuint32_t estr[3]    = { 1, 1, 1 };
     const CUresult r = enc(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(x.data), dims, strides, box,
                            estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -511,33 +681,64 @@ int run_alignment(const void* p, int64_t ld, size_t es)
 
 }    // namespace
 
-tb200_status pair_launch(tb200_ctx* ctx, const PairProduct& q)
+namespace
 {
+
+typedef void (*Kern)(const Params);
+
+template <bool PAIR>
+Kern pick(const PairProduct& q, int* bit)
+{
+    if (q.kind == PAIR_GATED && !q.a_mn)
+    {
+        *bit = q.b_mn ? 0 : 1;
+        return q.b_mn ? ffn_pair_kernel<EPI_GATED, false, true, PAIR> : ffn_pair_kernel<EPI_GATED, false, false, PAIR>;
+    }
+    if (q.kind == PAIR_GRAD && !q.a_mn && q.b_mn)
+    {
+        *bit = 2;
+        return ffn_pair_kernel<EPI_GRAD, false, true, PAIR>;
+    }
+    if (q.kind == PAIR_PLAIN && q.a_mn == q.b_mn)
+    {
+        *bit = q.a_mn ? 3 : 4;
+        return q.a_mn ? ffn_pair_kernel<EPI_PLAIN, true, true, PAIR> : ffn_pair_kernel<EPI_PLAIN, false, false, PAIR>;
+    }
+    return nullptr;
+}
+
+template <bool PAIR>
+tb200_status launch(tb200_ctx* ctx, const PairProduct& q, int splits)
+{
+    using S = Shape<PAIR>;
     Params k;
     memset(&k, 0, sizeof(k));
-    const bool bf16 = q.dt == TB200_BF16;
-    const bool gated = q.kind != PAIR_PLAIN;
-    tb200_status st  = encode(ctx, &k.tmA, q.a, bf16, !q.a_mn);
+    const bool bf16       = q.dt == TB200_BF16;
+    const bool gated      = q.kind != PAIR_PLAIN;
+    const uint32_t b_line = !PAIR && gated ? 64u : 128u;
+    tb200_status st       = encode(ctx, &k.tmA, q.a, bf16, !q.a_mn);
     if (st == TB200_OK)
-        st = encode(ctx, &k.tmB0, q.b[0], bf16, !q.b_mn);
+        st = encode(ctx, &k.tmB0, q.b[0], bf16, !q.b_mn, b_line);
     if (st == TB200_OK)
-        st = encode(ctx, &k.tmB1, q.b[1].data ? q.b[1] : q.b[0], bf16, !q.b_mn);
+        st = encode(ctx, &k.tmB1, q.b[1].data ? q.b[1] : q.b[0], bf16, !q.b_mn, b_line);
     if (st != TB200_OK)
         return st;
-    k.rows      = q.rows;
-    k.cols      = q.cols;
-    k.tiles_m   = (q.rows + 255) / 256;
-    k.tiles_n   = gated ? (q.cols + 127) / 128 : (q.cols + 255) / 256;
-    k.NB        = q.NB;
+    const int step_n    = gated ? S::kCols / 2 : S::kCols;
+    k.rows              = q.rows;
+    k.cols              = q.cols;
+    k.tiles_m           = (q.rows + S::kRows - 1) / S::kRows;
+    k.tiles_n           = (q.cols + step_n - 1) / step_n;
+    k.NB                = q.NB;
     const int64_t tiles = (int64_t)k.tiles_m * k.tiles_n * q.NB * (q.results == 2 && !gated ? 2 : 1);
     if (tiles > (1 << 30))
         return fail(ctx, TB200_ERROR, "a feed-forward product of %lld tiles is too large", (long long)tiles);
     k.num_tiles = (int)tiles;
     // A's rows of a group, about 32 MB, stay in L2
-    const int64_t a_tile = 256LL * q.K * q.phases * 2;
+    const int64_t a_tile = (int64_t)S::kRows * q.K * q.phases * 2;
     k.group_m  = (int)std::max<int64_t>(1, std::min<int64_t>(k.tiles_m, (32LL << 20) / std::max<int64_t>(1, a_tile)));
     k.chunks   = (int)((q.K + 63) / 64);
     k.phases   = q.phases;
+    k.splits   = splits;
     k.act      = q.act;
     k.bf16     = bf16 ? 1 : 0;
     k.out_dt   = q.out_dt[0];
@@ -550,55 +751,74 @@ tb200_status pair_launch(tb200_ctx* ctx, const PairProduct& q)
         k.vec = std::min(k.vec, run_alignment(q.out[1], q.ld, dtype_size(q.out_dt[1])));
     k.dout     = q.dout;
     k.dout_vec = q.dout && run_alignment(q.dout, q.cols, 2) > 0;
-    // K along the rows: 8-row groups of 128-byte swizzled rows 1024 bytes apart.  Across them: 64 columns of 64 K rows, the second
-    // half's 8192 bytes behind.
+    // K along the rows: 8-row groups of 128-byte swizzled rows 1024 bytes apart.  Across them: 64 columns of 64 K rows, the next 64
+    // 8192 bytes behind.
     k.a_desc_hi  = q.a_mn ? ptx::make_smem_desc_hi(8192, 1024, 2) : ptx::make_smem_desc_hi(16, 1024, 2);
     k.b_desc_hi  = q.b_mn ? ptx::make_smem_desc_hi(8192, 1024, 2) : ptx::make_smem_desc_hi(16, 1024, 2);
     const uint32_t fmt = bf16 ? 1u : 0u;
-    k.idesc      = ptx::make_idesc(1u, fmt, fmt, q.a_mn ? 1u : 0u, q.b_mn ? 1u : 0u, 256u, 256u);
+    k.idesc      = ptx::make_idesc(1u, fmt, fmt, q.a_mn ? 1u : 0u, q.b_mn ? 1u : 0u, (uint32_t)S::kRows, (uint32_t)S::kCols);
     k.wait_limit = ctx->wait_limit_cycles;
     k.status     = ctx->d_status;
-
-    void (*kern)(const Params) = nullptr;
-    int bit                    = 0;
-    if (q.kind == PAIR_GATED && !q.a_mn)
-    {
-        kern = q.b_mn ? ffn_pair_kernel<EPI_GATED, false, true> : ffn_pair_kernel<EPI_GATED, false, false>;
-        bit  = q.b_mn ? 0 : 1;
-    }
-    else if (q.kind == PAIR_GRAD && !q.a_mn && q.b_mn)
-    {
-        kern = ffn_pair_kernel<EPI_GRAD, false, true>;
-        bit  = 2;
-    }
-    else if (q.kind == PAIR_PLAIN && q.a_mn == q.b_mn)
-    {
-        kern = q.a_mn ? ffn_pair_kernel<EPI_PLAIN, true, true> : ffn_pair_kernel<EPI_PLAIN, false, false>;
-        bit  = q.a_mn ? 3 : 4;
-    }
+    int bit      = 0;
+    const Kern kern = pick<PAIR>(q, &bit);
     if (!kern)
         return fail(ctx, TB200_INTERNAL, "no kernel for this feed-forward product");
-    st = raise_smem_limit(ctx, 128 + bit, reinterpret_cast<const void*>(kern), kSmem);
+    st = raise_smem_limit(ctx, 128 + bit + (PAIR ? 0 : 48), reinterpret_cast<const void*>(kern), S::kSmem);
     if (st != TB200_OK)
         return st;
     cudaLaunchConfig_t cfg = {};
     cfg.blockDim           = dim3(kThreads);
-    cfg.dynamicSmemBytes   = (size_t)kSmem;
+    cfg.dynamicSmemBytes   = (size_t)S::kSmem;
     cfg.stream             = ctx->stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id               = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 2;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
+    cudaLaunchAttribute attr[2];
+    attr[0].id                                         = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = ctx->launch_overlap ? 1 : 0;
+    attr[1].id               = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = PAIR ? 2 : (unsigned)splits;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
     cfg.attrs    = attr;
-    cfg.numAttrs = 1;
-    cfg.gridDim  = dim3((unsigned)(2 * std::max(1, std::min(k.num_tiles, ctx->num_sms / 2))));
+    cfg.numAttrs = PAIR || splits > 1 ? 2 : 1;
+    // a tile that is shared is its cluster's only one
+    cfg.gridDim  = dim3((unsigned)(PAIR         ? 2 * std::max(1, std::min(k.num_tiles, ctx->num_sms / 2))
+                                   : splits > 1 ? k.num_tiles * splits
+                                                : std::min(k.num_tiles, ctx->num_sms)));
     timer_begin(ctx);
     const cudaError_t le = cudaLaunchKernelEx(&cfg, kern, k);
     timer_end(ctx);
     if (le != cudaSuccess)
         return fail(ctx, TB200_INTERNAL, "launch of a feed-forward product failed: %s", cudaGetErrorString(le));
     return post_launch(ctx, q.name);
+}
+
+}    // namespace
+
+tb200_status pair_launch(tb200_ctx* ctx, const PairProduct& q)
+{
+    // Pairs, or CTAs by themselves, K shared by up to eight: by their cycles.  A chunk of K takes a pair 520 and a CTA by itself 330; the last
+    // tile's epilogue shows, and so does the exchange of the shares' sums.
+    const bool gated     = q.kind != PAIR_PLAIN;
+    const int64_t copies = (int64_t)q.NB * (q.results == 2 && !gated ? 2 : 1), chunks = (q.K + 63) / 64 * q.phases;
+    auto tiles = [&](int rows, int cols) { return (int64_t)((q.rows + rows - 1) / rows) * ((q.cols + cols - 1) / cols) * copies; };
+    auto waves = [&](int64_t n, int64_t at_once) { return (double)((n + at_once - 1) / at_once); };
+    const int64_t large = tiles(256, gated ? 128 : 256), small = tiles(128, gated ? 64 : 128);
+    double best = waves(large, ctx->num_sms / 2) * (double)chunks * 520.0 + 4500.0;
+    int splits  = 0;
+    for (int s = 1; s <= 8; s *= 2)
+    {
+        if (s > 1 && (chunks < 4 * s || small * s > ctx->num_sms))
+            break;
+        const double cost = waves(small * s, ctx->num_sms) * (double)((chunks + s - 1) / s) * 330.0 + 2500.0 + (s > 1 ? 2500.0 : 0.0);
+        if (cost < best)
+        {
+            best   = cost;
+            splits = s;
+        }
+    }
+    const int forced = diag_env_int("TB200_FFN_SPLITS", -1);
+    if (forced >= 0)
+        splits = forced;
+    return splits ? launch<false>(ctx, q, splits) : launch<true>(ctx, q, 1);
 }
 
 }    // namespace ffn
