@@ -507,6 +507,8 @@ tb200_status matmul_rows_launch(tb200_ctx* ctx, tb200_dtype dt, const void* a, c
 
 // fp32 SGEMM on CUDA cores (sgemm_f32.cu): out[n] = a[n] x b[n], a [N,H,C], b [N,C,W]
 tb200_status sgemm_f32_launch(tb200_ctx* ctx, const float* a, const float* b, float* out, int N, int H, int C, int W);
+// ... two products of the same a in one launch: out0 = a x b0, out1 = a x b1, a [H,C], b0 and b1 [C,W]; all 16-byte aligned
+tb200_status sgemm_f32_two_launch(tb200_ctx* ctx, const float* a, const float* b0, const float* b1, float* out0, float* out1, int H, int C, int W);
 
 // fp32 CONV2D on the same kernel: the input gathered tap by tap as the product's rows, weights re-ordered once to
 // [KH*KW*IC][conv_f32_ldb(OC)] by conv_f32_weights_launch (which leaves 0 in *all_finite when a weight is not finite)
@@ -529,7 +531,7 @@ tb200_status conv_f32_launch(tb200_ctx* ctx, const ConvF32Problem& q);
 // The same two on the tensor cores, operands taken apart into three bf16 parts (sgemm_split.cu); the launches above choose.
 // Estimated SM cycles, 0 where that kernel does not serve.
 double sgemm_split_cost(const tb200_ctx* ctx, int64_t batches, int64_t M, int64_t N, int64_t K, bool conv);
-tb200_status sgemm_split_launch(tb200_ctx* ctx, const float* a, const float* b, float* out, int N, int H, int C, int W);
+tb200_status sgemm_split_launch(tb200_ctx* ctx, const float* a, const float* b, float* out, int N, int H, int C, int W, int64_t a_batch, int64_t b_batch, int64_t o_batch);
 tb200_status conv_f32_split_launch(tb200_ctx* ctx, const ConvF32Problem& q);
 
 }    // namespace tb200

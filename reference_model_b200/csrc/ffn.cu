@@ -61,11 +61,10 @@ size_t pad_bytes(int64_t inner, int64_t rows)
     return inner % 8 != 0 ? (size_t)rows * round_up(inner, 8) * 2 : 0;
 }
 
-tb200_status pad(tb200_ctx* ctx, const void* data, const Matrix& m)
+void pad(RowCopies* copies, const void* data, const Matrix& m)
 {
-    if (m.data == data)
-        return TB200_OK;
-    return pitch_copy_launch(ctx, data, const_cast<void*>(m.data), m.outer * m.batches, m.inner, m.pitch);
+    if (m.data != data)
+        copies->add(data, const_cast<void*>(m.data), m.outer * m.batches, m.inner * 2, m.inner * 2, m.pitch * 2);
 }
 
 #define TB200_TRY(expr)                     \
@@ -104,9 +103,11 @@ tb200_status gated_pair(tb200_ctx* ctx, const GatedProblem& q)
         k.a    = operand(q.a, q.C, q.H, q.NB, a);
         k.b[0] = operand(q.gate, q.W, q.C, q.NB, g);
         k.b[1] = operand(q.up, q.W, q.C, q.NB, u);
-        TB200_TRY(pad(ctx, q.a, k.a));
-        TB200_TRY(pad(ctx, q.gate, k.b[0]));
-        TB200_TRY(pad(ctx, q.up, k.b[1]));
+        RowCopies copies;
+        pad(&copies, q.a, k.a);
+        pad(&copies, q.gate, k.b[0]);
+        pad(&copies, q.up, k.b[1]);
+        TB200_TRY(row_copies_launch(ctx, copies));
         k.rows      = (int)q.H;
         k.cols      = q.W;
         k.K         = q.C;
@@ -143,9 +144,11 @@ tb200_status gated_backward_pair(tb200_ctx* ctx, const GatedProblem& q)
             continue;
         }
         const Matrix a = operand(q.a, q.C, q.H, q.NB, pa), gate = operand(q.gate, q.W, q.C, q.NB, pg), up = operand(q.up, q.W, q.C, q.NB, pu);
-        TB200_TRY(pad(ctx, q.a, a));
-        TB200_TRY(pad(ctx, q.gate, gate));
-        TB200_TRY(pad(ctx, q.up, up));
+        RowCopies copies;
+        pad(&copies, q.a, a);
+        pad(&copies, q.gate, gate);
+        pad(&copies, q.up, up);
+        TB200_TRY(row_copies_launch(ctx, copies));
         PairProduct k;
         memset(&k, 0, sizeof(k));
         k.dt      = q.dt;
@@ -219,22 +222,24 @@ tb200_status gated_backward_pair(tb200_ctx* ctx, const GatedProblem& q)
     return TB200_OK;
 }
 
+// fp32: both projections into scratch, G's batches and then U's, in one launch where the weights are one matrix each
+tb200_status projections_f32(tb200_ctx* ctx, const GatedProblem& q, float* gu)
+{
+    const float *a = reinterpret_cast<const float*>(q.a), *gate = reinterpret_cast<const float*>(q.gate), *up = reinterpret_cast<const float*>(q.up);
+    if (q.NB == 1)
+        return sgemm_f32_two_launch(ctx, a, gate, up, gu, gu + q.H * q.W, (int)q.H, q.C, q.W);
+    TB200_TRY(sgemm_f32_launch(ctx, a, gate, gu, q.NB, (int)q.H, q.C, q.W));
+    return sgemm_f32_launch(ctx, a, up, gu + (int64_t)q.NB * q.H * q.W, q.NB, (int)q.H, q.C, q.W);
+}
+
 // fp32: the two projections by the fp32 product, then a pass over them
 tb200_status gated_f32(tb200_ctx* ctx, const GatedProblem& q)
 {
-    const int64_t rows = q.NB * q.H, n = rows * q.W;
-    Carver c;
-    c.take((size_t)n * 4);
-    c.take((size_t)n * 4);
-    TB200_TRY(ensure_scratch(ctx, c.used));
-    c       = Carver();
-    c.base  = reinterpret_cast<uint8_t*>(ctx->scratch);
-    float* const g = reinterpret_cast<float*>(c.take((size_t)n * 4));
-    float* const u = reinterpret_cast<float*>(c.take((size_t)n * 4));
-    const float* a = reinterpret_cast<const float*>(q.a);
-    TB200_TRY(sgemm_f32_launch(ctx, a, reinterpret_cast<const float*>(q.gate), g, q.NB, (int)q.H, q.C, q.W));
-    TB200_TRY(sgemm_f32_launch(ctx, a, reinterpret_cast<const float*>(q.up), u, q.NB, (int)q.H, q.C, q.W));
-    TB200_TRY(gate_f32_launch(ctx, g, u, reinterpret_cast<float*>(q.out), n, q.act));
+    const int64_t n = q.NB * q.H * q.W;
+    TB200_TRY(ensure_scratch(ctx, (size_t)n * 8));
+    float* const gu = reinterpret_cast<float*>(ctx->scratch);
+    TB200_TRY(projections_f32(ctx, q, gu));
+    TB200_TRY(gate_f32_launch(ctx, gu, gu + n, reinterpret_cast<float*>(q.out), n, q.act));
     return post_launch(ctx, "gated_f32", 0);
 }
 
@@ -247,8 +252,8 @@ tb200_status gated_backward_f32(tb200_ctx* ctx, const GatedProblem& q)
     float *g = nullptr, *u = nullptr, *both = nullptr, *bt = nullptr, *at = nullptr;
     for (int pass = 0; pass < 2; pass++)
     {
-        g    = reinterpret_cast<float*>(c.take((size_t)n * 4));
-        u    = reinterpret_cast<float*>(c.take((size_t)n * 4));
+        g    = reinterpret_cast<float*>(c.take((size_t)n * 8));
+        u    = g + n;
         both = reinterpret_cast<float*>(c.take(q.da ? (size_t)n * 8 : 0));
         bt   = reinterpret_cast<float*>(c.take(q.da ? (size_t)q.NB * weights * 8 : 0));
         at   = reinterpret_cast<float*>(c.take(weights_too ? (size_t)rows * q.C * 4 : 0));
@@ -260,8 +265,7 @@ tb200_status gated_backward_f32(tb200_ctx* ctx, const GatedProblem& q)
         }
     }
     const float *a = reinterpret_cast<const float*>(q.a), *gate = reinterpret_cast<const float*>(q.gate), *up = reinterpret_cast<const float*>(q.up);
-    TB200_TRY(sgemm_f32_launch(ctx, a, gate, g, q.NB, (int)q.H, q.C, q.W));
-    TB200_TRY(sgemm_f32_launch(ctx, a, up, u, q.NB, (int)q.H, q.C, q.W));
+    TB200_TRY(projections_f32(ctx, q, g));
     TB200_TRY(grad_f32_launch(ctx, g, u, reinterpret_cast<const float*>(q.dout), q.da ? both : nullptr, rows, q.W, q.act));
     if (q.da)
     {
@@ -272,10 +276,16 @@ tb200_status gated_backward_f32(tb200_ctx* ctx, const GatedProblem& q)
     if (weights_too)
     {
         TB200_TRY(transpose_f32_launch(ctx, a, at, q.NB, q.H, q.C, q.H * q.C));
-        if (q.dgate)
-            TB200_TRY(sgemm_f32_launch(ctx, at, g, reinterpret_cast<float*>(q.dgate), q.NB, q.C, (int)q.H, q.W));
-        if (q.dup)
-            TB200_TRY(sgemm_f32_launch(ctx, at, u, reinterpret_cast<float*>(q.dup), q.NB, q.C, (int)q.H, q.W));
+        float *const dgate = reinterpret_cast<float*>(q.dgate), *const dup = reinterpret_cast<float*>(q.dup);
+        if (dgate && dup && q.NB == 1)
+            TB200_TRY(sgemm_f32_two_launch(ctx, at, g, u, dgate, dup, q.C, (int)q.H, q.W));
+        else if (dgate || dup)
+        {
+            if (dgate)
+                TB200_TRY(sgemm_f32_launch(ctx, at, g, dgate, q.NB, q.C, (int)q.H, q.W));
+            if (dup)
+                TB200_TRY(sgemm_f32_launch(ctx, at, u, dup, q.NB, q.C, (int)q.H, q.W));
+        }
     }
     return post_launch(ctx, "gated_backward_f32", 0);
 }
@@ -317,34 +327,34 @@ tb200_status w4_launch(tb200_ctx* ctx, const W4Problem& q)
     if (few)
     {
         W4Problem r = q;
+        RowCopies copies;
         for (int i = 0; i < q.mats; i++)
         {
             if (scale_row(i) % 16)
             {
-                const int64_t es = (int64_t)dtype_size(q.w[i].scale_dt), row = round_up(scale_row(i), 16);
-                TB200_TRY(byte_copy_launch(ctx, reinterpret_cast<const uint8_t*>(q.w[i].scale), reinterpret_cast<uint8_t*>(scale[i]), groups, scale_row(i),
-                                           scale_row(i), row));
+                const int64_t row = round_up(scale_row(i), 16);
+                copies.add(q.w[i].scale, scale[i], groups, scale_row(i), scale_row(i), row);
                 r.w[i].scale       = scale[i];
-                r.w[i].scale_pitch = row / es;
+                r.w[i].scale_pitch = row / (int64_t)dtype_size(q.w[i].scale_dt);
             }
             if (q.w[i].zero && q.W % 16)
             {
-                TB200_TRY(byte_copy_launch(ctx, reinterpret_cast<const uint8_t*>(q.w[i].zero), reinterpret_cast<uint8_t*>(zero[i]), groups, q.W, q.W,
-                                           round_up(q.W, 16)));
+                copies.add(q.w[i].zero, zero[i], groups, q.W, q.W, round_up(q.W, 16));
                 r.w[i].zero       = reinterpret_cast<const int8_t*>(zero[i]);
                 r.w[i].zero_pitch = round_up(q.W, 16);
             }
             if (q.w[i].pitch % 16)
             {
-                TB200_TRY(byte_copy_launch(ctx, q.w[i].data, reinterpret_cast<uint8_t*>(w[i]), q.W, (q.C + 1) / 2, q.w[i].pitch, wpitch));
+                copies.add(q.w[i].data, w[i], q.W, (q.C + 1) / 2, q.w[i].pitch, wpitch);
                 r.w[i].data  = reinterpret_cast<const uint8_t*>(w[i]);
                 r.w[i].pitch = wpitch;
             }
         }
         if (f32)
-            TB200_TRY(split_rows_launch(ctx, reinterpret_cast<const float*>(q.a), x, q.M, q.C, xpitch));
+            copies.add(q.a, x, q.M, (int64_t)q.C * 4, (int64_t)q.C * 4, xpitch * 2, true);
         else if (copy_x)
-            TB200_TRY(pitch_copy_launch(ctx, q.a, x, q.M, q.C, xpitch));
+            copies.add(q.a, x, q.M, (int64_t)q.C * 2, (int64_t)q.C * 2, xpitch * 2);
+        TB200_TRY(row_copies_launch(ctx, copies));
         return w4_rows_launch(ctx, r, f32 || copy_x ? x : q.a, f32 || copy_x ? xpitch : q.C, parts, f32 || q.dt == TB200_BF16,
                               reinterpret_cast<float*>(partial));
     }
@@ -365,7 +375,9 @@ tb200_status w4_launch(tb200_ctx* ctx, const W4Problem& q)
     k.dt   = q.dt;
     k.kind = q.mats == 2 ? PAIR_GATED : PAIR_PLAIN;
     k.a    = operand(q.a, q.C, q.M, 1, x);
-    TB200_TRY(pad(ctx, q.a, k.a));
+    RowCopies copies;
+    pad(&copies, q.a, k.a);
+    TB200_TRY(row_copies_launch(ctx, copies));
     for (int i = 0; i < q.mats; i++)
         k.b[i] = { w[i], q.C, q.W, 1, dpitch };
     k.rows      = (int)q.M;
@@ -380,6 +392,12 @@ tb200_status w4_launch(tb200_ctx* ctx, const W4Problem& q)
     k.ld        = q.W;
     k.name      = q.mats == 2 ? "gated_w4_pair" : "matmul_w4_pair";
     return pair_launch(ctx, k);
+}
+
+// The tiled kernels' 32-bit indexes step past the last element, by less than a tile.
+bool tiles_reach(int64_t rows, int64_t C, int64_t W)
+{
+    return rows <= (1 << 30) && C <= (1 << 30) && W <= (1 << 29);
 }
 
 size_t aligned(size_t bytes)
@@ -426,7 +444,7 @@ tb200_status w4_entry(tb200_ctx* ctx, const char* op, const tb200_tensor* a, con
         q.w[i].scale_pitch = q.w[i].zero_pitch = q.W;
         q.w[i].zero     = mats[i]->zero ? reinterpret_cast<const int8_t*>(mats[i]->zero->data) : nullptr;
     }
-    return ctx->policy == 0 && q.C <= (1 << 30) ? w4_launch(ctx, q) : w4_direct_launch(ctx, q);
+    return ctx->policy == 0 && tiles_reach(q.M, q.C, q.W) ? w4_launch(ctx, q) : w4_direct_launch(ctx, q);
 }
 
 GatedProblem gated_problem(const tb200_tensor* a, const tb200_tensor* gate, const tb200_tensor* up, int activation)
@@ -485,7 +503,7 @@ extern "C" tb200_status tb200_matmul_gated(tb200_ctx* ctx, const tb200_tensor* a
         GatedProblem q = gated_problem(a, gate, up, activation);
         q.out          = output->data;
         q.out_dt       = output->dtype;
-        if (ctx->policy == 0)
+        if (ctx->policy == 0 && tiles_reach(q.H, q.C, q.W))
             return q.dt == TB200_FP32 ? gated_f32(ctx, q) : gated_pair(ctx, q);
         return gated_direct_launch(ctx, q);
     });
@@ -534,7 +552,7 @@ extern "C" tb200_status tb200_matmul_gated_backward(tb200_ctx* ctx, const tb200_
             q.dup    = grad_up->data;
             q.dup_dt = grad_up->dtype;
         }
-        if (ctx->policy == 0)
+        if (ctx->policy == 0 && tiles_reach(q.H, q.C, q.W))
             return q.dt == TB200_FP32 ? gated_backward_f32(ctx, q) : gated_backward_pair(ctx, q);
         const size_t each     = aligned((size_t)q.NB * q.H * q.W * sizeof(float));
         const tb200_status st = ensure_scratch(ctx, 2 * each);

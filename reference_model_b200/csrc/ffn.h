@@ -103,10 +103,23 @@ tb200_status w4_rows_launch(tb200_ctx* ctx, const W4Problem& q, const void* x, i
 size_t w4_rows_partial_bytes(const tb200_ctx* ctx, int64_t xrows);
 
 // ---- ffn_small.cu: copies
-// fp32 rows to three bf16 rows each whose sum they are, rows `pitch` apart
-tb200_status split_rows_launch(tb200_ctx* ctx, const float* in, void* out, int64_t rows, int64_t inner, int64_t pitch);
-// rows of `inner` bytes, `in_pitch` apart, to rows `pitch` (a multiple of 16) apart
-tb200_status byte_copy_launch(tb200_ctx* ctx, const uint8_t* in, uint8_t* out, int64_t rows, int64_t inner, int64_t in_pitch, int64_t pitch);
+// rows of `inner` bytes, `in_pitch` apart, to rows `pitch` (a multiple of 16) apart with zeros behind them; split: fp32 rows to three bf16 rows each
+// whose sum they are.  Up to eight copies in a launch.
+struct RowCopy
+{
+    const uint8_t* in;
+    uint8_t* out;
+    int64_t inner, in_pitch, pitch;
+    int word, split;
+};
+struct RowCopies
+{
+    RowCopy copy[8];
+    int64_t items[8];    // of sixteen result bytes, up to and with each copy
+    int n = 0;
+    void add(const void* in, void* out, int64_t rows, int64_t inner, int64_t in_pitch, int64_t pitch, bool split = false);
+};
+tb200_status row_copies_launch(tb200_ctx* ctx, const RowCopies& q);
 // [W][pitch] 16-bit rows of a 4-bit matrix's values, or fp32 [C][W] (dt FP32)
 tb200_status w4_dense_launch(tb200_ctx* ctx, const W4Mat& w, int C, int W, int group, tb200_dtype dt, void* out, int64_t pitch);
 tb200_status gate_f32_launch(tb200_ctx* ctx, const float* g, const float* u, float* out, int64_t n, int act);
@@ -114,8 +127,5 @@ tb200_status gate_f32_launch(tb200_ctx* ctx, const float* g, const float* u, flo
 tb200_status grad_f32_launch(tb200_ctx* ctx, float* g, float* u, const float* d, float* both, int64_t rows, int W, int act);
 // [batches][R][C] to [batches][C][R], results `out_batch` elements apart
 tb200_status transpose_f32_launch(tb200_ctx* ctx, const float* in, float* out, int64_t batches, int64_t R, int64_t C, int64_t out_batch);
-// 16-bit rows of `inner` elements to rows `pitch` apart, zeros behind them
-tb200_status pitch_copy_launch(tb200_ctx* ctx, const void* in, void* out, int64_t rows, int64_t inner, int64_t pitch);
-
 }    // namespace ffn
 }    // namespace tb200

@@ -24,16 +24,16 @@ __device__ __forceinline__ float w4_dot(const W4Problem& q, const W4Mat& w, int6
 {
     const uint8_t* row = w.data + (int64_t)col * w.pitch;
     float total        = 0.f;
-    for (int c0 = 0, g = 0; c0 < q.C; g++)
+    for (int64_t c0 = 0, g = 0; c0 < q.C; g++)
     {
-        const int c1  = (int)min((int64_t)q.C, (int64_t)c0 + q.group);
-        const int64_t at = (int64_t)g * q.W + col;
+        const int64_t c1 = min((int64_t)q.C, c0 + q.group);
+        const int64_t at = g * q.W + col;
         const int z   = w.zero ? (int)w.zero[at] : 0;
         bad_zero |= z < -8 || z > 7;
         float s = 0.f;
         while (c0 < c1)
         {
-            const int run = min(c1, c0 + kDirectRun);
+            const int64_t run = min(c1, c0 + kDirectRun);
             float part    = 0.f;
             for (; c0 < run; c0++)
             {
@@ -73,15 +73,15 @@ __global__ void __launch_bounds__(kDirectThreads) gated_direct_kernel(const __gr
         const int64_t row = i / q.W, batch = row / q.H;
         const int64_t b0  = batch * q.C * q.W + (i - row * q.W);
         float g = 0.f, u = 0.f;
-        for (int c0 = 0; c0 < q.C; c0 += kDirectRun)
+        for (int64_t c0 = 0; c0 < q.C; c0 += kDirectRun)
         {
             float pg = 0.f, pu = 0.f;
-            const int c1 = min(q.C, c0 + kDirectRun);
-            for (int c = c0; c < c1; c++)
+            const int64_t c1 = min((int64_t)q.C, c0 + kDirectRun);
+            for (int64_t c = c0; c < c1; c++)
             {
                 const float x = load_fp(q.a, row * q.C + c, q.dt);
-                pg += x * load_fp(q.gate, b0 + (int64_t)c * q.W, q.dt);
-                pu += x * load_fp(q.up, b0 + (int64_t)c * q.W, q.dt);
+                pg += x * load_fp(q.gate, b0 + c * q.W, q.dt);
+                pu += x * load_fp(q.up, b0 + c * q.W, q.dt);
             }
             g += pg;
             u += pu;
@@ -107,11 +107,11 @@ __global__ void __launch_bounds__(kDirectThreads) gated_grad_a_direct_kernel(con
         const int64_t row = i / q.C, batch = row / q.H;
         const int64_t b0  = (batch * q.C + (i - row * q.C)) * q.W;
         float total       = 0.f;
-        for (int w0 = 0; w0 < q.W; w0 += kDirectRun)
+        for (int64_t w0 = 0; w0 < q.W; w0 += kDirectRun)
         {
-            float part   = 0.f;
-            const int w1 = min(q.W, w0 + kDirectRun);
-            for (int w = w0; w < w1; w++)
+            float part       = 0.f;
+            const int64_t w1 = min((int64_t)q.W, w0 + kDirectRun);
+            for (int64_t w = w0; w < w1; w++)
                 part += dg[row * q.W + w] * load_fp(q.gate, b0 + w, q.dt) + du[row * q.W + w] * load_fp(q.up, b0 + w, q.dt);
             total += part;
         }

@@ -35,65 +35,64 @@ cudaError_t launch_overlapped(tb200_ctx* ctx, K kernel, int grid, A... args)
     return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
-// A thread writes eight elements; rows of any length start at any even address, so they are read one element at a time (neighbouring
-// threads read neighbouring runs).
-__global__ void __launch_bounds__(kSmallThreads) pitch_copy_kernel(const uint16_t* __restrict__ in, uint16_t* __restrict__ out, int64_t rows, int64_t inner,
-                                                                   int64_t pitch)
+// Sixteen bytes of a row that starts anywhere, in words of UNIT bytes, zeros behind its end
+template <typename T>
+__device__ __forceinline__ uint4 row_piece(const uint8_t* src, int64_t left)
 {
-    const int64_t runs = pitch / 8, n = rows * runs;
-    for (int64_t i = (int64_t)blockIdx.x * kSmallThreads + threadIdx.x; i < n; i += (int64_t)gridDim.x * kSmallThreads)
-    {
-        const int64_t r = i / runs, c = (i - r * runs) * 8;
-        const uint16_t* s = in + r * inner + c;
-        uint32_t w[4];
+    constexpr int kWords = 16 / (int)sizeof(T);
+    T w[kWords];
 #pragma unroll
-        for (int j = 0; j < 4; j++)
+    for (int i = 0; i < kWords; i++)
+        w[i] = (int64_t)(i * sizeof(T)) < left ? reinterpret_cast<const T*>(src)[i] : T(0);
+    return *reinterpret_cast<const uint4*>(w);
+}
+
+// All copies of a call in one launch, a thread for sixteen bytes of a result row.  Words as wide as rows and addresses allow.  Split rows: an fp32 row
+// becomes three bf16 rows whose sum it is: the leading eight bits of the significand, the next eight, and the rest; every part is cut
+// off, not rounded, so that none overflows and the last is exact.  What is not finite goes into the first part alone.
+__global__ void __launch_bounds__(kSmallThreads) row_copies_kernel(const __grid_constant__ RowCopies q)
+{
+    ptx::dep_launch_trigger();
+    ptx::dep_launch_wait();
+    for (int64_t i = (int64_t)blockIdx.x * kSmallThreads + threadIdx.x; i < q.items[q.n - 1]; i += (int64_t)gridDim.x * kSmallThreads)
+    {
+        int k = 0;
+        while (i >= q.items[k])
+            k++;
+        const RowCopy& c  = q.copy[k];
+        const int64_t at  = i - (k ? q.items[k - 1] : 0), runs = c.pitch / 16;
+        const int64_t row = at / runs, byte = (at - row * runs) * 16;
+        if (c.split)
         {
-            const uint32_t lo = c + 2 * j < inner ? s[2 * j] : 0, hi = c + 2 * j + 1 < inner ? s[2 * j + 1] : 0;
-            w[j]              = lo | hi << 16;
-        }
-        *reinterpret_cast<uint4*>(out + r * pitch + c) = make_uint4(w[0], w[1], w[2], w[3]);
-    }
-}
-
-// fp32 rows as three bf16 rows each: the leading eight bits of the significand, the next eight, and the rest; every part is cut off, not rounded, so
-// that none overflows and the last is exact.  What is not finite goes into the first part alone.
-__global__ void __launch_bounds__(kSmallThreads) split_rows_kernel(const float* __restrict__ in, uint16_t* __restrict__ out, int64_t rows, int64_t inner,
-                                                                   int64_t pitch)
-{
-    const int64_t n = rows * inner;
-    for (int64_t i = (int64_t)blockIdx.x * kSmallThreads + threadIdx.x; i < n; i += (int64_t)gridDim.x * kSmallThreads)
-    {
-        const int64_t r = i / inner, c = i - r * inner;
-        const float x        = in[i];
-        const uint32_t bits  = __float_as_uint(x);
-        const bool finite    = (bits & 0x7F800000u) != 0x7F800000u;
-        const uint32_t first = (bits & 0x7FFFFFFFu) > 0x7F800000u ? 0x7FC00000u : bits & 0xFFFF0000u;
-        const float rest     = finite ? x - __uint_as_float(first) : 0.f;
-        const uint32_t mid   = __float_as_uint(rest) & 0xFFFF0000u;
-        const uint32_t last  = __float_as_uint(rest - __uint_as_float(mid));
-        uint16_t* o          = out + 3 * r * pitch + c;
-        o[0]                 = (uint16_t)(first >> 16);
-        o[pitch]             = (uint16_t)(mid >> 16);
-        o[2 * pitch]         = (uint16_t)(last >> 16);
-    }
-}
-
-// Rows of bytes that start anywhere; a thread writes sixteen.
-__global__ void __launch_bounds__(kSmallThreads) byte_copy_kernel(const uint8_t* __restrict__ in, uint8_t* __restrict__ out, int64_t rows, int64_t inner,
-                                                                  int64_t in_pitch, int64_t pitch)
-{
-    const int64_t runs = pitch / 16, n = rows * runs;
-    for (int64_t i = (int64_t)blockIdx.x * kSmallThreads + threadIdx.x; i < n; i += (int64_t)gridDim.x * kSmallThreads)
-    {
-        const int64_t r = i / runs, c = (i - r * runs) * 16;
-        const uint8_t* s = in + r * in_pitch + c;
-        uint32_t w[4]    = { 0, 0, 0, 0 };
+            // eight elements of the row and of its three parts
+            const float* const src = reinterpret_cast<const float*>(c.in + row * c.in_pitch) + byte / 2;
+            const int64_t left     = c.inner / 4 - byte / 2;
+            uint16_t part[3][8];
 #pragma unroll
-        for (int j = 0; j < 16; j++)
-            if (c + j < inner)
-                w[j >> 2] |= (uint32_t)s[j] << (8 * (j & 3));
-        *reinterpret_cast<uint4*>(out + r * pitch + c) = make_uint4(w[0], w[1], w[2], w[3]);
+            for (int e = 0; e < 8; e++)
+            {
+                const float x        = e < left ? src[e] : 0.f;
+                const uint32_t bits  = __float_as_uint(x);
+                const bool finite    = (bits & 0x7F800000u) != 0x7F800000u;
+                const uint32_t first = (bits & 0x7FFFFFFFu) > 0x7F800000u ? 0x7FC00000u : bits & 0xFFFF0000u;
+                const float rest     = finite ? x - __uint_as_float(first) : 0.f;
+                const uint32_t mid   = __float_as_uint(rest) & 0xFFFF0000u;
+                part[0][e]           = (uint16_t)(first >> 16);
+                part[1][e]           = (uint16_t)(mid >> 16);
+                part[2][e]           = (uint16_t)(__float_as_uint(rest - __uint_as_float(mid)) >> 16);
+            }
+#pragma unroll
+            for (int e = 0; e < 3; e++)
+                *reinterpret_cast<uint4*>(c.out + (3 * row + e) * c.pitch + byte) = *reinterpret_cast<const uint4*>(part[e]);
+            continue;
+        }
+        const uint8_t* const src = c.in + row * c.in_pitch + byte;
+        const int64_t left       = c.inner - byte;
+        const uint4 v            = c.word == 8   ? row_piece<uint64_t>(src, left)
+                                   : c.word == 4 ? row_piece<uint32_t>(src, left)
+                                   : c.word == 2 ? row_piece<uint16_t>(src, left)
+                                                 : row_piece<uint8_t>(src, left);
+        *reinterpret_cast<uint4*>(c.out + row * c.pitch + byte) = v;
     }
 }
 
@@ -241,16 +240,30 @@ __global__ void __launch_bounds__(256) transpose_f32_kernel(const float* __restr
 
 }    // namespace
 
-tb200_status split_rows_launch(tb200_ctx* ctx, const float* in, void* out, int64_t rows, int64_t inner, int64_t pitch)
+void RowCopies::add(const void* in, void* out, int64_t rows, int64_t inner, int64_t in_pitch, int64_t pitch, bool split)
 {
-    split_rows_kernel<<<small_grid(ctx, rows * inner), kSmallThreads, 0, ctx->stream>>>(in, reinterpret_cast<uint16_t*>(out), rows, inner, pitch);
-    return post_launch(ctx, "split_rows");
+    RowCopy& c = copy[n];
+    c.in       = reinterpret_cast<const uint8_t*>(in);
+    c.out      = reinterpret_cast<uint8_t*>(out);
+    c.inner    = inner;
+    c.in_pitch = in_pitch;
+    c.pitch    = pitch;
+    c.split    = split ? 1 : 0;
+    // a word never reaches behind the row: its width divides the row's length too
+    const uint64_t bits = (uint64_t)reinterpret_cast<uintptr_t>(in) | (uint64_t)in_pitch | (uint64_t)inner;
+    c.word              = bits % 8 == 0 ? 8 : bits % 4 == 0 ? 4 : bits % 2 == 0 ? 2 : 1;
+    items[n]            = (n ? items[n - 1] : 0) + rows * (pitch / 16);
+    n++;
 }
 
-tb200_status byte_copy_launch(tb200_ctx* ctx, const uint8_t* in, uint8_t* out, int64_t rows, int64_t inner, int64_t in_pitch, int64_t pitch)
+tb200_status row_copies_launch(tb200_ctx* ctx, const RowCopies& q)
 {
-    byte_copy_kernel<<<small_grid(ctx, rows * (pitch / 16)), kSmallThreads, 0, ctx->stream>>>(in, out, rows, inner, in_pitch, pitch);
-    return post_launch(ctx, "byte_copy");
+    if (q.n == 0 || q.items[q.n - 1] == 0)
+        return TB200_OK;
+    const cudaError_t e = launch_overlapped(ctx, row_copies_kernel, small_grid(ctx, q.items[q.n - 1]), q);
+    if (e != cudaSuccess)
+        return fail(ctx, TB200_INTERNAL, "launch of row_copies failed: %s", cudaGetErrorString(e));
+    return post_launch(ctx, "row_copies");
 }
 
 tb200_status w4_dense_launch(tb200_ctx* ctx, const W4Mat& w, int C, int W, int group, tb200_dtype dt, void* out, int64_t pitch)
@@ -285,13 +298,6 @@ tb200_status transpose_f32_launch(tb200_ctx* ctx, const float* in, float* out, i
     const int64_t tr = (R + 31) / 32, tc = (C + 31) / 32, n = batches * tr * tc;
     transpose_f32_kernel<<<(unsigned)std::min<int64_t>(n, (int64_t)ctx->num_sms * 8), 256, 0, ctx->stream>>>(in, out, R, C, out_batch, tr, tc, n);
     return post_launch(ctx, "transpose_f32");
-}
-
-tb200_status pitch_copy_launch(tb200_ctx* ctx, const void* in, void* out, int64_t rows, int64_t inner, int64_t pitch)
-{
-    pitch_copy_kernel<<<small_grid(ctx, rows * (pitch / 8)), kSmallThreads, 0, ctx->stream>>>(reinterpret_cast<const uint16_t*>(in),
-                                                                                             reinterpret_cast<uint16_t*>(out), rows, inner, pitch);
-    return post_launch(ctx, "pitch_copy");
 }
 
 }    // namespace ffn

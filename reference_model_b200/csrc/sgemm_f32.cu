@@ -479,20 +479,36 @@ __global__ void transpose_weights_f32_kernel(const float* __restrict__ w, float*
 
 }    // namespace
 
-tb200_status sgemm_f32_launch(tb200_ctx* ctx, const float* a, const float* b, float* out, int N, int H, int C, int W)
+static tb200_status sgemm_f32_run(tb200_ctx* ctx, const float* a, const float* b, float* out, int N, int H, int C, int W, int64_t a_batch, int64_t b_batch,
+                                  int64_t o_batch)
 {
     SgemmParams p;
     memset(&p, 0, sizeof(p));
     p.a = a; p.b = b; p.out = out;
     p.M = H; p.N = W; p.K = C; p.ldb = W;
-    p.a_batch = (int64_t)H * C; p.b_batch = (int64_t)C * W; p.o_batch = (int64_t)H * W;
+    p.a_batch = a_batch; p.b_batch = b_batch; p.o_batch = o_batch;
     const SgemmPlan plan = choose(ctx, p, N);
     const double split   = sgemm_split_cost(ctx, N, H, W, C, false);
     if (split > 0 && split < plan.cost)
-        return sgemm_split_launch(ctx, a, b, out, N, H, C, W);
-    const bool vec = (W % 4) == 0 && (C % 4) == 0 && ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b)) & 15) == 0;
+        return sgemm_split_launch(ctx, a, b, out, N, H, C, W, a_batch, b_batch, o_batch);
+    const bool vec = (W % 4) == 0 && (C % 4) == 0 && b_batch % 4 == 0 &&
+                     ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b)) & 15) == 0;
     const tb200_status st = vec ? launch_any<false, true>(ctx, p, N, plan) : launch_any<false, false>(ctx, p, N, plan);
     return st != TB200_OK ? st : post_launch(ctx, "sgemm_f32");
+}
+
+tb200_status sgemm_f32_launch(tb200_ctx* ctx, const float* a, const float* b, float* out, int N, int H, int C, int W)
+{
+    return sgemm_f32_run(ctx, a, b, out, N, H, C, W, (int64_t)H * C, (int64_t)C * W, (int64_t)H * W);
+}
+
+tb200_status sgemm_f32_two_launch(tb200_ctx* ctx, const float* a, const float* b0, const float* b1, float* out0, float* out1, int H, int C, int W)
+{
+    // two batches: the same a, second operands and results as far apart as they lie
+    auto apart = [](const float* x, const float* y) {
+        return ((int64_t)reinterpret_cast<uintptr_t>(y) - (int64_t)reinterpret_cast<uintptr_t>(x)) / (int64_t)sizeof(float);
+    };
+    return sgemm_f32_run(ctx, a, b0, out0, 2, H, C, W, 0, apart(b0, b1), apart(out0, out1));
 }
 
 int conv_f32_ldb(int OC)

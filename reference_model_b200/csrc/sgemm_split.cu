@@ -804,15 +804,15 @@ double sgemm_split_cost(const tb200_ctx* ctx, int64_t batches, int64_t M, int64_
     return rounds * ((double)((K + kStageK - 1) / kStageK) * stage + 1500.0) + 5000.0;
 }
 
-tb200_status sgemm_split_launch(tb200_ctx* ctx, const float* a, const float* b, float* out, int N, int H, int C, int W)
+tb200_status sgemm_split_launch(tb200_ctx* ctx, const float* a, const float* b, float* out, int N, int H, int C, int W, int64_t a_batch, int64_t b_batch, int64_t o_batch)
 {
     SplitParams p;
     memset(&p, 0, sizeof(p));
     p.a = a; p.b = b; p.out = out;
     p.M = H; p.N = W; p.K = C; p.ldb = W;
-    p.a_batch = (int64_t)H * C; p.b_batch = (int64_t)C * W; p.o_batch = (int64_t)H * W;
+    p.a_batch = a_batch; p.b_batch = b_batch; p.o_batch = o_batch;
     finish_split(ctx, p, N);
-    const bool vec = (W % 2) == 0 && (C % 2) == 0 && ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b)) & 7) == 0;
+    const bool vec = (W % 2) == 0 && (C % 2) == 0 && b_batch % 2 == 0 && ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b)) & 7) == 0;
     const tb200_status st = vec ? launch_split<false, true, true>(ctx, p) : launch_split<false, false, false>(ctx, p);
     return st != TB200_OK ? st : post_launch(ctx, "sgemm_f32");
 }
