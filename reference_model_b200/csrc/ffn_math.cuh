@@ -133,6 +133,30 @@ __device__ __forceinline__ void act_slope(int act, float g, float& value, float&
     }
 }
 
+__device__ __forceinline__ float act_value_16(int act, float g)
+{
+    switch (act)
+    {
+        case TB200_ACT_SILU: return act_value_16<TB200_ACT_SILU>(g);
+        case TB200_ACT_GELU: return act_value_16<TB200_ACT_GELU>(g);
+        case TB200_ACT_GELU_TANH: return act_value_16<TB200_ACT_GELU_TANH>(g);
+        case TB200_ACT_RELU: return act_value_16<TB200_ACT_RELU>(g);
+        default: return act_value_16<TB200_ACT_SIGMOID>(g);
+    }
+}
+
+__device__ __forceinline__ void act_slope_16(int act, float g, float& value, float& slope)
+{
+    switch (act)
+    {
+        case TB200_ACT_SILU: act_slope_16<TB200_ACT_SILU>(g, value, slope); break;
+        case TB200_ACT_GELU: act_slope_16<TB200_ACT_GELU>(g, value, slope); break;
+        case TB200_ACT_GELU_TANH: act_slope_16<TB200_ACT_GELU_TANH>(g, value, slope); break;
+        case TB200_ACT_RELU: act_slope_16<TB200_ACT_RELU>(g, value, slope); break;
+        default: act_slope_16<TB200_ACT_SIGMOID>(g, value, slope); break;
+    }
+}
+
 __device__ __forceinline__ float load_fp(const void* p, int64_t i, tb200_dtype dt)
 {
     if (dt == TB200_FP32)

@@ -163,22 +163,46 @@ __device__ __forceinline__ void grad_run(const uint32_t (&g)[16], const uint32_t
     }
 }
 
-// Sixteen neighbouring columns of a row of the tile, all sums there: results, activated and multiplied, or the two gradients.
+// Sixteen neighbouring columns of a row of the tile, all sums there: results, activated and multiplied, or the two gradients.  The
+// warp's lanes are 32 rows of the tile and call together: rows that may not be stored sixteen bytes at a time go through `stage` (32 x 17 words
+// of the warp's own) and out sixteen neighbouring columns of two rows at a time (a row a lane, one element at a time, touched 32 sectors with every
+// store: gradients of 6 x 280 x 2758 took 150 us).
 template <int EPI>
-__device__ __forceinline__ void finish_run(const Params& p, const Tile& t, int row, int run, const uint32_t (&g)[16], const uint32_t (&u)[16])
+__device__ __forceinline__ void finish_run(const Params& p, const Tile& t, int row, int run, const uint32_t (&g)[16], const uint32_t (&u)[16], float* stage)
 {
     const int m = t.m0 + row, col = t.n0 + run, n = min(16, p.cols - col);
-    if (m >= p.rows)
+    const bool valid = m < p.rows, together = p.vec == 0;
+    if (!valid && !together)
         return;
     const int batch    = t.idx < p.NB ? t.idx : t.idx - p.NB;
     const int64_t orow = ((int64_t)batch * p.rows + m) * p.ld;
+    auto emit          = [&](void* out, tb200_dtype dt, const float (&v)[16]) {
+        if (!together)
+        {
+            store_run(out, orow + col, dt, n, p.vec, v);
+            return;
+        }
+        const int lane = threadIdx.x & 31;
+#pragma unroll
+        for (int i = 0; i < 16; i++)
+            stage[lane * 17 + i] = v[i];
+        __syncwarp();
+#pragma unroll 4
+        for (int i = 0; i < 16; i++)
+        {
+            const int r = 2 * i + (lane >> 4), c = lane & 15;
+            if (m - lane + r < p.rows && c < n)
+                store_fp(out, orow + (int64_t)(r - lane) * p.ld + col + c, dt, stage[r * 17 + c]);
+        }
+        __syncwarp();
+    };
     if (EPI == EPI_PLAIN)
     {
         float v[16];
 #pragma unroll
         for (int i = 0; i < 16; i++)
             v[i] = __uint_as_float(g[i]);
-        store_run(t.idx < p.NB ? p.out0 : p.out1, orow + col, t.idx < p.NB ? p.out_dt : p.out1_dt, n, p.vec, v);
+        emit(t.idx < p.NB ? p.out0 : p.out1, t.idx < p.NB ? p.out_dt : p.out1_dt, v);
     }
     else if (EPI == EPI_GATED)
     {
@@ -191,13 +215,13 @@ __device__ __forceinline__ void finish_run(const Params& p, const Tile& t, int r
             case TB200_ACT_RELU: gate_run<TB200_ACT_RELU>(g, u, v); break;
             default: gate_run<TB200_ACT_SIGMOID>(g, u, v); break;
         }
-        store_run(p.out0, orow + col, p.out_dt, n, p.vec, v);
+        emit(p.out0, p.out_dt, v);
     }
     else
     {
         float d[16], dg[16], du[16];
         const uint16_t* const s = reinterpret_cast<const uint16_t*>(p.dout) + ((int64_t)batch * p.rows + m) * p.cols + col;
-        if (n == 16 && p.dout_vec)
+        if (valid && n == 16 && p.dout_vec)
         {
             const uint4 lo = *reinterpret_cast<const uint4*>(s), hi = *(reinterpret_cast<const uint4*>(s) + 1);
             const uint32_t w[8] = { lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w };
@@ -213,7 +237,7 @@ __device__ __forceinline__ void finish_run(const Params& p, const Tile& t, int r
         {
 #pragma unroll
             for (int i = 0; i < 16; i++)
-                d[i] = i < n ? unpack2(s[i], p.bf16 != 0).x : 0.f;
+                d[i] = valid && i < n ? unpack2(s[i], p.bf16 != 0).x : 0.f;
         }
         switch (p.act)
         {
@@ -223,8 +247,60 @@ __device__ __forceinline__ void finish_run(const Params& p, const Tile& t, int r
             case TB200_ACT_RELU: grad_run<TB200_ACT_RELU>(g, u, d, dg, du); break;
             default: grad_run<TB200_ACT_SIGMOID>(g, u, d, dg, du); break;
         }
-        store_run(p.out0, orow + col, p.out_dt, n, p.vec, dg);
-        store_run(p.out1, orow + col, p.out_dt, n, p.vec, du);
+        emit(p.out0, p.out_dt, dg);
+        emit(p.out1, p.out_dt, du);
+    }
+}
+
+__device__ __forceinline__ void store_quad(void* base, int64_t at, tb200_dtype dt, int n, int vec, const float (&v)[4])
+{
+    if (n == 4 && vec > 0)
+    {
+        if (dt == TB200_FP32)
+            *reinterpret_cast<float4*>(reinterpret_cast<float*>(base) + at) = make_float4(v[0], v[1], v[2], v[3]);
+        else
+            *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(base) + at) =
+                make_uint2(pack2(v[0], v[1], dt == TB200_BF16), pack2(v[2], v[3], dt == TB200_BF16));
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        if (i < n)
+            store_fp(base, at + i, dt, v[i]);
+}
+
+// The same for four columns, whichever thread has them.
+template <int EPI>
+__device__ __forceinline__ void finish_quad(const Params& p, const Tile& t, int row, int run, const float (&g)[4], const float (&u)[4])
+{
+    const int m = t.m0 + row, col = t.n0 + run, n = min(4, p.cols - col);
+    const int batch    = t.idx < p.NB ? t.idx : t.idx - p.NB;
+    const int64_t orow = ((int64_t)batch * p.rows + m) * p.ld + col;
+    if (EPI == EPI_PLAIN)
+        store_quad(t.idx < p.NB ? p.out0 : p.out1, orow, t.idx < p.NB ? p.out_dt : p.out1_dt, n, p.vec, g);
+    else if (EPI == EPI_GATED)
+    {
+        float v[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            v[i] = act_value_16(p.act, g[i]) * u[i];
+        store_quad(p.out0, orow, p.out_dt, n, p.vec, v);
+    }
+    else
+    {
+        const int64_t at = ((int64_t)batch * p.rows + m) * p.cols + col;
+        float dg[4], du[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+        {
+            const float d = i < n ? load_fp(p.dout, at + i, p.bf16 ? TB200_BF16 : TB200_FP16) : 0.f;
+            float value, slope;
+            act_slope_16(p.act, g[i], value, slope);
+            dg[i] = d * u[i] * slope;
+            du[i] = d * value;
+        }
+        store_quad(p.out0, orow, p.out_dt, n, p.vec, dg);
+        store_quad(p.out1, orow, p.out_dt, n, p.vec, du);
     }
 }
 
@@ -242,6 +318,7 @@ __global__ void __launch_bounds__(kThreads, 1) ffn_pair_kernel(const __grid_cons
     __shared__ __align__(8) uint64_t bar_ready;                // first CTA: tensor memory taken in both
     __shared__ __align__(8) uint64_t bar_drain;                // first CTA: MMAs in flight when the issuer gives up
     __shared__ uint32_t tmem_base_holder;
+    __shared__ float stages[kEpiWarps][32 * 17];    // of the epilogue's warps
 
     const int warp           = threadIdx.x >> 5;
     const int lane           = threadIdx.x & 31;
@@ -506,6 +583,7 @@ __global__ void __launch_bounds__(kThreads, 1) ffn_pair_kernel(const __grid_cons
         const int quarter = warp & 3;           // TMEM lane quarter this warp may read
         const int slot    = (warp - 2) >> 2;    // the two warps of a quarter take 16-column runs in turn
         const int row     = quarter * 32 + lane;
+        float* const stage = stages[warp - 2];
         const uint32_t empty_first[2] = { PAIR ? ptx::map_to_cta(ptx::smem_u32(&bar_tmem_empty[0]), 0) : ptx::smem_u32(&bar_tmem_empty[0]),
                                           PAIR ? ptx::map_to_cta(ptx::smem_u32(&bar_tmem_empty[1]), 0) : ptx::smem_u32(&bar_tmem_empty[1]) };
         int acc            = 0;
@@ -544,7 +622,7 @@ __global__ void __launch_bounds__(kThreads, 1) ffn_pair_kernel(const __grid_cons
                     uint32_t g[16];
                     ptx::tmem_ld_32x32b_x16(taddr + (uint32_t)(c * 16), g);
                     ptx::tmem_ld_wait_x16(g);
-                    finish_run<EPI>(p, t, (int)rank * 128 + row, c * 16, g, g);
+                    finish_run<EPI>(p, t, (int)rank * 128 + row, c * 16, g, g, stage);
                 }
             }
             else
@@ -558,7 +636,7 @@ __global__ void __launch_bounds__(kThreads, 1) ffn_pair_kernel(const __grid_cons
                     ptx::tmem_ld_32x32b_x16(taddr + (uint32_t)(kHalf + c * 16), u);
                     ptx::tmem_ld_wait_x16(g);
                     ptx::tmem_ld_wait_x16(u);
-                    finish_run<EPI>(p, t, (int)rank * 128 + row, c * 16, g, u);
+                    finish_run<EPI>(p, t, (int)rank * 128 + row, c * 16, g, u, stage);
                 }
             }
             // this warp has read its part of the buffer: one arrival per warp on the first CTA's barrier
@@ -585,52 +663,42 @@ __global__ void __launch_bounds__(kThreads, 1) ffn_pair_kernel(const __grid_cons
         // A share whose wait gave up holds sums that do not count; every share reaches both barriers.
         ptx::cluster_sync();
         const Tile t         = decode<EPI, PAIR>(p, cluster_id);
-        constexpr int kRuns  = (EPI == EPI_PLAIN ? S::kCols : kHalf) / 16;    // of a row
+        constexpr int kQuads = (EPI == EPI_PLAIN ? S::kCols : kHalf) / 4;    // of a row
         const uint32_t local = ptx::smem_u32(red);
-        for (int e = share * kThreads + (int)threadIdx.x; e < 128 * kRuns; e += p.splits * kThreads)
+        // four neighbouring columns a thread, the shares' sums all on their way before the first is added (sixteen columns, a share at a
+        // time, took 2 to 8 us)
+        for (int e = share * kThreads + (int)threadIdx.x; e < 128 * kQuads; e += p.splits * kThreads)
         {
-            const int r = e / kRuns, run = e % kRuns * 16;
-            if (t.m0 + r >= p.rows || t.n0 + run >= p.cols)
+            const int r = e / kQuads, col = e % kQuads * 4;
+            if (t.m0 + r >= p.rows || t.n0 + col >= p.cols)
                 continue;
-            uint32_t g[16], u[16];
-            auto sum = [&](int col, uint32_t (&v)[16]) {
-                float total[16];
+            auto sum = [&](int c, float (&v)[4]) {
+                float4 x[8];
+                const uint32_t at = local + (uint32_t)((r * S::kRedLd + c) * 4);
 #pragma unroll
-                for (int i = 0; i < 16; i++)
-                    total[i] = 0.f;
-                for (int k = 0; k < p.splits; k++)
-                {
-                    const uint32_t at = ptx::map_to_cta(local + (uint32_t)((r * S::kRedLd + col) * 4), (uint32_t)k);
-                    float4 x[4];
-#pragma unroll
-                    for (int i = 0; i < 4; i++)
+                for (int k = 0; k < 8; k++)
+                    if (k < p.splits)
                         asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                                     : "=f"(x[i].x), "=f"(x[i].y), "=f"(x[i].z), "=f"(x[i].w)
-                                     : "r"(at + (uint32_t)(16 * i))
+                                     : "=f"(x[k].x), "=f"(x[k].y), "=f"(x[k].z), "=f"(x[k].w)
+                                     : "r"(ptx::map_to_cta(at, (uint32_t)k))
                                      : "memory");
+                    else
+                        x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                v[0] = v[1] = v[2] = v[3] = 0.f;
 #pragma unroll
-                    for (int i = 0; i < 4; i++)
-                    {
-                        total[4 * i] += x[i].x;
-                        total[4 * i + 1] += x[i].y;
-                        total[4 * i + 2] += x[i].z;
-                        total[4 * i + 3] += x[i].w;
-                    }
+                for (int k = 0; k < 8; k++)
+                {
+                    v[0] += x[k].x;
+                    v[1] += x[k].y;
+                    v[2] += x[k].z;
+                    v[3] += x[k].w;
                 }
-#pragma unroll
-                for (int i = 0; i < 16; i++)
-                    v[i] = __float_as_uint(total[i]);
             };
-            sum(run, g);
+            float g[4], u[4] = {};
+            sum(col, g);
             if (EPI != EPI_PLAIN)
-                sum(kHalf + run, u);
-            else
-            {
-#pragma unroll
-                for (int i = 0; i < 16; i++)
-                    u[i] = 0;
-            }
-            finish_run<EPI>(p, t, r, run, g, u);
+                sum(kHalf + col, u);
+            finish_quad<EPI>(p, t, r, col, g, u);
         }
         ptx::cluster_sync();    // nobody leaves while another share may still read its sums
     }
@@ -795,8 +863,9 @@ tb200_status launch(tb200_ctx* ctx, const PairProduct& q, int splits)
 
 tb200_status pair_launch(tb200_ctx* ctx, const PairProduct& q)
 {
-    // Pairs, or CTAs by themselves, K shared by up to eight: by their cycles.  A chunk of K takes a pair 520 and a CTA by itself 330; the last
-    // tile's epilogue shows, and so does the exchange of the shares' sums.
+    // Pairs, or CTAs by themselves, K shared by up to eight: by their cycles.  A chunk of K takes a pair 520 and a CTA by itself 330, up to 700 when
+    // all SMs run one, since their smaller tiles move twice the bytes for a product; the last tile's epilogue shows, and so does the exchange
+    // of the shares' sums.
     const bool gated     = q.kind != PAIR_PLAIN;
     const int64_t copies = (int64_t)q.NB * (q.results == 2 && !gated ? 2 : 1), chunks = (q.K + 63) / 64 * q.phases;
     auto tiles = [&](int rows, int cols) { return (int64_t)((q.rows + rows - 1) / rows) * ((q.cols + cols - 1) / cols) * copies; };
@@ -808,7 +877,8 @@ tb200_status pair_launch(tb200_ctx* ctx, const PairProduct& q)
     {
         if (s > 1 && (chunks < 4 * s || small * s > ctx->num_sms))
             break;
-        const double cost = waves(small * s, ctx->num_sms) * (double)((chunks + s - 1) / s) * 330.0 + 2500.0 + (s > 1 ? 2500.0 : 0.0);
+        const double chunk = std::max(330.0, 700.0 * (double)std::min<int64_t>(small * s, ctx->num_sms) / ctx->num_sms);
+        const double cost  = waves(small * s, ctx->num_sms) * (double)((chunks + s - 1) / s) * chunk + 2500.0 + (s > 1 ? 2500.0 : 0.0);
         if (cost < best)
         {
             best   = cost;
