@@ -178,7 +178,7 @@ struct tb200_ctx
     std::unique_ptr<tb200::SizeMemo<tb200::DwPieces>> dw_memo;
     int dw_blocks[16]    = {};             // resident blocks per SM of the sliding depthwise kernels, 0 = not asked yet
     int rows_blocks[12]  = {};             // ... of the kernels for MATMUL with up to four rows
-    std::bitset<192> smem_attr_set;        // bit per kernel whose dynamic shared-memory limit has been raised on this device
+    std::bitset<256> smem_attr_set;        // bit per kernel whose dynamic shared-memory limit has been raised on this device
     // output gather across GPUs (dist.cu): an NCCL communicator created by tb200_comm_init or handed in by the host
     void* comm           = nullptr;
     bool comm_owned      = false;

@@ -301,18 +301,13 @@ tb200_status w4_launch(tb200_ctx* ctx, const W4Problem& q)
     const bool copy_x    = !f32 && q.C % 8 != 0;
     const int64_t n      = q.M * q.W;
     Carver c;
-    // few rows: TMA wants rows of bytes, scales and zero points a multiple of 16 bytes apart
-    const int64_t groups = ((int64_t)q.C + q.group - 1) / q.group;
-    auto scale_row       = [&](int i) { return (int64_t)q.W * (int64_t)dtype_size(q.w[i].scale_dt); };
-    void *x = nullptr, *w[2] = {}, *proj[2] = {}, *partial = nullptr, *scale[2] = {}, *zero[2] = {};
+    void *x = nullptr, *w[2] = {}, *proj[2] = {}, *partial = nullptr;
     for (int pass = 0; pass < 2; pass++)
     {
         x = c.take(few && f32 ? (size_t)q.M * 3 * xpitch * 2 : copy_x ? (size_t)q.M * xpitch * 2 : 0);
         for (int i = 0; i < q.mats; i++)
         {
             w[i]    = c.take(few ? (q.w[i].pitch % 16 ? (size_t)q.W * wpitch : 0) : f32 ? (size_t)q.C * q.W * 4 : (size_t)q.W * dpitch * 2);
-            scale[i] = c.take(few && scale_row(i) % 16 ? (size_t)groups * round_up(scale_row(i), 16) : 0);
-            zero[i]  = c.take(few && q.w[i].zero && q.W % 16 ? (size_t)groups * round_up(q.W, 16) : 0);
             proj[i] = c.take(!few && f32 && q.mats == 2 ? (size_t)n * 4 : 0);
         }
         partial = c.take(few ? w4_rows_partial_bytes(ctx, q.M * parts) : 0);
@@ -329,27 +324,12 @@ tb200_status w4_launch(tb200_ctx* ctx, const W4Problem& q)
         W4Problem r = q;
         RowCopies copies;
         for (int i = 0; i < q.mats; i++)
-        {
-            if (scale_row(i) % 16)
-            {
-                const int64_t row = round_up(scale_row(i), 16);
-                copies.add(q.w[i].scale, scale[i], groups, scale_row(i), scale_row(i), row);
-                r.w[i].scale       = scale[i];
-                r.w[i].scale_pitch = row / (int64_t)dtype_size(q.w[i].scale_dt);
-            }
-            if (q.w[i].zero && q.W % 16)
-            {
-                copies.add(q.w[i].zero, zero[i], groups, q.W, q.W, round_up(q.W, 16));
-                r.w[i].zero       = reinterpret_cast<const int8_t*>(zero[i]);
-                r.w[i].zero_pitch = round_up(q.W, 16);
-            }
             if (q.w[i].pitch % 16)
             {
                 copies.add(q.w[i].data, w[i], q.W, (q.C + 1) / 2, q.w[i].pitch, wpitch);
                 r.w[i].data  = reinterpret_cast<const uint8_t*>(w[i]);
                 r.w[i].pitch = wpitch;
             }
-        }
         if (f32)
             copies.add(q.a, x, q.M, (int64_t)q.C * 4, (int64_t)q.C * 4, xpitch * 2, true);
         else if (copy_x)
@@ -358,8 +338,7 @@ tb200_status w4_launch(tb200_ctx* ctx, const W4Problem& q)
         return w4_rows_launch(ctx, r, f32 || copy_x ? x : q.a, f32 || copy_x ? xpitch : q.C, parts, f32 || q.dt == TB200_BF16,
                               reinterpret_cast<float*>(partial));
     }
-    for (int i = 0; i < q.mats; i++)
-        TB200_TRY(w4_dense_launch(ctx, q.w[i], q.C, q.W, q.group, q.dt, w[i], dpitch));
+    TB200_TRY(w4_dense_launch(ctx, q.w, q.mats, q.C, q.W, q.group, q.dt, w, dpitch));
     if (f32)
     {
         for (int i = 0; i < q.mats; i++)
@@ -441,7 +420,6 @@ tb200_status w4_entry(tb200_ctx* ctx, const char* op, const tb200_tensor* a, con
         q.w[i].pitch    = mats[i]->data->shape[1];
         q.w[i].scale    = mats[i]->scale->data;
         q.w[i].scale_dt = mats[i]->scale->dtype;
-        q.w[i].scale_pitch = q.w[i].zero_pitch = q.W;
         q.w[i].zero     = mats[i]->zero ? reinterpret_cast<const int8_t*>(mats[i]->zero->data) : nullptr;
     }
     return ctx->policy == 0 && tiles_reach(q.M, q.C, q.W) ? w4_launch(ctx, q) : w4_direct_launch(ctx, q);

@@ -19,7 +19,6 @@ struct W4Mat
     const void* scale;
     const int8_t* zero;    // or null
     tb200_dtype scale_dt;
-    int64_t scale_pitch, zero_pitch;    // elements from one group's to the next
 };
 
 struct W4Problem
@@ -98,7 +97,7 @@ tb200_status gated_rows_launch(tb200_ctx* ctx, const PairProduct& q);
 
 // ---- w4_rows.cu: up to 64 16-bit rows against 4-bit weights
 // x: a's rows in 16 bits, `x_pitch` elements apart (a multiple of 8), 16-byte aligned; fp32 rows as three bf16 rows each (parts 3,
-// bf16).  The pitches of the weights, scales and zero points are multiples of 16 bytes.
+// bf16).  The weights' pitch is a multiple of 16 bytes.
 tb200_status w4_rows_launch(tb200_ctx* ctx, const W4Problem& q, const void* x, int64_t x_pitch, int parts, bool bf16, float* partial);
 size_t w4_rows_partial_bytes(const tb200_ctx* ctx, int64_t xrows);
 
@@ -109,7 +108,7 @@ struct RowCopy
 {
     const uint8_t* in;
     uint8_t* out;
-    int64_t inner, in_pitch, pitch;
+    int64_t inner, in_pitch, pitch, bytes;    // bytes: of the whole operand
     int word, split;
 };
 struct RowCopies
@@ -120,8 +119,8 @@ struct RowCopies
     void add(const void* in, void* out, int64_t rows, int64_t inner, int64_t in_pitch, int64_t pitch, bool split = false);
 };
 tb200_status row_copies_launch(tb200_ctx* ctx, const RowCopies& q);
-// [W][pitch] 16-bit rows of a 4-bit matrix's values, or fp32 [C][W] (dt FP32)
-tb200_status w4_dense_launch(tb200_ctx* ctx, const W4Mat& w, int C, int W, int group, tb200_dtype dt, void* out, int64_t pitch);
+// [W][pitch] 16-bit rows of one or two 4-bit matrices' values, or fp32 [C][W] (dt FP32)
+tb200_status w4_dense_launch(tb200_ctx* ctx, const W4Mat* w, int mats, int C, int W, int group, tb200_dtype dt, void* const* out, int64_t pitch);
 tb200_status gate_f32_launch(tb200_ctx* ctx, const float* g, const float* u, float* out, int64_t n, int act);
 // g and u hold dG and dU afterwards, `both` (or null) the two side by side
 tb200_status grad_f32_launch(tb200_ctx* ctx, float* g, float* u, const float* d, float* both, int64_t rows, int W, int act);

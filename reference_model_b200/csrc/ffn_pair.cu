@@ -67,6 +67,7 @@ struct Params
     tb200_dtype out1_dt;
     int64_t ld;
     int vec;               // whole 16-element runs of a result's row may be stored 32 bytes at a time (2), 16 (1), or not (0)
+    int even;              // whole pairs of elements in every row, at 4-byte addresses
     const void* dout;      // [NB][rows][cols]
     int dout_vec;          // its rows may be read 16 bytes at a time
     long long wait_limit;
@@ -187,12 +188,27 @@ __device__ __forceinline__ void finish_run(const Params& p, const Tile& t, int r
         for (int i = 0; i < 16; i++)
             stage[lane * 17 + i] = v[i];
         __syncwarp();
-#pragma unroll 4
-        for (int i = 0; i < 16; i++)
+        if (p.even && dt != TB200_FP32)
         {
-            const int r = 2 * i + (lane >> 4), c = lane & 15;
-            if (m - lane + r < p.rows && c < n)
-                store_fp(out, orow + (int64_t)(r - lane) * p.ld + col + c, dt, stage[r * 17 + c]);
+            // two elements at a time, four rows
+#pragma unroll 4
+            for (int i = 0; i < 8; i++)
+            {
+                const int r = 4 * i + (lane >> 3), c = (lane & 7) * 2;
+                if (m - lane + r < p.rows && c < n)
+                    *reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(out) + orow + (int64_t)(r - lane) * p.ld + col + c) =
+                        pack2(stage[r * 17 + c], stage[r * 17 + c + 1], dt == TB200_BF16);
+            }
+        }
+        else
+        {
+#pragma unroll 4
+            for (int i = 0; i < 16; i++)
+            {
+                const int r = 2 * i + (lane >> 4), c = lane & 15;
+                if (m - lane + r < p.rows && c < n)
+                    store_fp(out, orow + (int64_t)(r - lane) * p.ld + col + c, dt, stage[r * 17 + c]);
+            }
         }
         __syncwarp();
     };
@@ -817,6 +833,7 @@ tb200_status launch(tb200_ctx* ctx, const PairProduct& q, int splits)
     k.vec      = q.out[0] ? run_alignment(q.out[0], q.ld, dtype_size(q.out_dt[0])) : 2;
     if (q.out[1])
         k.vec = std::min(k.vec, run_alignment(q.out[1], q.ld, dtype_size(q.out_dt[1])));
+    k.even     = q.ld % 2 == 0 && q.cols % 2 == 0;
     k.dout     = q.dout;
     k.dout_vec = q.dout && run_alignment(q.dout, q.cols, 2) > 0;
     // K along the rows: 8-row groups of 128-byte swizzled rows 1024 bytes apart.  Across them: 64 columns of 64 K rows, the next 64

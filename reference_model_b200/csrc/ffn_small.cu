@@ -21,10 +21,10 @@ int small_grid(const tb200_ctx* ctx, int64_t items)
 
 // A launch that may start while the kernel before it drains (the kernel waits for it before it reads or writes).
 template <typename K, typename... A>
-cudaError_t launch_overlapped(tb200_ctx* ctx, K kernel, int grid, A... args)
+cudaError_t launch_overlapped(tb200_ctx* ctx, K kernel, dim3 grid, A... args)
 {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim            = dim3((unsigned)grid);
+    cfg.gridDim            = grid;
     cfg.blockDim           = dim3(kSmallThreads);
     cfg.stream             = ctx->stream;
     cudaLaunchAttribute at[1];
@@ -45,6 +45,36 @@ __device__ __forceinline__ uint4 row_piece(const uint8_t* src, int64_t left)
     for (int i = 0; i < kWords; i++)
         w[i] = (int64_t)(i * sizeof(T)) < left ? reinterpret_cast<const T*>(src)[i] : T(0);
     return *reinterpret_cast<const uint4*>(w);
+}
+
+// The same from any byte: the two aligned sixteens that hold it, shifted (two bytes at a time, copies ran at 2 TB/s)
+__device__ __forceinline__ uint4 row_piece_shifted(const uint8_t* src, int64_t left)
+{
+    const uintptr_t at = reinterpret_cast<uintptr_t>(src) & ~(uintptr_t)15;
+    const int by       = (int)(reinterpret_cast<uintptr_t>(src) & 15);
+    const uint4 lo = *reinterpret_cast<const uint4*>(at), hi = *reinterpret_cast<const uint4*>(at + 16);
+    uint32_t w[8] = { lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w };
+    if (by & 4)
+    {
+#pragma unroll
+        for (int i = 0; i < 7; i++)
+            w[i] = w[i + 1];
+    }
+    if (by & 8)
+    {
+#pragma unroll
+        for (int i = 0; i < 6; i++)
+            w[i] = w[i + 2];
+    }
+    uint32_t v[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+    {
+        v[i]           = __funnelshift_r(w[i], w[i + 1], (by & 3) * 8);
+        const int keep = (int)min((int64_t)4, left - 4 * i);    // bytes of the row
+        v[i]           = keep >= 4 ? v[i] : keep <= 0 ? 0u : v[i] & ((1u << (8 * keep)) - 1u);
+    }
+    return make_uint4(v[0], v[1], v[2], v[3]);
 }
 
 // All copies of a call in one launch, a thread for sixteen bytes of a result row.  Words as wide as rows and addresses allow.  Split rows: an fp32 row
@@ -88,7 +118,11 @@ __global__ void __launch_bounds__(kSmallThreads) row_copies_kernel(const __grid_
         }
         const uint8_t* const src = c.in + row * c.in_pitch + byte;
         const int64_t left       = c.inner - byte;
-        const uint4 v            = c.word == 8   ? row_piece<uint64_t>(src, left)
+        // both sixteens within the operand
+        const uintptr_t first = reinterpret_cast<uintptr_t>(src) & ~(uintptr_t)15;
+        const bool inside     = first >= reinterpret_cast<uintptr_t>(c.in) && first + 32 <= reinterpret_cast<uintptr_t>(c.in) + (uintptr_t)c.bytes;
+        const uint4 v            = inside        ? row_piece_shifted(src, left)
+                                   : c.word == 8 ? row_piece<uint64_t>(src, left)
                                    : c.word == 4 ? row_piece<uint32_t>(src, left)
                                    : c.word == 2 ? row_piece<uint16_t>(src, left)
                                                  : row_piece<uint8_t>(src, left);
@@ -99,8 +133,11 @@ __global__ void __launch_bounds__(kSmallThreads) row_copies_kernel(const __grid_
 // The values of a 4-bit matrix in 16 bits, rows [W][pitch], a value rounded once.  A warp takes 1024 elements of a row, a lane four runs of eight
 // (which share a group): it reads 128 bytes and writes 512 that follow one another at a time, all of a lane's loads on their way together
 // (32 neighbouring elements a thread, whose stores lay 64 bytes apart, took 19 us for 4096 x 4096; one run at a time 15 us).
-__global__ void __launch_bounds__(kSmallThreads) w4_dense_16_kernel(const W4Mat w, int C, int W, int group, bool bf16, uint16_t* out, int64_t pitch, int* status)
+__global__ void __launch_bounds__(kSmallThreads) w4_dense_16_kernel(const W4Mat w0, const W4Mat w1, int C, int W, int group, bool bf16, uint16_t* out0,
+                                                                    uint16_t* out1, int64_t pitch, int* status)
 {
+    const W4Mat& w      = blockIdx.y ? w1 : w0;
+    uint16_t* const out = blockIdx.y ? out1 : out0;
     ptx::dep_launch_trigger();
     ptx::dep_launch_wait();
     const int pieces    = (C + 1023) / 1024;    // of a row
@@ -120,8 +157,8 @@ __global__ void __launch_bounds__(kSmallThreads) w4_dense_16_kernel(const W4Mat 
         {
             const int c0 = min(first + 256 * e, C - 1) & ~7;    // the last run, more than once, where the row ends
             const int g  = (int)((uint32_t)c0 / (uint32_t)group);
-            s[e]         = load_fp(w.scale, g * w.scale_pitch + row, w.scale_dt);
-            z[e]         = w.zero ? (int)w.zero[g * w.zero_pitch + row] : 0;
+            s[e]         = load_fp(w.scale, (int64_t)g * W + row, w.scale_dt);
+            z[e]         = w.zero ? (int)w.zero[(int64_t)g * W + row] : 0;
             if (words)
                 b[e] = *reinterpret_cast<const uint32_t*>(src + c0 / 2);
             else
@@ -164,8 +201,8 @@ __global__ void __launch_bounds__(kSmallThreads) w4_dense_32_kernel(const W4Mat 
         const int64_t row = i % W, run = i / W;
         const int c0      = (int)(run * 32), count = min(32, C - c0);
         const int64_t g   = c0 / group;
-        const float s     = load_fp(w.scale, g * w.scale_pitch + row, w.scale_dt);
-        const int z       = w.zero ? (int)w.zero[g * w.zero_pitch + row] : 0;
+        const float s     = load_fp(w.scale, (int64_t)g * W + row, w.scale_dt);
+        const int z       = w.zero ? (int)w.zero[(int64_t)g * W + row] : 0;
         bad |= z < -8 || z > 7;
         const uint8_t* src = w.data + row * w.pitch + c0 / 2;
         uint32_t b[4]      = { 0, 0, 0, 0 };
@@ -249,6 +286,7 @@ void RowCopies::add(const void* in, void* out, int64_t rows, int64_t inner, int6
     c.in_pitch = in_pitch;
     c.pitch    = pitch;
     c.split    = split ? 1 : 0;
+    c.bytes    = rows ? (rows - 1) * in_pitch + inner : 0;
     // a word never reaches behind the row: its width divides the row's length too
     const uint64_t bits = (uint64_t)reinterpret_cast<uintptr_t>(in) | (uint64_t)in_pitch | (uint64_t)inner;
     c.word              = bits % 8 == 0 ? 8 : bits % 4 == 0 ? 4 : bits % 2 == 0 ? 2 : 1;
@@ -260,24 +298,26 @@ tb200_status row_copies_launch(tb200_ctx* ctx, const RowCopies& q)
 {
     if (q.n == 0 || q.items[q.n - 1] == 0)
         return TB200_OK;
-    const cudaError_t e = launch_overlapped(ctx, row_copies_kernel, small_grid(ctx, q.items[q.n - 1]), q);
+    const cudaError_t e = launch_overlapped(ctx, row_copies_kernel, dim3((unsigned)small_grid(ctx, q.items[q.n - 1])), q);
     if (e != cudaSuccess)
         return fail(ctx, TB200_INTERNAL, "launch of row_copies failed: %s", cudaGetErrorString(e));
     return post_launch(ctx, "row_copies");
 }
 
-tb200_status w4_dense_launch(tb200_ctx* ctx, const W4Mat& w, int C, int W, int group, tb200_dtype dt, void* out, int64_t pitch)
+tb200_status w4_dense_launch(tb200_ctx* ctx, const W4Mat* w, int mats, int C, int W, int group, tb200_dtype dt, void* const* out, int64_t pitch)
 {
     if (dt == TB200_FP32)
-        w4_dense_32_kernel<<<small_grid(ctx, (int64_t)((C + 31) / 32) * W), kSmallThreads, 0, ctx->stream>>>(w, C, W, group, reinterpret_cast<float*>(out),
-                                                                                                         ctx->d_status);
-    else
     {
-        const cudaError_t e = launch_overlapped(ctx, w4_dense_16_kernel, small_grid(ctx, (int64_t)((C + 1023) / 1024) * 32 * W), w, C, W, group, dt == TB200_BF16,
-                                                reinterpret_cast<uint16_t*>(out), pitch, ctx->d_status);
-        if (e != cudaSuccess)
-            return fail(ctx, TB200_INTERNAL, "launch of w4_dense failed: %s", cudaGetErrorString(e));
+        for (int i = 0; i < mats; i++)
+            w4_dense_32_kernel<<<small_grid(ctx, (int64_t)((C + 31) / 32) * W), kSmallThreads, 0, ctx->stream>>>(w[i], C, W, group,
+                                                                                                             reinterpret_cast<float*>(out[i]), ctx->d_status);
+        return post_launch(ctx, "w4_dense", mats);
     }
+    const cudaError_t e = launch_overlapped(ctx, w4_dense_16_kernel, dim3((unsigned)small_grid(ctx, (int64_t)((C + 1023) / 1024) * 32 * W), (unsigned)mats), w[0],
+                                            w[mats - 1], C, W, group, dt == TB200_BF16, reinterpret_cast<uint16_t*>(out[0]),
+                                            reinterpret_cast<uint16_t*>(out[mats - 1]), pitch, ctx->d_status);
+    if (e != cudaSuccess)
+        return fail(ctx, TB200_INTERNAL, "launch of w4_dense failed: %s", cudaGetErrorString(e));
     return post_launch(ctx, "w4_dense");
 }
 

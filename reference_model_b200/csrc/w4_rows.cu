@@ -1,31 +1,8 @@
-// Products with 4-bit weights, up to 64 rows: the weights are read once, straight from their bytes, and multiplied on the warp-level
-// matrix instruction (m16n8k16) with the output's columns as its sixteen rows and eight rows of `a` as its columns.  A 128-row
-// tensor-core tile would be padding, and CUDA cores cannot keep up: at the memory's rate an SM receives 46 weights a clock, which
-// leaves 2.8 lane instructions for each.
-//
-// q - z (element minus zero point) is a whole number of at most 15, exact in fp16 and bf16; products of those with a's elements are exact in fp32,
-// where the instruction adds them.  The scale multiplies the fp32 sum of a group: no weight is ever rounded.  fp32 rows go as three
-// bf16 rows each (24 bits taken apart), whose results are added at the end.
-//
-// A nibble becomes a number by one bit operation and one multiply-add for two of them: (word & 000F000F) ^ 43084308 is the bf16 pair
-// 128 + 8 + q (fp16: 1024 + 8 + q from 64086408), minus 136 + z.  A word holds eight elements of K and the instruction does not mind the order
-// of K, so word t of a 32-element run feeds thread t of a quad twice; a's elements are paired to match ((0,4), (1,5), ...) by
-// byte permutes of one 16-byte read.
-//
-// Work is cut into stages of 128 matrix rows (64 of each matrix for the gated product) by 256 elements of K; every block takes the same
-// number of consecutive stages, whatever tile they belong to, so that all SMs end together (whole tiles over 148 SMs left up to
-// half of them idle).  A tile that several blocks share goes through fp32 sums in scratch: the block whose stages complete it adds them
-// up, in block order, so results do not depend on which one that is.
-// Eight warps take 32 rows each and one half of every stage (with more rows of `a`, 16 and all of it).  One thread feeds a ring of stages by TMA (weights and rows of `a` with
-// 128-byte swizzle, so that both are read from shared memory without bank conflicts; scales and zero points as they lie).
+// Host side of the products with 4-bit weights and few rows (w4_rows.cuh): tensor maps, shares, launch.
 #include <algorithm>
 #include <cstring>
-#include <cuda.h>
-#include <type_traits>
 
-#include "ffn.h"
-#include "ffn_math.cuh"
-#include "ptx_sm100.cuh"
+#include "w4_rows.cuh"
 
 namespace tb200
 {
@@ -33,548 +10,6 @@ namespace ffn
 {
 namespace
 {
-
-constexpr int kRowsWarps   = 8;
-constexpr int kRowsThreads = 32 * (kRowsWarps + 2);    // and the TMA warp, and one that looks at the zero points
-constexpr int kRowsTile    = 128;                      // matrix rows of a block
-constexpr int kRowsStageK  = 256;                      // elements of K in a stage: 128 bytes of weights a row
-constexpr int kRowsWBytes  = kRowsTile * 128;
-constexpr int kRowsMaxStages = 6;
-constexpr int kRowsRedLd   = kRowsTile + 4;            // row pitch of the sums in shared memory: a warp's stores meet 32 banks
-
-struct RowsParams
-{
-    CUtensorMap tmW0, tmW1;    // bytes [W][pitch], box 128 x 128 (gated: 128 x 64 of each)
-    CUtensorMap tmX;           // [rows][C] 16-bit, box 64 x 8 NT
-    CUtensorMap tmS[2], tmZ[2];    // scales and zero points [groups][W], boxes of a tile's columns x the runs of a stage
-    tb200_dtype scale_dt[2];
-    int has_zero[2];
-    int s_off[2], z_off[2];    // of a stage's scales and zero points in the ring
-    int W, C, rows;            // rows of `a`
-    int parts;                 // 16-bit rows that make a row of `a`: 1, or 3 for fp32
-    int group, act;
-    int stages_total;          // stages of a tile
-    int units_total, per_block;    // stages of all tiles, of a block
-    int num_stages, stage_bytes, loaded_bytes;
-    float* partial;                // [blocks][2][8 NT][kRowsTile]: sums of a block's first and last tile
-    int* counts;                   // [tiles]: stages that have arrived; zero between launches
-    int unit;                  // 32-element pieces of a run that shares a group: 1, 2 or 4
-    uint32_t units_group;      // runs of a group
-    void* out;
-    tb200_dtype out_dt;
-    long long wait_limit;
-    int* status;
-};
-
-template <bool BF16>
-__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
-{
-    if (BF16)
-        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-    else
-        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
-__device__ __forceinline__ uint32_t fma2_bf16(uint32_t a, uint32_t b, uint32_t c)
-{
-    uint32_t d;
-    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
-    return d;
-}
-
-__device__ __forceinline__ uint32_t fma2_f16(uint32_t a, uint32_t b, uint32_t c)
-{
-    uint32_t d;
-    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
-    return d;
-}
-
-// (w & m) ^ x in one instruction
-__device__ __forceinline__ uint32_t and_xor(uint32_t w, uint32_t m, uint32_t x)
-{
-    uint32_t d;
-    asm("lop3.b32 %0, %1, %2, %3, 0x6A;" : "=r"(d) : "r"(w), "r"(m), "r"(x));
-    return d;
-}
-
-// Eight elements to four pairs (0,4), (1,5), (2,6), (3,7), minus their zero point; `base` holds -(136 + z) twice (fp16: -(1032 + z)).
-// One multiply-add by 1 takes it off (a bf16 subtraction of pairs is no instruction of its own: ncu counted five in its place).
-// fp16 reads every second pair four bits higher, as 1024 + 16 (8 + q), and scales by 1/16 in the same multiply-add: one shift in place of three.
-template <bool BF16>
-__device__ __forceinline__ void unpack8(uint32_t w, uint32_t base, uint32_t (&p)[4])
-{
-    if (BF16)
-    {
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-            p[i] = fma2_bf16(and_xor(w >> (4 * i), 0x000F000Fu, 0x43084308u), 0x3F803F80u, base);
-    }
-    else
-    {
-        const uint32_t high = fma2_f16(base, 0x3C003C00u, 0x63806380u);    // 960 - (1032 + z) = -(72 + z)
-        const uint32_t v    = w >> 8;
-        p[0]                = fma2_f16(and_xor(w, 0x000F000Fu, 0x64086408u), 0x3C003C00u, base);
-        p[1]                = fma2_f16(and_xor(w, 0x00F000F0u, 0x64806480u), 0x2C002C00u, high);
-        p[2]                = fma2_f16(and_xor(v, 0x000F000Fu, 0x64086408u), 0x3C003C00u, base);
-        p[3]                = fma2_f16(and_xor(v, 0x00F000F0u, 0x64806480u), 0x2C002C00u, high);
-    }
-}
-
-__device__ __forceinline__ uint4 lds128(uint32_t addr)
-{
-    uint4 v;
-    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
-    return v;
-}
-
-__device__ __forceinline__ uint32_t lds32(uint32_t addr)
-{
-    uint32_t v;
-    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(addr));
-    return v;
-}
-
-// What a warp needs to know of its matrix: where a run's scales and zero points are, for its rows
-struct RowsRun
-{
-    uint32_t scale, zero;    // shared addresses of the first run's, at the lane's first row
-    int scale_step, zero_step;    // bytes from one run to the next
-    tb200_dtype dt;
-    bool has_zero;
-};
-
-// Scales of rows +0, +8, +16, +24, and minus their zero point: -(136 + z) twice as bf16 (steps of 1 from 128 on), -(1032 + z) as fp16 (steps
-// of 1 from 1024 on).  A zero point that is none of -8 .. 7 is reported by the warp that looks for it; the product is then not one.
-template <bool BF16, int MT>
-__device__ __forceinline__ void run_scales(const RowsRun& r, int i, float (&scale)[2 * MT], uint32_t (&base)[2 * MT])
-{
-    const uint32_t at = r.scale + (uint32_t)(i * r.scale_step);
-    if (r.dt == TB200_FP32)
-    {
-#pragma unroll
-        for (int q = 0; q < 2 * MT; q++)
-            scale[q] = __uint_as_float(lds32(at + (uint32_t)(q * 32)));
-    }
-    else
-    {
-#pragma unroll
-        for (int q = 0; q < 2 * MT; q++)
-        {
-            uint16_t h;
-            asm volatile("ld.shared.b16 %0, [%1];" : "=h"(h) : "r"(at + (uint32_t)(q * 16)));
-            scale[q] = r.dt == TB200_BF16 ? __uint_as_float((uint32_t)h << 16) : __half2float(__ushort_as_half(h));
-        }
-    }
-#pragma unroll
-    for (int q = 0; q < 2 * MT; q++)
-    {
-        int z = 0;
-        if (r.has_zero)
-            asm volatile("ld.shared.s8 %0, [%1];" : "=r"(z) : "r"(r.zero + (uint32_t)(i * r.zero_step + q * 8)));
-        base[q] = (BF16 ? 0xC308C308u : 0xE408E408u) + (uint32_t)z * 0x10001u;
-    }
-}
-
-// One warp's part of a stage: eight 32-element pieces of 16 matrix rows, or four of 32 (MT 1 or 2 sixteens), against all rows of `a`; runs of
-// UNIT pieces share a group.  `runs`: the row of scales that each run takes, four bits each.
-template <bool BF16, int NT, int MT, int UNIT>
-__device__ __forceinline__ void stage_part(float (&total)[MT][NT][4], uint32_t sW, uint32_t sX, const uint32_t (&offW)[8 / MT],
-                                           const uint32_t (&offX)[2], const RowsRun& run, uint32_t runs)
-{
-#pragma unroll
-    for (int r = 0; r < 8 / MT / UNIT; r++)
-    {
-        float scale[2 * MT];
-        uint32_t base[2 * MT];
-        run_scales<BF16, MT>(run, (int)(runs >> (4 * r) & 15), scale, base);
-        float accum[MT][NT][4];
-#pragma unroll
-        for (int m = 0; m < MT; m++)
-#pragma unroll
-            for (int j = 0; j < NT; j++)
-                accum[m][j][0] = accum[m][j][1] = accum[m][j][2] = accum[m][j][3] = 0.f;
-#pragma unroll
-        for (int c = r * UNIT; c < (r + 1) * UNIT; c++)
-        {
-            uint32_t w[2 * MT][4];
-#pragma unroll
-            for (int q = 0; q < 2 * MT; q++)
-                unpack8<BF16>(lds32(sW + offW[c] + (uint32_t)(q * 1024)), base[q], w[q]);
-#pragma unroll
-            for (int j = 0; j < NT; j++)
-            {
-                const uint4 x     = lds128(sX + offX[c & 1] + (uint32_t)((c >> 1) * 8 * NT * 128 + j * 1024));
-                const uint32_t x0 = __byte_perm(x.x, x.z, 0x5410), x1 = __byte_perm(x.x, x.z, 0x7632), x2 = __byte_perm(x.y, x.w, 0x5410),
-                               x3 = __byte_perm(x.y, x.w, 0x7632);
-#pragma unroll
-                for (int m = 0; m < MT; m++)
-                {
-                    mma<BF16>(accum[m][j], w[2 * m][0], w[2 * m + 1][0], w[2 * m][1], w[2 * m + 1][1], x0, x1);
-                    mma<BF16>(accum[m][j], w[2 * m][2], w[2 * m + 1][2], w[2 * m][3], w[2 * m + 1][3], x2, x3);
-                }
-            }
-        }
-        // the run's sum under its scale
-#pragma unroll
-        for (int m = 0; m < MT; m++)
-#pragma unroll
-            for (int j = 0; j < NT; j++)
-            {
-                total[m][j][0] = fmaf(scale[2 * m], accum[m][j][0], total[m][j][0]);
-                total[m][j][1] = fmaf(scale[2 * m], accum[m][j][1], total[m][j][1]);
-                total[m][j][2] = fmaf(scale[2 * m + 1], accum[m][j][2], total[m][j][2]);
-                total[m][j][3] = fmaf(scale[2 * m + 1], accum[m][j][3], total[m][j][3]);
-            }
-    }
-}
-
-// Rows of the matrix that a warp takes, in sixteens, and blocks to an SM.  Few rows of `a`: 32 matrix rows share every read and permutation of a's
-// elements.  More: sixteen, whose sums leave registers for two blocks, and the matrix instructions take as long as the rest.
-constexpr int rows_mt(int nt)
-{
-    return nt <= 2 ? 2 : 1;
-}
-constexpr int rows_blocks_sm(int nt)
-{
-    return nt <= 4 ? 2 : 1;
-}
-
-template <bool BF16, int NT, int MATS>
-__global__ void __launch_bounds__(kRowsThreads, rows_blocks_sm(NT)) w4_rows_kernel(const __grid_constant__ RowsParams p)
-{
-    extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t bar_full[kRowsMaxStages];
-    __shared__ __align__(8) uint64_t bar_empty[kRowsMaxStages];
-    __shared__ int completes[2];
-
-    constexpr int kPer       = kRowsTile / MATS;    // columns of the output
-    constexpr int MT         = rows_mt(NT);
-    const int tid            = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const uint32_t smem_base = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
-    uint8_t* const ring      = smem_raw + (smem_base - ptx::smem_u32(smem_raw));
-    float* const red         = reinterpret_cast<float*>(ring + p.num_stages * p.stage_bytes);    // sums of a tile
-    const int S = p.stages_total, begin = (int)blockIdx.x * p.per_block, end = min(p.units_total, begin + p.per_block);
-
-    if (tid == 0)
-    {
-        for (int s = 0; s < p.num_stages; s++)
-        {
-            ptx::mbar_init(ptx::smem_u32(&bar_full[s]), 1);
-            ptx::mbar_init(ptx::smem_u32(&bar_empty[s]), kRowsWarps + 1);
-        }
-        ptx::fence_barrier_init();
-        ptx::prefetch_tmap(&p.tmW0);
-        ptx::prefetch_tmap(&p.tmX);
-        if (MATS == 2)
-            ptx::prefetch_tmap(&p.tmW1);
-        ptx::dep_launch_trigger();
-        // the ring's first weights on their way to L2, where a write by the kernel before would still find them
-        for (int u = begin, i = 0; u < end && i < p.num_stages; u++, i++)
-        {
-            ptx::prefetch_2d(&p.tmW0, u % S * 128, u / S * kPer);
-            if (MATS == 2)
-                ptx::prefetch_2d(&p.tmW1, u % S * 128, u / S * kPer);
-        }
-    }
-    __syncthreads();
-    // everything a kernel before this one may have written is read behind this wait
-    ptx::dep_launch_wait();
-
-    const int units = p.unit == 4 ? 2 : p.unit == 2 ? 4 : 8;    // runs of a stage
-    const int tile0 = begin / S, stage0 = begin - tile0 * S;
-
-    if (warp == kRowsWarps)
-    {
-        if (lane == 0)
-        {
-            bool ok = true;
-            int i = 0, s = 0, tile = tile0, k = stage0;
-            uint32_t phase = 0;
-            for (; i < end - begin; i++)
-            {
-                if (!ptx::mbar_wait_bounded(ptx::smem_u32(&bar_empty[s]), phase ^ 1u, p.wait_limit))
-                {
-                    ok = false;
-                    break;
-                }
-                const uint32_t full = ptx::smem_u32(&bar_full[s]);
-                const uint32_t sW   = smem_base + (uint32_t)(s * p.stage_bytes), sX = sW + kRowsWBytes;
-                ptx::mbar_arrive_expect_tx(full, (uint32_t)p.loaded_bytes);
-                ptx::tma_load_2d(sW, &p.tmW0, full, k * 128, tile * kPer);
-                if (MATS == 2)
-                    ptx::tma_load_2d(sW + kPer * 128, &p.tmW1, full, k * 128, tile * kPer);
-#pragma unroll
-                for (int j = 0; j < 4; j++)
-                    ptx::tma_load_2d(sX + (uint32_t)(j * 8 * NT * 128), &p.tmX, full, k * kRowsStageK + j * 64, 0);
-                const int group = (int)((uint32_t)(k * units) / p.units_group);    // of the stage's first run
-#pragma unroll
-                for (int m = 0; m < MATS; m++)
-                {
-                    ptx::tma_load_2d(sW + (uint32_t)p.s_off[m], &p.tmS[m], full, tile * kPer, group);
-                    if (p.has_zero[m])
-                        ptx::tma_load_2d(sW + (uint32_t)p.z_off[m], &p.tmZ[m], full, tile * kPer, group);
-                }
-                if (++k == S)
-                {
-                    k = 0;
-                    tile++;
-                }
-                if (++s == p.num_stages)
-                {
-                    s = 0;
-                    phase ^= 1u;
-                }
-            }
-            if (!ok)
-            {
-                atomicOr(p.status, TB200_DEV_TIMEOUT);
-                // copies in flight land before the block leaves
-                for (int j = max(0, i - p.num_stages); j < i; j++)
-                    ptx::mbar_wait_bounded(ptx::smem_u32(&bar_full[j % p.num_stages]), (uint32_t)(j / p.num_stages) & 1u, p.wait_limit);
-            }
-        }
-    }
-    else if (warp > kRowsWarps)
-    {
-        // REQUIRE: zero points are 4-bit numbers, -8 .. 7 (what lies outside the matrix reads as 0)
-        bool ok = true;
-        uint32_t bad = 0, phase = 0;
-        for (int u = begin, s = 0; u < end && ok; u++)
-        {
-            ok = ptx::mbar_wait_bounded(ptx::smem_u32(&bar_full[s]), phase, p.wait_limit);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok)
-                break;
-#pragma unroll
-            for (int m = 0; m < MATS; m++)
-                for (int e = lane; p.has_zero[m] && e < units * kPer / 4; e += 32)
-                {
-                    const uint32_t z = lds32(smem_base + (uint32_t)(s * p.stage_bytes + p.z_off[m] + 4 * e));
-                    bad |= __vcmpgts4(z, 0x07070707u) | __vcmplts4(z, 0xF8F8F8F8u);
-                }
-            __syncwarp();
-            if (lane == 0)
-                ptx::mbar_arrive(ptx::smem_u32(&bar_empty[s]));
-            if (++s == p.num_stages)
-            {
-                s = 0;
-                phase ^= 1u;
-            }
-        }
-        if (!ok && lane == 0)
-            atomicOr(p.status, TB200_DEV_TIMEOUT);
-        if (bad)
-            atomicOr(p.status, TB200_DEV_UNPREDICTABLE);
-    }
-    else
-    {
-        const int g = lane >> 2, t = lane & 3;
-        const int group = MT == 2 ? warp & 3 : warp;    // of 16 MT matrix rows
-        const int half  = MT == 2 ? warp >> 2 : 0;      // of a stage: 32-element pieces 4 half .. 4 half + 3, or all eight
-        const int wrow  = group * 16 * MT + g;          // and wrow + 8 (+ 16, + 24)
-        // column n of the instruction is row perm(n) of the tile of eight: neighbouring lanes' reads then meet different banks
-        const int xr = (g >> 1) + (g & 1) * 4;
-        uint32_t offW[8 / MT], offX[2];
-#pragma unroll
-        for (int c = 0; c < 8 / MT; c++)
-            offW[c] = (uint32_t)(wrow * 128 + t * 4) + (uint32_t)((((half * 4 + c) ^ g) & 7) << 4);
-#pragma unroll
-        for (int c = 0; c < 2; c++)
-            offX[c] = (uint32_t)(half * 2 * 8 * NT * 128 + xr * 128) + (uint32_t)(((c * 4 + t) ^ xr) << 4);
-        const int values = p.rows * p.parts * kRowsTile, items = p.rows * kPer;
-        // results of a tile whose sums are in `red`
-        auto results = [&](int col0) {
-            for (int e = tid; e < items; e += 32 * kRowsWarps)
-            {
-                const int r = e / kPer, c = e % kPer;
-                if (col0 + c >= p.W)
-                    continue;
-                float v[MATS];
-#pragma unroll
-                for (int m = 0; m < MATS; m++)
-                {
-                    v[m] = 0.f;
-                    for (int part = p.parts - 1; part >= 0; part--)    // the smallest first
-                        v[m] += red[(r * p.parts + part) * kRowsRedLd + m * kPer + c];
-                }
-                store_fp(p.out, (int64_t)r * p.W + col0 + c, p.out_dt, MATS == 2 ? act_value(p.act, v[0]) * v[MATS - 1] : v[0]);
-            }
-        };
-        constexpr int kSlot = 8 * NT * kRowsTile;
-        bool ok = true;
-        int s = 0, tile = tile0, k = stage0;
-        uint32_t phase = 0;
-        const int mat = MATS == 2 ? wrow / kPer : 0, mrow = wrow - mat * kPer;    // row of its matrix in the tile
-        RowsRun run;
-        run.dt         = p.scale_dt[mat];
-        run.has_zero   = p.has_zero[mat] != 0;
-        run.scale_step = kPer * (run.dt == TB200_FP32 ? 4 : 2);
-        run.zero_step  = kPer;
-        const uint32_t s_off = (uint32_t)(p.s_off[mat] + mrow * (run.dt == TB200_FP32 ? 4 : 2)), z_off = (uint32_t)(p.z_off[mat] + mrow);
-        const uint32_t full0 = ptx::smem_u32(&bar_full[0]), empty0 = ptx::smem_u32(&bar_empty[0]);
-        for (int u = begin; u < end;)
-        {
-            const int n = min(end - u, S - k);    // stages of this tile
-            float total[MT][NT][4];
-#pragma unroll
-            for (int m = 0; m < MT; m++)
-#pragma unroll
-                for (int j = 0; j < NT; j++)
-                    total[m][j][0] = total[m][j][1] = total[m][j][2] = total[m][j][3] = 0.f;
-            auto stages = [&](auto pieces) {
-                constexpr int UNIT = decltype(pieces)::value, kRuns = 8 / UNIT;
-                // rows of scales that this part's runs take: one each, or fewer where a group holds several runs
-                const uint32_t own = half ? 0x76543210u >> (2 * kRuns) : 0x76543210u;
-                for (int i = 0; i < n; i++)
-                {
-                    ok = __all_sync(0xffffffffu, ptx::mbar_wait_bounded(full0 + 8 * s, phase, p.wait_limit));
-                    if (!ok)
-                        break;
-                    const uint32_t sW = smem_base + (uint32_t)(s * p.stage_bytes);
-                    run.scale         = sW + s_off;
-                    run.zero          = sW + z_off;
-                    uint32_t runs     = own;
-                    if (p.units_group > 1)
-                    {
-                        const uint32_t u0 = (uint32_t)((k + i) * kRuns), g0 = u0 / p.units_group;
-                        runs              = 0;
-#pragma unroll
-                        for (int r = 0; r < kRuns / MT; r++)
-                            runs |= ((u0 + (own >> (4 * r) & 15)) / p.units_group - g0) << (4 * r);
-                    }
-                    stage_part<BF16, NT, MT, UNIT>(total, sW, sW + kRowsWBytes, offW, offX, run, runs);
-                    __syncwarp();
-                    if (lane == 0)
-                        ptx::mbar_arrive(empty0 + 8 * s);
-                    if (++s == p.num_stages)
-                    {
-                        s = 0;
-                        phase ^= 1u;
-                    }
-                }
-            };
-            if (ok)
-            {
-                if (p.unit == 4)
-                    stages(std::integral_constant<int, 4>());
-                else if (p.unit == 2)
-                    stages(std::integral_constant<int, 2>());
-                else
-                    stages(std::integral_constant<int, 1>());
-            }
-            // the eight warps go on together; after a wait that gave up they only count their stages, so that the counts end at zero
-            ok = ptx::named_barrier_and(1, 32 * kRowsWarps, ok);
-            const int col0 = tile * kPer;
-            if (ok)
-            {
-                // the first half's sums, then the second's on top
-#pragma unroll
-                for (int pass = 0; pass < MT; pass++)
-                {
-                    if (half == pass)
-                    {
-#pragma unroll
-                        for (int m = 0; m < MT; m++)
-#pragma unroll
-                            for (int j = 0; j < NT; j++)
-#pragma unroll
-                                for (int e = 0; e < 4; e++)
-                                {
-                                    // instruction columns 2t and 2t + 1 are rows t and t + 4 of the tile of eight
-                                    float* const at = red + (j * 8 + t + (e & 1) * 4) * kRowsRedLd + wrow + m * 16 + (e >> 1) * 8;
-                                    *at             = pass ? *at + total[m][j][e] : total[m][j][e];
-                                }
-                    }
-                    ptx::named_barrier_and(1, 32 * kRowsWarps, true);
-                }
-            }
-            if (n == S)
-            {
-                if (ok)
-                    results(col0);
-            }
-            else if (ok)
-            {
-                float4* const mine = reinterpret_cast<float4*>(p.partial + ((int64_t)blockIdx.x * 2 + (u == begin ? 0 : 1)) * kSlot);
-                for (int e = tid; e < values / 4; e += 32 * kRowsWarps)
-                    __stcg(mine + e, *reinterpret_cast<const float4*>(red + e / (kRowsTile / 4) * kRowsRedLd + e % (kRowsTile / 4) * 4));
-            }
-            ptx::named_barrier_and(1, 32 * kRowsWarps, true);    // `red` is free again
-            u += n;
-            k = 0;
-            tile++;
-        }
-        // tiles shared with other blocks, at most the first and the last: whoever brings the last stages adds the sums up, in block order
-        const int n_first = min(end - begin, S - stage0), tile_last = (end - 1) / S, n_last = end - tile_last * S;
-        const bool share_first = n_first < S, share_last = tile_last > tile0 && n_last < S;
-        if (tid == 0)
-        {
-            __threadfence();    // the block's sums, which the barrier above has put before this
-            const int first = share_first ? atomicAdd(p.counts + tile0, n_first) : 0, last = share_last ? atomicAdd(p.counts + tile_last, n_last) : 0;
-            completes[0]    = share_first && first + n_first == S;
-            completes[1]    = share_last && last + n_last == S;
-            if (completes[0])
-                p.counts[tile0] = 0;    // for the next launch
-            if (completes[1])
-                p.counts[tile_last] = 0;
-            __threadfence();
-        }
-        ptx::named_barrier_and(1, 32 * kRowsWarps, true);
-#pragma unroll
-        for (int which = 0; which < 2; which++)
-        {
-            if (!completes[which] || !ok)
-                continue;
-            const int shared = which ? tile_last : tile0;
-            const int lo = shared * S / p.per_block, hi = (shared * S + S - 1) / p.per_block;
-            // the tile is the first of every block but maybe `lo`, which may have come from the one before
-            const int slot_lo = lo * p.per_block >= shared * S ? 0 : 1;
-            const float4* const first = reinterpret_cast<const float4*>(p.partial + ((int64_t)lo * 2 + slot_lo) * kSlot);
-            constexpr int kAtOnce = 4;    // loads of a thread on their way together
-            for (int e0 = tid; e0 < values / 4; e0 += 32 * kRowsWarps * kAtOnce)
-            {
-                float4 v[kAtOnce];
-#pragma unroll
-                for (int e = 0; e < kAtOnce; e++)
-                {
-                    const int at = e0 + e * 32 * kRowsWarps;
-                    v[e]         = at < values / 4 ? __ldcg(first + at) : make_float4(0.f, 0.f, 0.f, 0.f);
-                }
-#pragma unroll 4
-                for (int block = lo + 1; block <= hi; block++)
-                {
-                    const float4* const next = reinterpret_cast<const float4*>(p.partial + (int64_t)block * 2 * kSlot);
-#pragma unroll
-                    for (int e = 0; e < kAtOnce; e++)
-                    {
-                        const int at   = e0 + e * 32 * kRowsWarps;
-                        const float4 x = at < values / 4 ? __ldcg(next + at) : make_float4(0.f, 0.f, 0.f, 0.f);
-                        v[e].x += x.x;
-                        v[e].y += x.y;
-                        v[e].z += x.z;
-                        v[e].w += x.w;
-                    }
-                }
-#pragma unroll
-                for (int e = 0; e < kAtOnce; e++)
-                {
-                    const int at = e0 + e * 32 * kRowsWarps;
-                    if (at < values / 4)
-                        *reinterpret_cast<float4*>(red + at / (kRowsTile / 4) * kRowsRedLd + at % (kRowsTile / 4) * 4) = v[e];
-                }
-            }
-            ptx::named_barrier_and(1, 32 * kRowsWarps, true);
-            results(shared * kPer);
-            ptx::named_barrier_and(1, 32 * kRowsWarps, true);
-        }
-        if (!ok && lane == 0)
-            atomicOr(p.status, TB200_DEV_TIMEOUT);
-    }
-}
 
 typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                                 const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -614,20 +49,11 @@ tb200_status encode_plain(tb200_ctx* ctx, CUtensorMap* m, size_t es, const void*
     return TB200_OK;
 }
 
-typedef void (*RowsKern)(const RowsParams);
-
-template <bool BF16, int MATS>
-RowsKern pick(int nt)
+// elements, up to whole sixteens of bytes
+int64_t round_up16(int64_t n, size_t es)
 {
-    switch (nt)
-    {
-        case 1: return w4_rows_kernel<BF16, 1, MATS>;
-        case 2: return w4_rows_kernel<BF16, 2, MATS>;
-        case 3: return w4_rows_kernel<BF16, 3, MATS>;
-        case 4: return w4_rows_kernel<BF16, 4, MATS>;
-        case 6: return w4_rows_kernel<BF16, 6, MATS>;
-        default: return w4_rows_kernel<BF16, 8, MATS>;
-    }
+    const int64_t per = 16 / (int64_t)es;
+    return (n + per - 1) / per * per;
 }
 
 int tiles_of_eight(int64_t xrows)
@@ -685,24 +111,31 @@ tb200_status w4_rows_launch(tb200_ctx* ctx, const W4Problem& q, const void* x, i
     p.units_group = q.group >= q.C ? 0x7fffffffu : (uint32_t)(q.group / (32 * p.unit));
     const int units      = 8 / p.unit;
     const int64_t groups = ((int64_t)q.C + q.group - 1) / q.group;
-    size_t stage         = kRowsWBytes + (size_t)nt * 8 * 512;
+    size_t stage         = kRowsWBytes + (size_t)nt * 8 * 512, loaded = stage;    // its place in the ring, what is copied there
     for (int m = 0; m < q.mats; m++)
     {
         const size_t es = dtype_size(q.w[m].scale_dt);
         p.scale_dt[m]   = q.w[m].scale_dt;
         p.has_zero[m]   = q.w[m].zero ? 1 : 0;
-        st = encode_plain(ctx, &p.tmS[m], es, q.w[m].scale, q.W, groups, q.w[m].scale_pitch, (uint32_t)kPer, (uint32_t)units);
+        auto operand = [&](CUtensorMap* map, size_t size, const void* data, int* off, int* step, int* flat) {
+            const bool whole = (size_t)q.W * size % 16 == 0;
+            *flat            = whole ? 0 : (int)(16 / size);
+            *off             = (int)stage;
+            // (a box of its own starts at a multiple of 128 bytes)
+            *step = whole ? (int)(kPer * size) : (int)((kPer * size + 16 + 127) / 128 * 128);
+            stage += (size_t)units * *step;
+            loaded += (size_t)units * (kPer * size + (whole ? 0 : 16));
+            return whole ? encode_plain(ctx, map, size, data, q.W, groups, q.W, (uint32_t)kPer, (uint32_t)units)
+                         : encode_plain(ctx, map, size, data, groups * q.W, 1, round_up16(groups * q.W, size), (uint32_t)(kPer + 16 / size), 1);
+        };
+        st = operand(&p.tmS[m], es, q.w[m].scale, &p.s_off[m], &p.s_step[m], &p.s_flat[m]);
         if (st == TB200_OK && q.w[m].zero)
-            st = encode_plain(ctx, &p.tmZ[m], 1, q.w[m].zero, q.W, groups, q.w[m].zero_pitch, (uint32_t)kPer, (uint32_t)units);
+            st = operand(&p.tmZ[m], 1, q.w[m].zero, &p.z_off[m], &p.z_step[m], &p.z_flat[m]);
         if (st != TB200_OK)
             return st;
-        p.s_off[m] = (int)stage;
-        stage += (size_t)units * kPer * es;
-        p.z_off[m] = (int)stage;
-        stage += q.w[m].zero ? (size_t)units * kPer : 0;
+        p.z_words[m] = (kPer + (p.z_flat[m] ? 16 : 0)) / 4;
     }
-    const size_t loaded = stage;
-    stage               = (stage + 1023) & ~(size_t)1023;
+    stage = (stage + 1023) & ~(size_t)1023;
     p.W = q.W; p.C = q.C; p.rows = (int)q.M; p.parts = parts;
     p.group = q.group; p.act = q.act; p.out = q.out; p.out_dt = q.out_dt;
     p.wait_limit   = ctx->wait_limit_cycles;
@@ -720,9 +153,10 @@ tb200_status w4_rows_launch(tb200_ctx* ctx, const W4Problem& q, const void* x, i
     const size_t room  = (rows_blocks_sm(nt) == 2 ? 113 : 226) * 1024 - (red + 2048);
     p.num_stages       = std::max(2, std::min(kRowsMaxStages, (int)(room / stage)));
     const size_t smem  = p.num_stages * stage + red + 1024;
-    const RowsKern kern = q.mats == 2 ? (bf16 ? pick<true, 2>(nt) : pick<false, 2>(nt)) : (bf16 ? pick<true, 1>(nt) : pick<false, 1>(nt));
+    const bool flat     = p.s_flat[0] || p.z_flat[0] || p.s_flat[1] || p.z_flat[1];
+    const RowsKern kern = bf16 ? w4_rows_kernel_bf16(nt, q.mats, flat) : w4_rows_kernel_f16(nt, q.mats, flat);
     const int size_id   = nt <= 4 ? nt - 1 : nt / 2 + 1;
-    st = raise_smem_limit(ctx, 136 + size_id * 4 + (bf16 ? 2 : 0) + q.mats - 1, reinterpret_cast<const void*>(kern), (int)smem);
+    st = raise_smem_limit(ctx, 192 + size_id * 8 + (flat ? 4 : 0) + (bf16 ? 2 : 0) + q.mats - 1, reinterpret_cast<const void*>(kern), (int)smem);
     if (st != TB200_OK)
         return st;
     cudaLaunchConfig_t cfg = {};
