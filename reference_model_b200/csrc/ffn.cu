@@ -119,7 +119,7 @@ tb200_status gated_pair(tb200_ctx* ctx, const GatedProblem& q)
         k.out_dt[0] = k.out_dt[1] = q.out_dt;
         k.ld        = q.W;
         k.name      = "gated_pair_f16";
-        TB200_TRY(q.H <= kFewRows ? gated_rows_launch(ctx, k) : pair_launch(ctx, k));
+        TB200_TRY(q.H <= kFewRows && q.NB <= 65535 ? gated_rows_launch(ctx, k) : pair_launch(ctx, k));
     }
     return TB200_OK;
 }

@@ -39,7 +39,9 @@ struct Shape
     static constexpr int kRows = 128 * kCtas, kCols = PAIR ? 256 : 128;    // of a tile
     static constexpr int kSub  = PAIR ? 2 : 1;                             // chunks per stage
     static constexpr int kStage = 2 * kSub * kChunk;                       // each CTA holds 128 rows of A and 128 columns of B
-    static constexpr int kSmem  = kStages * kStage + 1024;
+    // (with the static part all of an SM's: a CTA that waits for tensor memory never shares an SM with another kernel's that holds some)
+    static constexpr int kSmem  = 208 * 1024;
+    static_assert(kStages * kStage + 1024 <= kSmem, "the ring fits");
     static constexpr int kTmemCols = 2 * kCols;
     static constexpr int kRedLd    = kCols + 4;    // row pitch of a tile's sums in shared memory: a warp's stores meet every bank
 };
@@ -502,10 +504,13 @@ __global__ void __launch_bounds__(kThreads, 1) ffn_pair_kernel(const __grid_cons
             if (!ok)
             {
                 atomicOr(p.status, TB200_DEV_TIMEOUT);
-                // the pair's copies in flight land before either CTA leaves (all of them report to the first CTA)
+                // the pair's copies in flight land before either CTA leaves (all of them report to the first CTA, which may have given up on a
+                // stage that the second has asked for)
                 if (rank == 0)
                     for (int64_t i = max((int64_t)0, issued - kStages); i < issued; i++)
-                        ptx::mbar_wait_bounded(ptx::smem_u32(&bar_full[i % kStages]), (uint32_t)(i / kStages) & 1u, p.wait_limit);
+                        ptx::mbar_wait_bounded(ptx::smem_u32(&bar_full[i % kStages]), (uint32_t)(i / kStages) & 1u, ptx::kDrainCycles);
+                if (PAIR)
+                    ptx::settle();
             }
         }
     }
@@ -589,7 +594,7 @@ __global__ void __launch_bounds__(kThreads, 1) ffn_pair_kernel(const __grid_cons
                     ptx::mma_commit_pair(ptx::smem_u32(&bar_drain), 1);
                 else
                     ptx::mma_commit(ptx::smem_u32(&bar_drain));
-                ptx::mbar_wait_bounded(ptx::smem_u32(&bar_drain), 0, p.wait_limit);
+                ptx::mbar_wait_bounded(ptx::smem_u32(&bar_drain), 0, ptx::kDrainCycles);
             }
         }
     }

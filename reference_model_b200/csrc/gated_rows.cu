@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(kFewThreads) gated_rows_kernel(const __grid_co
                 atomicOr(p.status, TB200_DEV_TIMEOUT);
                 // copies in flight land before the block leaves
                 for (int j = max(0, i - p.num_stages); j < i; j++)
-                    ptx::mbar_wait_bounded(ptx::smem_u32(&bar_full[j % p.num_stages]), (uint32_t)(j / p.num_stages) & 1u, p.wait_limit);
+                    ptx::mbar_wait_bounded(ptx::smem_u32(&bar_full[j % p.num_stages]), (uint32_t)(j / p.num_stages) & 1u, ptx::kDrainCycles);
             }
         }
     }

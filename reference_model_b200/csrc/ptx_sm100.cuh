@@ -79,6 +79,18 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint32_t bar, uint32_t parity,
     return true;
 }
 
+// What a role waits for after it has given up: copies and MMAs that are on their way land within microseconds, whatever the limit above is.
+constexpr long long kDrainCycles = 1 << 22;
+
+// ... and where their arrival cannot be seen (the other CTA's barrier): time in which they land
+__device__ __forceinline__ void settle()
+{
+    const long long t0 = clock64();
+    while (clock64() - t0 < (1 << 17))
+    {
+    }
+}
+
 // ---------------------------------------------------------------- programmatic dependent launch
 // A kernel launched with the programmatic-serialization attribute may start while its predecessor in the stream is
 // still running.  dep_launch_trigger: this grid lets its successor be scheduled (once every CTA of the grid has said so

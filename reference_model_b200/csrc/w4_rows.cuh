@@ -356,7 +356,7 @@ __global__ void __launch_bounds__(kRowsThreads, rows_blocks_sm(NT)) w4_rows_kern
                 atomicOr(p.status, TB200_DEV_TIMEOUT);
                 // copies in flight land before the block leaves
                 for (int j = max(0, i - p.num_stages); j < i; j++)
-                    ptx::mbar_wait_bounded(ptx::smem_u32(&bar_full[j % p.num_stages]), (uint32_t)(j / p.num_stages) & 1u, p.wait_limit);
+                    ptx::mbar_wait_bounded(ptx::smem_u32(&bar_full[j % p.num_stages]), (uint32_t)(j / p.num_stages) & 1u, ptx::kDrainCycles);
             }
         }
     }

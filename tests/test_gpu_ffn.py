@@ -569,3 +569,208 @@ def test_repeated_calls_give_the_same_bits(ctx):
         got = [get(t) for t in grads]
         first = first or got
         assert all(torch.equal(x, y) for x, y in zip(first, got))
+
+
+# ------------------------------------------------------------------------------------------------ forms, limits, neighbours
+def whole(seed, dtype, lo, hi, *shape):
+    """Small whole numbers: every product and sum is exact, whatever the order."""
+    return torch.randint(lo, hi, shape, generator=torch.Generator().manual_seed(seed)).to(TT[dtype])
+
+
+def forms(ctx):
+    """(name, kernel, call, outputs, exact results) of calls that reach every kernel and shape of it, with exact results."""
+    made = []
+
+    def gated(name, kernel, n, nb, h, c, w):
+        a, bg, bu = whole(1, "bf16", -1, 2, n, h, c), whole(2, "bf16", -1, 2, nb, c, w), whole(3, "bf16", -1, 2, nb, c, w)
+        out = blank(ctx, "fp32", (n, h, w))
+        ts = [put(ctx, t) for t in (a, bg, bu)]
+        a, bg, bu = a.double(), bg.double(), bu.double()
+        made.append((name, kernel, lambda: ctx.matmul_gated(ts[0], ts[1], ts[2], out, "RELU"), [out], [(a @ bg).clamp(min=0) * (a @ bu)]))
+
+    def four(name, kernel, h, c, w, gated_too):
+        a = whole(4, "fp16", -1, 2, 1, h, c)
+        r = np.random.default_rng(5)
+        data = [r.integers(0, 256, size=(w, (c + 31) // 32 * 16)).astype(np.uint8) for _ in range(2)]
+        ops, dense = [], []
+        for d in data:
+            q = np.stack([d & 15, d >> 4], axis=2).reshape(w, -1)[:, :c].astype(np.float64).T
+            q[q > 7] -= 16
+            dense.append(torch.from_numpy(q))
+            ops.append(tb.W4(ctx.from_numpy(d), put(ctx, torch.ones((-(-c // 64), w), dtype=torch.float16)), None, 64))
+        ta, out = put(ctx, a), blank(ctx, "fp32", (1, h, w))
+        a = a.double()
+        if gated_too:
+            made.append((name, kernel, lambda: ctx.matmul_gated_w4(ta, ops[0], ops[1], out, "RELU"), [out],
+                         [(a @ dense[0]).clamp(min=0) * (a @ dense[1])]))
+        else:
+            made.append((name, kernel, lambda: ctx.matmul_w4(ta, ops[0], out), [out], [a @ dense[0]]))
+
+    def backward(name, kernel, n, nb, h, c, w):
+        # one column of `a` apart, dG and dU are whole numbers below 256: exact in bf16
+        a, bg, bu = whole(6, "bf16", 0, 2, n, h, c), whole(7, "bf16", -1, 2, nb, c, w), whole(8, "bf16", -1, 2, nb, c, w)
+        a[:, :, 8:] = 0
+        d = whole(9, "bf16", -1, 2, n, h, w)
+        ts = [put(ctx, t) for t in (a, bg, bu, d)]
+        grads = [blank(ctx, "fp32", tuple(t.shape)) for t in (a, bg, bu)]
+        a, bg, bu, d = a.double(), bg.double(), bu.double(), d.double()
+        G, U = a @ bg, a @ bu
+        dG, dU = d * U * (G > 0), d * G.clamp(min=0)
+        wg, wu = (a.transpose(1, 2) @ x for x in (dG, dU))
+        if nb == 1:
+            wg, wu = wg.sum(0, keepdim=True), wu.sum(0, keepdim=True)
+        made.append((name, kernel, lambda: ctx.matmul_gated_backward(*ts, *grads, activation="RELU"), grads,
+                     [dG @ bg.transpose(1, 2) + dU @ bu.transpose(1, 2), wg, wu]))
+
+    gated("few rows, K over clusters", "gated_rows_f16", 1, 1, 3, 4000, 200)
+    gated("few rows, many columns", "gated_rows_f16", 2, 2, 40, 264, 12000)
+    gated("pairs", "gated_pair_f16", 1, 1, 1500, 520, 2000)
+    gated("single, K over clusters", "gated_pair_f16", 1, 1, 100, 4000, 72)
+    gated("single", "gated_pair_f16", 3, 3, 150, 100, 300)
+    four("few rows", "matmul_w4_rows", 1, 9000, 700, False)
+    four("few rows, gated", "gated_w4_rows", 20, 3000, 333, True)
+    four("48 rows", "matmul_w4_rows", 45, 5000, 129, False)
+    four("many rows", "matmul_w4_pair", 200, 1000, 300, False)
+    four("many rows, gated", "gated_w4_pair", 90, 2000, 200, True)
+    backward("small", "gated_backward_pair_f16", 2, 2, 130, 72, 200)
+    backward("long K", "gated_backward_pair_f16", 1, 1, 2600, 64, 40)
+    backward("large", "gated_backward_pair_f16", 1, 1, 700, 2100, 1290)
+    return made
+
+
+FORMS = ["few rows, K over clusters", "few rows, many columns", "pairs", "single, K over clusters", "single", "few rows", "few rows, gated", "48 rows",
+         "many rows", "many rows, gated", "small", "long K", "large"]
+
+
+@pytest.fixture(scope="module")
+def all_forms(ctx):
+    return {f[0]: f for f in forms(ctx)}
+
+
+@pytest.mark.parametrize("name", FORMS)
+def test_every_form_is_exact_and_recovers_from_waits_that_give_up(ctx, all_forms, name):
+    """Exact results of whole numbers; then the shortest wait limit: every call ends and reports (a short one may well finish within the
+    time that a barrier waits by itself), the context stays usable, and the same call is right again."""
+    _, kernel, call, outs, refs = all_forms[name]
+    call()
+    assert ctx.last_kernel() == kernel
+    for o, r in zip(outs, refs):
+        assert torch.equal(get(o).double(), r)
+    ctx.set_wait_limit(1)
+    try:
+        for _ in range(20):
+            call()
+            st = ctx.sync(check=False)
+            if st == tb.Status.INTERNAL:
+                break
+    finally:
+        ctx.set_wait_limit(4000000000)
+    assert st in (tb.Status.OK, tb.Status.INTERNAL)
+    for _ in range(2):
+        call()
+        for o, r in zip(outs, refs):
+            assert torch.equal(get(o).double(), r)
+
+
+@pytest.mark.parametrize("name", FORMS)
+def test_plain_launches_give_the_same(ctx, all_forms, name):
+    """Without programmatic launches, and with them back to back: calls that follow one another closely share workspaces."""
+    _, _, call, outs, refs = all_forms[name]
+    for overlap in (0, 1):
+        ctx.set_launch_overlap(overlap)
+        for _ in range(5):
+            call()
+        for o, r in zip(outs, refs):
+            assert torch.equal(get(o).double(), r)
+    ctx.set_launch_overlap(1)
+
+
+def test_forms_one_after_another(ctx, all_forms):
+    """Every form behind every other without a wait between them: none reads what the one before has not written yet, and none
+    starts writing into a workspace that is still read."""
+    names = list(all_forms)
+    for i, a in enumerate(names):
+        b = names[(i * 5 + 3) % len(names)]
+        for n in (a, b, a):
+            all_forms[n][2]()
+        for n in (a, b):
+            for o, r in zip(all_forms[n][3], all_forms[n][4]):
+                assert torch.equal(get(o).double(), r), (a, b)
+
+
+def test_two_contexts_at_once():
+    """The same forms from two contexts (two streams, two threads) at once."""
+    import threading
+    errors = []
+
+    def work(shift):
+        try:
+            with tb.Context(0) as c:
+                made = forms(c)
+                for rep in range(3):
+                    for i in range(len(made)):
+                        made[(i + shift) % len(made)][2]()
+                    for _, _, _, outs, refs in made:
+                        for o, r in zip(outs, refs):
+                            assert torch.equal(get(o).double(), r)
+        except Exception as e:    # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(s,)) for s in (0, 6)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+
+
+def test_more_batches_than_a_grid_has_rows(ctx):
+    n, h, c, w = 70000, 1, 8, 8
+    a, bg, bu = whole(1, "fp16", -2, 3, n, h, c), whole(2, "fp16", -2, 3, n, c, w), whole(3, "fp16", -2, 3, n, c, w)
+    ts, out = [put(ctx, t) for t in (a, bg, bu)], blank(ctx, "fp32", (n, h, w))
+    ctx.matmul_gated(*ts, out, "RELU")
+    a, bg, bu = a.double(), bg.double(), bu.double()
+    assert torch.equal(get(out).double(), (a @ bg).clamp(min=0) * (a @ bu))
+    for t in ts + [out]:
+        t.free()
+
+
+def test_operands_inside_larger_tensors(ctx):
+    """Contiguous cuts along the first dimension start at any multiple of sixteen bytes; what lies beside an output stays as it was."""
+    c, w = 72, 40
+    big_a, big_b = put(ctx, whole(1, "fp16", -2, 3, 5, 9, c)), put(ctx, whole(2, "fp16", -2, 3, 4, c, w))
+    big_o = put(ctx, torch.full((7, 9, w), 5.0))
+    out = big_o.slice([2, 0, 0], [2, 9, w])
+    ctx.matmul_gated(big_a.slice([3, 0, 0], [2, 9, c]), big_b.slice([0, 0, 0], [2, c, w]), big_b.slice([2, 0, 0], [2, c, w]), out, "RELU")
+    a, b = whole(1, "fp16", -2, 3, 5, 9, c).double()[3:], whole(2, "fp16", -2, 3, 4, c, w).double()
+    got = get(big_o).double()
+    assert torch.equal(got[2:4], (a @ b[:2]).clamp(min=0) * (a @ b[2:]))
+    assert (got[:2] == 5).all() and (got[4:] == 5).all()
+    with pytest.raises(tb.Tb200Error):    # a cut that leaves gaps
+        ctx.matmul_gated(big_a.slice([0, 0, 0], [2, 8, c]), big_b.slice([0, 0, 0], [2, c, w]), big_b.slice([2, 0, 0], [2, c, w]), out, "RELU")
+
+
+def test_capture_before_the_first_call():
+    """A call that would have to make workspaces is refused while capturing; after it has run once it can be captured, and a workspace that
+    grows under a live graph leaves the graph's alone."""
+    with tb.Context(0) as c:
+        x = whole(1, "fp16", -1, 2, 1, 2, 640)
+        m = Four(c, 2, 640, 256, 64, True, True, "fp16")
+        a, out, big = put(c, x), blank(c, "fp32", (1, 2, 256)), blank(c, "fp32", (1, 300, 256))
+        c.capture_begin()
+        with pytest.raises(tb.Tb200Error):
+            c.matmul_w4(a, m.op, out)
+        c.graph_destroy(c.capture_end())
+        c.matmul_w4(a, m.op, out)
+        ref = get(out)
+        c.capture_begin()
+        c.matmul_w4(a, m.op, out)
+        graph = c.capture_end()
+        c.matmul_w4(put(c, whole(3, "fp16", -1, 2, 1, 300, 640)), m.op, big)    # a larger workspace
+        wide = Four(c, 4, 64, 700000, 64, False, True, "fp16")                    # more counters
+        c.matmul_w4(put(c, whole(5, "fp16", -1, 2, 1, 1, 64)), wide.op, blank(c, "fp32", (1, 1, 700000)))
+        for _ in range(3):
+            out.upload(np.full((1, 2, 256), np.nan, np.float32))
+            c.graph_launch(graph)
+            assert torch.equal(get(out), ref)
+        c.graph_destroy(graph)
