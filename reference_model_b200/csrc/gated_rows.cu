@@ -225,12 +225,11 @@ __global__ void __launch_bounds__(kFewThreads) gated_rows_kernel(const __grid_co
         ptx::cluster_sync();
     else
         __syncthreads();
-    const int items = min(p.H - row0, 8 * NT) * kFewCols;
-    for (int e = (int)rank * kFewThreads + tid; e < items && !timed_out; e += p.splits * kFewThreads)
+    // a thread stays with its column; the cluster's blocks share the rows out
+    const int rows = min(p.H - row0, 8 * NT), c = tid % kFewCols;
+    constexpr int kStep = 32 * kFewWarps / kFewCols;
+    for (int n = (int)rank * kStep + tid / kFewCols; n < rows && tid < 32 * kFewWarps && col0 + c < p.W && !timed_out; n += p.splits * kStep)
     {
-        const int n = e / kFewCols, c = e % kFewCols;
-        if (col0 + c >= p.W)
-            continue;
         float v[2];
 #pragma unroll
         for (int m = 0; m < 2; m++)

@@ -409,23 +409,27 @@ __global__ void __launch_bounds__(kRowsThreads, rows_blocks_sm(NT)) w4_rows_kern
 #pragma unroll
         for (int c = 0; c < 2; c++)
             offX[c] = (uint32_t)(half * 2 * 8 * NT * 128 + xr * 128) + (uint32_t)(((c * 4 + t) ^ xr) << 4);
-        const int values = p.rows * p.parts * kRowsTile, items = p.rows * kPer;
+        const int values = p.rows * p.parts * kRowsTile;
         // results of a tile whose sums are in `red`
         auto results = [&](int col0) {
-            for (int e = tid; e < items; e += 32 * kRowsWarps)
+            // a thread stays with its column
+            const int c = tid % kPer;
+            if (col0 + c >= p.W)
+                return;
+            constexpr int kStep = 32 * kRowsWarps / kPer;
+            const int64_t out   = (int64_t)(tid / kPer) * p.W + col0 + c;
+            const float* at     = red + tid / kPer * p.parts * kRowsRedLd + c;
+#pragma unroll 4
+            for (int r = tid / kPer, i = 0; r < p.rows; r += kStep, i++)
             {
-                const int r = e / kPer, c = e % kPer;
-                if (col0 + c >= p.W)
-                    continue;
                 float v[MATS];
 #pragma unroll
                 for (int m = 0; m < MATS; m++)
                 {
-                    v[m] = 0.f;
-                    for (int part = p.parts - 1; part >= 0; part--)    // the smallest first
-                        v[m] += red[(r * p.parts + part) * kRowsRedLd + m * kPer + c];
+                    const float* const x = at + (int64_t)i * kStep * p.parts * kRowsRedLd + m * kPer;
+                    v[m]                 = p.parts == 3 ? x[2 * kRowsRedLd] + x[kRowsRedLd] + x[0] : x[0];    // the smallest first
                 }
-                store_fp(p.out, (int64_t)r * p.W + col0 + c, p.out_dt, MATS == 2 ? act_value(p.act, v[0]) * v[MATS - 1] : v[0]);
+                store_fp(p.out, out + (int64_t)i * kStep * p.W, p.out_dt, MATS == 2 ? act_value(p.act, v[0]) * v[MATS - 1] : v[0]);
             }
         };
         constexpr int kSlot = 8 * NT * kRowsTile;
@@ -543,6 +547,7 @@ __global__ void __launch_bounds__(kRowsThreads, rows_blocks_sm(NT)) w4_rows_kern
         const bool share_first = n_first < S, share_last = tile_last > tile0 && n_last < S;
         if (tid == 0)
         {
+            // (the block's sums, which the barrier above has put before this, are published with the addition)
             __threadfence();    // the block's sums, which the barrier above has put before this
             const int first = share_first ? atomicAdd(p.counts + tile0, n_first) : 0, last = share_last ? atomicAdd(p.counts + tile_last, n_last) : 0;
             completes[0]    = share_first && first + n_first == S;
