@@ -151,6 +151,7 @@ struct tb200_ctx
     uint32_t pair_epoch  = 0;          // bumped per launch; a flag equal to it means "written in this launch"
     int* ffn_count       = nullptr;    // arrivals at shared tiles of 4-bit products; zero whenever none runs
     int ffn_counts       = 0;
+    int ffn_clusters[3] = {};     // clusters of 2, 4 and 8 CTAs of the feed-forward products that run at once, when known
     void* stage          = nullptr;    // grow-on-demand staging of TRANSPOSE_CONV2D (spread input, mirrored weights)
     size_t stage_bytes   = 0;
     void* io_pinned      = nullptr;    // 64 MiB pinned host buffer of the .npy loader / writer, allocated on first use

@@ -290,13 +290,14 @@ tb200_status gated_backward_f32(tb200_ctx* ctx, const GatedProblem& q)
     return post_launch(ctx, "gated_backward_f32", 0);
 }
 
-// 4-bit weights: few rows read them as they are; more go through the values laid out in scratch, in a's type.
+// 4-bit weights: few rows multiply whole numbers and scale the sums; more take the weights' values, rounded to a's type as a tile needs them.  Many fp32
+// rows go through fp32 values laid out in scratch.
 tb200_status w4_launch(tb200_ctx* ctx, const W4Problem& q)
 {
     const bool f32      = q.dt == TB200_FP32;
     const int parts     = f32 ? 3 : 1;
     const int64_t xpitch = round_up(q.C, 8);
-    const int64_t wpitch = round_up((q.C + 1) / 2, 16), dpitch = round_up(q.C, 32);
+    const int64_t wpitch = round_up((q.C + 1) / 2, 16);
     const bool few       = q.M * parts <= kFewRows;
     const bool copy_x    = !f32 && q.C % 8 != 0;
     const int64_t n      = q.M * q.W;
@@ -307,7 +308,7 @@ tb200_status w4_launch(tb200_ctx* ctx, const W4Problem& q)
         x = c.take(few && f32 ? (size_t)q.M * 3 * xpitch * 2 : copy_x ? (size_t)q.M * xpitch * 2 : 0);
         for (int i = 0; i < q.mats; i++)
         {
-            w[i]    = c.take(few ? (q.w[i].pitch % 16 ? (size_t)q.W * wpitch : 0) : f32 ? (size_t)q.C * q.W * 4 : (size_t)q.W * dpitch * 2);
+            w[i]    = c.take(!few && f32 ? (size_t)q.C * q.W * 4 : q.w[i].pitch % 16 ? (size_t)q.W * wpitch : 0);
             proj[i] = c.take(!few && f32 && q.mats == 2 ? (size_t)n * 4 : 0);
         }
         partial = c.take(few ? w4_rows_partial_bytes(ctx, q.M * parts) : 0);
@@ -319,28 +320,9 @@ tb200_status w4_launch(tb200_ctx* ctx, const W4Problem& q)
             c.base = reinterpret_cast<uint8_t*>(ctx->scratch);
         }
     }
-    if (few)
+    if (!few && f32)
     {
-        W4Problem r = q;
-        RowCopies copies;
-        for (int i = 0; i < q.mats; i++)
-            if (q.w[i].pitch % 16)
-            {
-                copies.add(q.w[i].data, w[i], q.W, (q.C + 1) / 2, q.w[i].pitch, wpitch);
-                r.w[i].data  = reinterpret_cast<const uint8_t*>(w[i]);
-                r.w[i].pitch = wpitch;
-            }
-        if (f32)
-            copies.add(q.a, x, q.M, (int64_t)q.C * 4, (int64_t)q.C * 4, xpitch * 2, true);
-        else if (copy_x)
-            copies.add(q.a, x, q.M, (int64_t)q.C * 2, (int64_t)q.C * 2, xpitch * 2);
-        TB200_TRY(row_copies_launch(ctx, copies));
-        return w4_rows_launch(ctx, r, f32 || copy_x ? x : q.a, f32 || copy_x ? xpitch : q.C, parts, f32 || q.dt == TB200_BF16,
-                              reinterpret_cast<float*>(partial));
-    }
-    TB200_TRY(w4_dense_launch(ctx, q.w, q.mats, q.C, q.W, q.group, q.dt, w, dpitch));
-    if (f32)
-    {
+        TB200_TRY(w4_dense_launch(ctx, q.w, q.mats, q.C, q.W, q.group, w));
         for (int i = 0; i < q.mats; i++)
             TB200_TRY(sgemm_f32_launch(ctx, reinterpret_cast<const float*>(q.a), reinterpret_cast<const float*>(w[i]),
                                        reinterpret_cast<float*>(q.mats == 2 ? proj[i] : q.out), 1, (int)q.M, q.C, q.W));
@@ -349,16 +331,30 @@ tb200_status w4_launch(tb200_ctx* ctx, const W4Problem& q)
                                       q.act));
         return post_launch(ctx, q.mats == 2 ? "gated_w4_f32" : "matmul_w4_f32", 0);
     }
+    W4Problem r = q;
+    RowCopies copies;
+    for (int i = 0; i < q.mats; i++)
+        if (q.w[i].pitch % 16)
+        {
+            copies.add(q.w[i].data, w[i], q.W, (q.C + 1) / 2, q.w[i].pitch, wpitch);
+            r.w[i].data  = reinterpret_cast<const uint8_t*>(w[i]);
+            r.w[i].pitch = wpitch;
+        }
+    if (f32)
+        copies.add(q.a, x, q.M, (int64_t)q.C * 4, (int64_t)q.C * 4, xpitch * 2, true);
+    else if (copy_x)
+        copies.add(q.a, x, q.M, (int64_t)q.C * 2, (int64_t)q.C * 2, xpitch * 2);
+    TB200_TRY(row_copies_launch(ctx, copies));
+    if (few)
+        return w4_rows_launch(ctx, r, f32 || copy_x ? x : q.a, f32 || copy_x ? xpitch : q.C, parts, f32 || q.dt == TB200_BF16,
+                              reinterpret_cast<float*>(partial));
     PairProduct k;
     memset(&k, 0, sizeof(k));
-    k.dt   = q.dt;
-    k.kind = q.mats == 2 ? PAIR_GATED : PAIR_PLAIN;
-    k.a    = operand(q.a, q.C, q.M, 1, x);
-    RowCopies copies;
-    pad(&copies, q.a, k.a);
-    TB200_TRY(row_copies_launch(ctx, copies));
-    for (int i = 0; i < q.mats; i++)
-        k.b[i] = { w[i], q.C, q.W, 1, dpitch };
+    k.dt        = q.dt;
+    k.kind      = q.mats == 2 ? PAIR_GATED : PAIR_PLAIN;
+    k.a         = operand(q.a, q.C, q.M, 1, x);
+    k.w4        = r.w;
+    k.group     = q.group;
     k.rows      = (int)q.M;
     k.cols      = q.W;
     k.K         = q.C;
@@ -377,11 +373,6 @@ tb200_status w4_launch(tb200_ctx* ctx, const W4Problem& q)
 bool tiles_reach(int64_t rows, int64_t C, int64_t W)
 {
     return rows <= (1 << 30) && C <= (1 << 30) && W <= (1 << 29);
-}
-
-size_t aligned(size_t bytes)
-{
-    return (bytes + 255) & ~(size_t)255;
 }
 
 // A sum over nothing is zero in every type.
@@ -422,7 +413,10 @@ tb200_status w4_entry(tb200_ctx* ctx, const char* op, const tb200_tensor* a, con
         q.w[i].scale_dt = mats[i]->scale->dtype;
         q.w[i].zero     = mats[i]->zero ? reinterpret_cast<const int8_t*>(mats[i]->zero->data) : nullptr;
     }
-    return ctx->policy == 0 && tiles_reach(q.M, q.C, q.W) ? w4_launch(ctx, q) : w4_direct_launch(ctx, q);
+    // (scales of any width are read as one row, whose elements have 32-bit coordinates)
+    const int64_t groups = ((int64_t)q.C + q.group - 1) / q.group;
+    const bool tiled     = ctx->policy == 0 && tiles_reach(q.M, q.C, q.W) && groups * q.W < (1LL << 31) - 256;
+    return tiled ? w4_launch(ctx, q) : w4_direct_launch(ctx, q);
 }
 
 GatedProblem gated_problem(const tb200_tensor* a, const tb200_tensor* gate, const tb200_tensor* up, int activation)
@@ -532,11 +526,11 @@ extern "C" tb200_status tb200_matmul_gated_backward(tb200_ctx* ctx, const tb200_
         }
         if (ctx->policy == 0 && tiles_reach(q.H, q.C, q.W))
             return q.dt == TB200_FP32 ? gated_backward_f32(ctx, q) : gated_backward_pair(ctx, q);
-        const size_t each     = aligned((size_t)q.NB * q.H * q.W * sizeof(float));
+        const size_t each     = (size_t)q.NB * q.H * q.W * sizeof(float);
         const tb200_status st = ensure_scratch(ctx, 2 * each);
         if (st != TB200_OK)
             return st;
         float* const dg = reinterpret_cast<float*>(ctx->scratch);
-        return gated_backward_direct_launch(ctx, q, dg, reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(ctx->scratch) + each));
+        return gated_backward_direct_launch(ctx, q, dg, dg + each / sizeof(float));
     });
 }

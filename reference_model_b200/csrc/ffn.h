@@ -88,6 +88,8 @@ struct PairProduct
     void* out[2];
     tb200_dtype out_dt[2];
     int64_t ld;        // elements from one result row to the next
+    const W4Mat* w4;   // in b's place: 4-bit matrices, rows a multiple of 16 bytes apart (PAIR_PLAIN and PAIR_GATED, NB and phases 1)
+    int group;
     const char* name;
 };
 tb200_status pair_launch(tb200_ctx* ctx, const PairProduct& q);
@@ -119,8 +121,8 @@ struct RowCopies
     void add(const void* in, void* out, int64_t rows, int64_t inner, int64_t in_pitch, int64_t pitch, bool split = false);
 };
 tb200_status row_copies_launch(tb200_ctx* ctx, const RowCopies& q);
-// [W][pitch] 16-bit rows of one or two 4-bit matrices' values, or fp32 [C][W] (dt FP32)
-tb200_status w4_dense_launch(tb200_ctx* ctx, const W4Mat* w, int mats, int C, int W, int group, tb200_dtype dt, void* const* out, int64_t pitch);
+// fp32 values [C][W] of one or two 4-bit matrices
+tb200_status w4_dense_launch(tb200_ctx* ctx, const W4Mat* w, int mats, int C, int W, int group, void* const* out);
 tb200_status gate_f32_launch(tb200_ctx* ctx, const float* g, const float* u, float* out, int64_t n, int act);
 // g and u hold dG and dU afterwards, `both` (or null) the two side by side
 tb200_status grad_f32_launch(tb200_ctx* ctx, float* g, float* u, const float* d, float* both, int64_t rows, int W, int act);

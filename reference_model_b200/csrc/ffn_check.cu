@@ -68,7 +68,7 @@ std::string check_w4(const char* op, const tb200_tensor* a, const tb200_w4* cons
             return say("%s: zero-copy views are accepted only as the CONV2D input; this operand must be contiguous", op);
         if (d->shape[0] != W)
             return say("%s: the weights must have a row for each of the output's %d columns", op, W);
-        if (d->shape[1] < (C + 1) / 2)
+        if (d->shape[1] < C / 2 + C % 2)
             return say("%s: a weight row of %d bytes does not hold %d elements", op, d->shape[1], C);
         if (group < 1 || (group % 32 != 0 && group < C))
             return say("%s: a group must be a multiple of 32 elements, or hold a whole row", op);

@@ -27,6 +27,13 @@ __device__ __forceinline__ float act_value(float g)
     return 1.f / (1.f + expf(-g));
 }
 
+// 1 + 3 * 0.044715 g^2 of GELU_TANH's derivative.  Where s (1 - s) has long been 0 the square must not overflow beside it.
+__device__ __forceinline__ float tanh_growth(float g)
+{
+    const float c = fminf(fabsf(g), 1e9f);
+    return 1.f + 0.134145f * c * c;
+}
+
 // Value and derivative.
 template <int ACT>
 __device__ __forceinline__ void act_slope(float g, float& value, float& slope)
@@ -47,7 +54,7 @@ __device__ __forceinline__ void act_slope(float g, float& value, float& slope)
     {
         const float s = 1.f / (1.f + expf(-1.5957691216057308f * (g + 0.044715f * g * g * g)));
         value         = g * s;
-        slope         = s + g * s * (1.f - s) * 1.5957691216057308f * (1.f + 0.134145f * g * g);
+        slope         = s + g * s * (1.f - s) * 1.5957691216057308f * tanh_growth(g);
     }
     else
     {
@@ -103,7 +110,7 @@ __device__ __forceinline__ void act_slope_16(float g, float& value, float& slope
     {
         const float s = __fdividef(1.f, 1.f + __expf(-1.5957691216057308f * (g + 0.044715f * g * g * g)));
         value         = g * s;
-        slope         = s + g * s * (1.f - s) * 1.5957691216057308f * (1.f + 0.134145f * g * g);
+        slope         = s + g * s * (1.f - s) * 1.5957691216057308f * tanh_growth(g);
     }
     else
         act_slope<ACT>(g, value, slope);
@@ -164,6 +171,12 @@ __device__ __forceinline__ float load_fp(const void* p, int64_t i, tb200_dtype d
     if (dt == TB200_FP16)
         return __half2float(reinterpret_cast<const __half*>(p)[i]);
     return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p)[i]);
+}
+
+// The number that an element's bits stand for
+__device__ __forceinline__ float bits_fp(uint32_t bits, tb200_dtype dt)
+{
+    return dt == TB200_FP32 ? __uint_as_float(bits) : dt == TB200_BF16 ? __uint_as_float(bits << 16) : __half2float(__ushort_as_half((unsigned short)bits));
 }
 
 // Results are rounded once, to nearest, where they are stored.

@@ -14,10 +14,12 @@
 #include <algorithm>
 #include <cstring>
 #include <cuda.h>
+#include <type_traits>
 
 #include "ffn.h"
 #include "ffn_math.cuh"
 #include "ptx_sm100.cuh"
+#include "w4_unpack.cuh"
 
 namespace tb200
 {
@@ -27,17 +29,21 @@ namespace
 {
 
 constexpr int kEpiWarps = 8;
-constexpr int kThreads  = 64 + 32 * kEpiWarps;    // TMA warp, MMA warp, epilogue
+constexpr int kExpandGroups = 3;                  // of four warps: 4-bit weights to 16 bits
+constexpr int kExpandWarps = 4 * kExpandGroups;
+constexpr int kRawBytes    = 128 * 32;            // 128 rows x 64 elements of 4-bit weights
 constexpr int kChunk    = 16384;                  // 128 rows (or columns) x 64 elements of K
 
 // Pairs of CTAs (PAIR) with tiles of 256 rows and 256 accumulator columns, or CTAs by themselves with 128 x 128; one CTA to an SM.
-template <bool PAIR>
+template <bool PAIR, bool W4 = false>
 struct Shape
 {
-    static constexpr int kStages = PAIR ? 3 : 6;
+    static constexpr int kThreads = 64 + 32 * (kEpiWarps + (W4 ? kExpandWarps : 0));    // TMA warp, MMA warp, epilogue, and those
+    static constexpr int kStages = PAIR && !W4 ? 3 : 6;
+    static_assert(!W4 || kStages % kExpandGroups == 0, "a group keeps to its stages");
     static constexpr int kCtas = PAIR ? 2 : 1;
     static constexpr int kRows = 128 * kCtas, kCols = PAIR ? 256 : 128;    // of a tile
-    static constexpr int kSub  = PAIR ? 2 : 1;                             // chunks per stage
+    static constexpr int kSub  = PAIR && !W4 ? 2 : 1;                      // chunks per stage
     static constexpr int kStage = 2 * kSub * kChunk;                       // each CTA holds 128 rows of A and 128 columns of B
     // (with the static part all of an SM's: a CTA that waits for tensor memory never shares an SM with another kernel's that holds some)
     static constexpr int kSmem  = 208 * 1024;
@@ -72,6 +78,12 @@ struct Params
     int even;              // whole pairs of elements in every row, at 4-byte addresses
     const void* dout;      // [NB][rows][cols]
     int dout_vec;          // its rows may be read 16 bytes at a time
+    // 4-bit weights: tmB0 and tmB1 are [W][pitch] bytes, boxes of 32 bytes
+    const void* scale[2];
+    const int8_t* zero[2];
+    tb200_dtype scale_dt[2];
+    int K, groups;
+    uint32_t group32;      // of 32 elements
     long long wait_limit;
     int* status;
 };
@@ -161,7 +173,7 @@ __device__ __forceinline__ void grad_run(const uint32_t (&g)[16], const uint32_t
     {
         float value, slope;
         act_slope_16<ACT>(__uint_as_float(g[i]), value, slope);
-        dg[i] = d[i] * __uint_as_float(u[i]) * slope;
+        dg[i] = d[i] * slope * __uint_as_float(u[i]);    // (the slope is 1.13 at most: only the result itself can overflow)
         du[i] = d[i] * value;
     }
 }
@@ -314,7 +326,7 @@ __device__ __forceinline__ void finish_quad(const Params& p, const Tile& t, int 
             const float d = i < n ? load_fp(p.dout, at + i, p.bf16 ? TB200_BF16 : TB200_FP16) : 0.f;
             float value, slope;
             act_slope_16(p.act, g[i], value, slope);
-            dg[i] = d * u[i] * slope;
+            dg[i] = d * slope * u[i];
             du[i] = d * value;
         }
         store_quad(p.out0, orow, p.out_dt, n, p.vec, dg);
@@ -322,19 +334,83 @@ __device__ __forceinline__ void finish_quad(const Params& p, const Tile& t, int 
     }
 }
 
-template <int EPI, bool A_MN, bool B_MN, bool PAIR>
-__global__ void __launch_bounds__(kThreads, 1) ffn_pair_kernel(const __grid_constant__ Params p)
+// Elements as bits, by one instruction into their register, so that the thread goes on without them (a conversion, or a choice between two
+// loads' results, waited for each here: 2100 cycles a chunk).
+__device__ __forceinline__ void load_bits(uint32_t& v, const uint8_t* at, bool wide)
 {
-    using S               = Shape<PAIR>;
-    constexpr int kSub    = S::kSub, kStage = S::kStage, kHalf = S::kCols / 2, kStages = S::kStages;
+    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t@q ld.global.b32 %0, [%1];\n\t@!q ld.global.u16 %0, [%1];\n\t}"
+                 : "=r"(v)
+                 : "l"(at), "r"((int)wide));
+}
+
+__device__ __forceinline__ void load_zero(int& v, const int8_t* at, bool any)
+{
+    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\tmov.b32 %0, 0;\n\t@q ld.global.s8 %0, [%1];\n\t}" : "=r"(v) : "l"(at), "r"((int)any));
+}
+
+// A row's 64 elements of 4-bit weights (two sixteens of bytes) as 16-bit values in a chunk of B: 128 bytes, swizzled.  Values are rounded to the
+// operands' type, once: by scales of that type (SAME) as they are, by others in fp32.  TAIL: `left` elements up to the end of K.
+template <bool BF16, bool SAME, bool TAIL>
+__device__ __forceinline__ void expand_row(const uint4 (&raw)[2], const uint32_t (&bits)[2], tb200_dtype scale_dt, const int (&zero)[2], int left, uint32_t dst, int row)
+{
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+    {
+        const uint32_t w[4] = { raw[h].x, raw[h].y, raw[h].z, raw[h].w };
+        const uint32_t base = unpack_base<BF16>(zero[h]), s2 = bits[h] * 0x10001u;
+        const float scale   = SAME ? 0.f : bits_fp(bits[h], scale_dt);
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+        {
+            uint32_t v[4], o[4];
+            unpack8<BF16>(w[i], base, v);
+            o[0] = __byte_perm(v[0], v[1], 0x5410);
+            o[1] = __byte_perm(v[2], v[3], 0x5410);
+            o[2] = __byte_perm(v[0], v[1], 0x7632);
+            o[3] = __byte_perm(v[2], v[3], 0x7632);
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+            {
+                if (SAME)
+                    o[j] = BF16 ? fma2_bf16(o[j], s2, 0x80008000u) : fma2_f16(o[j], s2, 0x80008000u);
+                else
+                {
+                    const float2 f = unpack2(o[j], BF16);
+                    o[j]           = pack2(f.x * scale, f.y * scale, BF16);
+                }
+            }
+            if (TAIL)
+            {
+                // behind the end lies whatever the row holds there, under a scale that may not be finite
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                {
+                    const int at = h * 32 + i * 8 + j * 2;
+                    o[j]         = at + 1 < left ? o[j] : at < left ? o[j] & 0xffffu : 0u;
+                }
+            }
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + (uint32_t)(((h * 4 + i) ^ (row & 7)) << 4)), "r"(o[0]), "r"(o[1]), "r"(o[2]),
+                         "r"(o[3])
+                         : "memory");
+        }
+    }
+}
+
+template <int EPI, bool A_MN, bool B_MN, bool PAIR, bool W4 = false>
+__global__ void __launch_bounds__((Shape<PAIR, W4>::kThreads), 1) ffn_pair_kernel(const __grid_constant__ Params p)
+{
+    static_assert(W4 || EPI == EPI_PLAIN || B_MN, "both projections' matrices have K across their rows");
+    using S               = Shape<PAIR, W4>;
+    constexpr int kSub    = S::kSub, kStage = S::kStage, kHalf = S::kCols / 2, kStages = S::kStages, kThreads = S::kThreads;
     extern __shared__ uint8_t smem_raw[];
     // identical layout in both CTAs of a pair: remote signals address a barrier by its offset
-    __shared__ __align__(8) uint64_t bar_full[kStages];     // used in the first CTA: bytes of both CTAs
+    __shared__ __align__(8) uint64_t bar_full[kStages];     // used in the first CTA: bytes of both CTAs, values of 4-bit weights in place
     __shared__ __align__(8) uint64_t bar_empty[kStages];    // per CTA: stage consumed by the MMAs
     __shared__ __align__(8) uint64_t bar_tmem_full[2];         // per CTA: accumulator buffer complete
     __shared__ __align__(8) uint64_t bar_tmem_empty[2];        // first CTA: buffer drained by both CTAs' epilogues
     __shared__ __align__(8) uint64_t bar_ready;                // first CTA: tensor memory taken in both
     __shared__ __align__(8) uint64_t bar_drain;                // first CTA: MMAs in flight when the issuer gives up
+    __shared__ __align__(8) uint64_t bar_raw[W4 ? kStages : 1];         // per CTA: 4-bit weights of the stage
     __shared__ uint32_t tmem_base_holder;
     __shared__ float stages[kEpiWarps][32 * 17];    // of the epilogue's warps
 
@@ -353,8 +429,10 @@ __global__ void __launch_bounds__(kThreads, 1) ffn_pair_kernel(const __grid_cons
     {
         for (int s = 0; s < kStages; s++)
         {
-            ptx::mbar_init(ptx::smem_u32(&bar_full[s]), 1);
+            ptx::mbar_init(ptx::smem_u32(&bar_full[s]), 1 + (W4 ? 4 * S::kCtas : 0));    // (and a group's warps)
             ptx::mbar_init(ptx::smem_u32(&bar_empty[s]), 1);
+            if (W4)
+                ptx::mbar_init(ptx::smem_u32(&bar_raw[s]), 1);
         }
         for (int a = 0; a < 2; a++)
         {
@@ -368,18 +446,25 @@ __global__ void __launch_bounds__(kThreads, 1) ffn_pair_kernel(const __grid_cons
         ptx::prefetch_tmap(&p.tmB0);
         ptx::prefetch_tmap(&p.tmB1);
         // the first weights on their way to L2, where a write by the kernel before would still find them
-        if (EPI != EPI_PLAIN && cluster_id < p.num_tiles)
+        if (W4 && cluster_id < p.num_tiles)
+        {
+            const Tile t = decode<EPI, PAIR>(p, cluster_id);
+            for (int c = chunk0; c < chunk0 + min(total, kStages); c++)
+            {
+                ptx::prefetch_2d(EPI != EPI_PLAIN && rank ? &p.tmB1 : &p.tmB0, c * 32, EPI == EPI_PLAIN ? t.n0 + (int)rank * 128 : t.n0);
+                if (EPI != EPI_PLAIN && !PAIR)
+                    ptx::prefetch_2d(&p.tmB1, c * 32, t.n0);
+            }
+        }
+        else if (EPI != EPI_PLAIN && cluster_id < p.num_tiles)
         {
             const Tile t = decode<EPI, PAIR>(p, cluster_id);
             for (int c = chunk0; c < min(p.chunks, chunk0 + min(total, kStages * kSub)); c++)
                 for (int m = PAIR ? (int)rank : 0; m < (PAIR ? (int)rank + 1 : 2); m++)
                 {
                     const CUtensorMap* const b = m ? &p.tmB1 : &p.tmB0;
-                    if (!B_MN)
-                        ptx::prefetch_3d(b, c * 64, t.n0, t.idx);
-                    else
-                        for (int n = 0; n < kHalf; n += 64)
-                            ptx::prefetch_3d(b, t.n0 + n, c * 64, t.idx);
+                    for (int n = 0; n < kHalf; n += 64)
+                        ptx::prefetch_3d(b, t.n0 + n, c * 64, t.idx);
                 }
         }
     }
@@ -447,7 +532,7 @@ __global__ void __launch_bounds__(kThreads, 1) ffn_pair_kernel(const __grid_cons
                     const uint32_t full_local = ptx::smem_u32(&bar_full[stage]);
                     // the first CTA arms the barrier with the bytes of both CTAs; each CTA's copies report there
                     if (rank == 0)
-                        ptx::mbar_arrive_expect_tx(full_local, (uint32_t)(nch * 2 * S::kCtas * kChunk));
+                        ptx::mbar_arrive_expect_tx(full_local, (uint32_t)(nch * (W4 ? 1 : 2) * S::kCtas * kChunk));
                     const uint32_t full_first = PAIR ? ptx::map_to_cta(full_local, 0) : full_local;
                     const uint32_t sA         = smem_base + (uint32_t)(stage * kStage);
                     const uint32_t sB         = sA + (uint32_t)(kSub * kChunk);
@@ -469,19 +554,21 @@ __global__ void __launch_bounds__(kThreads, 1) ffn_pair_kernel(const __grid_cons
                         }
                         else
                             load(dA, &p.tmA, k, m0, batch + ph * p.NB);
+                        if (W4)
+                        {
+                            // where their values will be
+                            const uint32_t raw = ptx::smem_u32(&bar_raw[stage]);
+                            ptx::mbar_arrive_expect_tx(raw, kRawBytes);
+                            ptx::tma_load_2d(dB, EPI != EPI_PLAIN && rank ? &p.tmB1 : &p.tmB0, raw, c * 32, n0);
+                            if (EPI != EPI_PLAIN && !PAIR)
+                                ptx::tma_load_2d(dB + kRawBytes / 2, &p.tmB1, raw, c * 32, n0);
+                            continue;
+                        }
                         if (EPI != EPI_PLAIN && !PAIR)
                         {
                             // one CTA holds 64 columns of each matrix
-                            if (B_MN)
-                            {
-                                load(dB, &p.tmB0, n0, k, b_batch);
-                                load(dB + 8192, &p.tmB1, n0, k, b_batch);
-                            }
-                            else
-                            {
-                                load(dB, &p.tmB0, k, n0, b_batch);
-                                load(dB + 8192, &p.tmB1, k, n0, b_batch);
-                            }
+                            load(dB, &p.tmB0, n0, k, b_batch);
+                            load(dB + 8192, &p.tmB1, n0, k, b_batch);
                             continue;
                         }
                         const CUtensorMap* mb = (EPI == EPI_PLAIN ? ph != 0 : rank != 0) ? &p.tmB1 : &p.tmB0;
@@ -509,6 +596,9 @@ __global__ void __launch_bounds__(kThreads, 1) ffn_pair_kernel(const __grid_cons
                 if (rank == 0)
                     for (int64_t i = max((int64_t)0, issued - kStages); i < issued; i++)
                         ptx::mbar_wait_bounded(ptx::smem_u32(&bar_full[i % kStages]), (uint32_t)(i / kStages) & 1u, ptx::kDrainCycles);
+                if (W4)
+                    for (int64_t i = max((int64_t)0, issued - kStages); i < issued; i++)
+                        ptx::mbar_wait_bounded(ptx::smem_u32(&bar_raw[i % kStages]), (uint32_t)(i / kStages) & 1u, ptx::kDrainCycles);
                 if (PAIR)
                     ptx::settle();
             }
@@ -534,6 +624,7 @@ __global__ void __launch_bounds__(kThreads, 1) ffn_pair_kernel(const __grid_cons
             // the MMAs write both CTAs' tensor memory
             if (PAIR)
                 ok = ptx::mbar_wait_bounded(ptx::smem_u32(&bar_ready), 0, p.wait_limit);
+            bool ready = false;    // the stage is known to be complete
             for (int tile = cluster_id; tile < p.num_tiles && ok; tile += num_clusters)
             {
                 if (!ptx::mbar_wait_bounded(ptx::smem_u32(&bar_tmem_empty[acc]), acc_phase ^ 1u, p.wait_limit))
@@ -546,7 +637,7 @@ __global__ void __launch_bounds__(kThreads, 1) ffn_pair_kernel(const __grid_cons
                 uint32_t accum        = 0;    // the first MMA of a tile overwrites the accumulator
                 for (int left = total; left > 0; left -= kSub)
                 {
-                    if (!ptx::mbar_wait_bounded(ptx::smem_u32(&bar_full[stage]), phase, p.wait_limit))
+                    if (!ready && !ptx::mbar_wait_bounded(ptx::smem_u32(&bar_full[stage]), phase, p.wait_limit))
                     {
                         ok = false;
                         break;
@@ -570,6 +661,9 @@ __global__ void __launch_bounds__(kThreads, 1) ffn_pair_kernel(const __grid_cons
                             // sixteen elements of K: 32 bytes inside the swizzled row, or sixteen rows of 128 bytes
                             ad += A_MN ? 128 : 2;
                             bd += B_MN ? 128 : 2;
+                            // the next stage, looked at while MMAs are queued: a look takes 110 cycles, in which the tensor cores ran dry
+                            if (W4 && m == 1)
+                                ready = ptx::mbar_test(ptx::smem_u32(&bar_full[stage + 1 < kStages ? stage + 1 : 0]), stage + 1 < kStages ? phase : phase ^ 1u);
                         }
                     }
                     // frees the stage in both CTAs once the MMAs above have read it
@@ -597,6 +691,118 @@ __global__ void __launch_bounds__(kThreads, 1) ffn_pair_kernel(const __grid_cons
                 ptx::mbar_wait_bounded(ptx::smem_u32(&bar_drain), 0, ptx::kDrainCycles);
             }
         }
+    }
+    else if (W4 && warp >= 2 + kEpiWarps)
+    {
+        // ------------------------------------------------------------------ 4-bit weights to 16 bits (both CTAs)
+        // Groups of four warps take chunks in turn, a thread a row of 64 elements.  The bytes lie where the values go, so a group has read
+        // all of them before it writes.
+        const int group = (warp - 2 - kEpiWarps) >> 2, row = ((warp - 2 - kEpiWarps) & 3) * 32 + lane;
+        const int mat   = EPI == EPI_PLAIN ? 0 : PAIR ? (int)rank : row >> 6;
+        const int shift = EPI == EPI_PLAIN ? (int)rank * 128 + row : PAIR ? row : row & 63;    // of the thread's column in the tile
+        const bool same = p.scale_dt[mat] == (p.bf16 ? TB200_BF16 : TB200_FP16);
+        bool ok = true, bad = false;
+        int tile = cluster_id, c = chunk0 + group, stage = group;
+        uint32_t phase = 0;
+        int zero[2] = {}, zero_next[2] = {};
+        uint32_t scale[2] = {}, scale_next[2] = {};    // bits
+        // the next chunk's first group, and how many 32-element pieces of it lie before the chunk
+        int first_group = 0;
+        uint32_t into   = 0;
+        // The next chunk's scales and zero points are on their way while this one's values are made.
+        const bool wide          = p.scale_dt[mat] == TB200_FP32;
+        const bool with_zero     = p.zero[mat] != nullptr;
+        const uint8_t* scale_at  = nullptr;    // of the thread's column, first group
+        const int8_t* zero_at    = nullptr;
+        const int scale_step     = p.cols * (wide ? 4 : 2), last_group = p.groups - 1;
+        auto to_column = [&]() {
+            const int col = min(decode<EPI, PAIR>(p, tile).n0 + shift, p.cols - 1);
+            scale_at      = reinterpret_cast<const uint8_t*>(p.scale[mat]) + (int64_t)col * (wide ? 4 : 2);
+            zero_at       = p.zero[mat] + col;
+            first_group   = (int)((uint32_t)(2 * c) / p.group32);
+            into          = (uint32_t)(2 * c) - (uint32_t)first_group * p.group32;
+        };
+        auto fetch = [&]() {
+            const int g0 = min(first_group, last_group), g1 = min(first_group + (into + 1 >= p.group32 ? 1 : 0), last_group);
+            load_bits(scale_next[0], scale_at + (int64_t)g0 * scale_step, wide);
+            load_bits(scale_next[1], scale_at + (int64_t)g1 * scale_step, wide);
+            load_zero(zero_next[0], zero_at + (int64_t)g0 * p.cols, with_zero);
+            load_zero(zero_next[1], zero_at + (int64_t)g1 * p.cols, with_zero);
+        };
+        auto to_tile = [&]() {
+            bool moved = false;
+            for (; c >= chunk0 + total && tile < p.num_tiles; moved = true)
+            {
+                c -= total;
+                tile += num_clusters;
+            }
+            if (moved && tile < p.num_tiles)
+                to_column();
+        };
+        if (tile < p.num_tiles)
+            to_column();
+        to_tile();
+        if (tile < p.num_tiles)
+            fetch();
+        while (tile < p.num_tiles && ok)
+        {
+            const int left = p.K - c * 64;
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+            {
+                scale[h] = scale_next[h];
+                zero[h]  = zero_next[h];
+                bad |= zero[h] < -8 || zero[h] > 7;
+            }
+            c += kExpandGroups;
+            for (into += 2 * kExpandGroups; into >= p.group32; into -= p.group32)
+                first_group++;
+            to_tile();
+            if (tile < p.num_tiles)
+                fetch();
+            const uint32_t sB = smem_base + (uint32_t)(stage * kStage + kChunk);
+            ok                = ptx::mbar_wait_bounded(ptx::smem_u32(&bar_raw[stage]), phase, p.wait_limit);
+            uint4 raw[2];
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+                raw[h] = lds128(sB + (uint32_t)(row * 32 + ((h ^ ((row >> 2) & 1)) << 4)));
+            ok = ptx::named_barrier_and(2 + group, 128, ok);
+            if (!ok)
+                break;
+            const uint32_t dst = sB + (uint32_t)(row * 128);
+            auto expand        = [&](auto bf16) {
+                constexpr bool kBf16 = decltype(bf16)::value;
+                if (left < 64)
+                    expand_row<kBf16, false, true>(raw, scale, p.scale_dt[mat], zero, left, dst, row);
+                else if (same)
+                    expand_row<kBf16, true, false>(raw, scale, p.scale_dt[mat], zero, left, dst, row);
+                else
+                    expand_row<kBf16, false, false>(raw, scale, p.scale_dt[mat], zero, left, dst, row);
+            };
+            if (p.bf16)
+                expand(std::true_type());
+            else
+                expand(std::false_type());
+            ptx::fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0)
+            {
+                if (PAIR)
+                    ptx::mbar_arrive_cluster_release(ptx::map_to_cta(ptx::smem_u32(&bar_full[stage]), 0));
+                else
+                    ptx::mbar_arrive(ptx::smem_u32(&bar_full[stage]));
+            }
+            stage += kExpandGroups;
+            if (stage >= kStages)
+            {
+                stage -= kStages;
+                phase ^= 1u;
+            }
+        }
+        if (!ok && lane == 0)
+            atomicOr(p.status, TB200_DEV_TIMEOUT);
+        if (bad)
+            atomicOr(p.status, TB200_DEV_UNPREDICTABLE);
     }
     else
     {
@@ -762,6 +968,23 @@ tb200_status encode(tb200_ctx* ctx, CUtensorMap* m, const Matrix& x, bool bf16, 
     return TB200_OK;
 }
 
+// Rows of 4-bit weights, 64 elements of `lines` of them at a time; eight threads' sixteens of bytes, one from each row, meet all banks.
+tb200_status encode_raw(tb200_ctx* ctx, CUtensorMap* m, const W4Mat& w, int cols, uint32_t lines)
+{
+    const EncodeTiled enc = reinterpret_cast<EncodeTiled>(tensor_map_encode_fn());
+    if (!enc)
+        return fail(ctx, TB200_INTERNAL, "cuTensorMapEncodeTiled is not available from the driver");
+    const cuuint64_t dims[2]    = { (cuuint64_t)w.pitch, (cuuint64_t)cols };
+    const cuuint64_t strides[1] = { (cuuint64_t)w.pitch };
+    const cuuint32_t box[2]     = { 32, lines };
+    const cuuint32_t estr[2]    = { 1, 1 };
+    const CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(w.data), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           CU_TENSOR_MAP_SWIZZLE_32B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS)
+        return fail(ctx, TB200_INTERNAL, "tensor map of 4-bit weights rejected (CUresult %d)", (int)r);
+    return TB200_OK;
+}
+
 int run_alignment(const void* p, int64_t ld, size_t es)
 {
     const uintptr_t bits = reinterpret_cast<uintptr_t>(p) | (uintptr_t)(ld * (int64_t)es);
@@ -778,19 +1001,19 @@ typedef void (*Kern)(const Params);
 template <bool PAIR>
 Kern pick(const PairProduct& q, int* bit)
 {
-    if (q.kind == PAIR_GATED && !q.a_mn)
+    if (q.w4)
     {
-        *bit = q.b_mn ? 0 : 1;
-        return q.b_mn ? ffn_pair_kernel<EPI_GATED, false, true, PAIR> : ffn_pair_kernel<EPI_GATED, false, false, PAIR>;
+        *bit = q.kind == PAIR_GATED ? 5 : 4;
+        return q.kind == PAIR_GATED ? ffn_pair_kernel<EPI_GATED, false, false, PAIR, true> : ffn_pair_kernel<EPI_PLAIN, false, false, PAIR, true>;
     }
-    if (q.kind == PAIR_GRAD && !q.a_mn && q.b_mn)
+    if (q.kind != PAIR_PLAIN && !q.a_mn && q.b_mn)
     {
-        *bit = 2;
-        return ffn_pair_kernel<EPI_GRAD, false, true, PAIR>;
+        *bit = q.kind == PAIR_GATED ? 0 : 1;
+        return q.kind == PAIR_GATED ? ffn_pair_kernel<EPI_GATED, false, true, PAIR> : ffn_pair_kernel<EPI_GRAD, false, true, PAIR>;
     }
     if (q.kind == PAIR_PLAIN && q.a_mn == q.b_mn)
     {
-        *bit = q.a_mn ? 3 : 4;
+        *bit = q.a_mn ? 2 : 3;
         return q.a_mn ? ffn_pair_kernel<EPI_PLAIN, true, true, PAIR> : ffn_pair_kernel<EPI_PLAIN, false, false, PAIR>;
     }
     return nullptr;
@@ -799,16 +1022,31 @@ Kern pick(const PairProduct& q, int* bit)
 template <bool PAIR>
 tb200_status launch(tb200_ctx* ctx, const PairProduct& q, int splits)
 {
-    using S = Shape<PAIR>;
+    using S = Shape<PAIR>;    // (4-bit weights: the same but for the ring's division into stages)
     Params k;
     memset(&k, 0, sizeof(k));
     const bool bf16       = q.dt == TB200_BF16;
     const bool gated      = q.kind != PAIR_PLAIN;
     const uint32_t b_line = !PAIR && gated ? 64u : 128u;
     tb200_status st       = encode(ctx, &k.tmA, q.a, bf16, !q.a_mn);
-    if (st == TB200_OK)
+    for (int i = 0; q.w4 && i < (gated ? 2 : 1) && st == TB200_OK; i++)
+    {
+        st             = encode_raw(ctx, i ? &k.tmB1 : &k.tmB0, q.w4[i], q.cols, b_line);
+        k.scale[i]     = q.w4[i].scale;
+        k.scale_dt[i]  = q.w4[i].scale_dt;
+        k.zero[i]      = q.w4[i].zero;
+    }
+    if (q.w4)
+    {
+        if (!gated)
+            k.tmB1 = k.tmB0;
+        k.K       = (int)q.K;
+        k.groups  = (int)((q.K + q.group - 1) / q.group);
+        k.group32 = q.group >= q.K ? 1u << 30 : (uint32_t)q.group / 32;    // (a group that holds a whole row has any length)
+    }
+    if (st == TB200_OK && !q.w4)
         st = encode(ctx, &k.tmB0, q.b[0], bf16, !q.b_mn, b_line);
-    if (st == TB200_OK)
+    if (st == TB200_OK && !q.w4)
         st = encode(ctx, &k.tmB1, q.b[1].data ? q.b[1] : q.b[0], bf16, !q.b_mn, b_line);
     if (st != TB200_OK)
         return st;
@@ -857,7 +1095,7 @@ tb200_status launch(tb200_ctx* ctx, const PairProduct& q, int splits)
     if (st != TB200_OK)
         return st;
     cudaLaunchConfig_t cfg = {};
-    cfg.blockDim           = dim3(kThreads);
+    cfg.blockDim           = dim3(q.w4 ? Shape<PAIR, true>::kThreads : S::kThreads);
     cfg.dynamicSmemBytes   = (size_t)S::kSmem;
     cfg.stream             = ctx->stream;
     cudaLaunchAttribute attr[2];
@@ -881,35 +1119,67 @@ tb200_status launch(tb200_ctx* ctx, const PairProduct& q, int splits)
     return post_launch(ctx, q.name);
 }
 
+// How many clusters of `size` CTAs by themselves run at once
+tb200_status clusters_at_once(tb200_ctx* ctx, int which, int size, int* n)
+{
+    if (ctx->ffn_clusters[which] == 0)
+    {
+        const Kern kern       = ffn_pair_kernel<EPI_PLAIN, false, false, false>;
+        const tb200_status st = raise_smem_limit(ctx, 128 + 48 + 3, reinterpret_cast<const void*>(kern), Shape<false>::kSmem);
+        if (st != TB200_OK)
+            return st;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim            = dim3((unsigned)ctx->num_sms * size);
+        cfg.blockDim           = dim3(Shape<false>::kThreads);
+        cfg.dynamicSmemBytes   = (size_t)Shape<false>::kSmem;
+        cudaLaunchAttribute attr[1];
+        attr[0].id               = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = (unsigned)size;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cfg.attrs    = attr;
+        cfg.numAttrs = 1;
+        TB200_CUDA_CHECK(ctx, cudaOccupancyMaxActiveClusters(&ctx->ffn_clusters[which], kern, &cfg));
+        ctx->ffn_clusters[which] = std::max(1, ctx->ffn_clusters[which]);
+    }
+    *n = ctx->ffn_clusters[which];
+    return TB200_OK;
+}
+
 }    // namespace
 
 tb200_status pair_launch(tb200_ctx* ctx, const PairProduct& q)
 {
     // Pairs, or CTAs by themselves, K shared by up to eight: by their cycles.  A chunk of K takes a pair 520 and a CTA by itself 330, up to 700 when
-    // all SMs run one, since their smaller tiles move twice the bytes for a product; the last tile's epilogue shows, and so does the exchange
-    // of the shares' sums.
+    // all SMs run one, since their smaller tiles move twice the bytes for a product; with 4-bit weights, whose values pass through shared
+    // memory twice, 690 and 490.  The last tile's epilogue shows, and so does the exchange of the shares' sums.
     const bool gated     = q.kind != PAIR_PLAIN;
     const int64_t copies = (int64_t)q.NB * (q.results == 2 && !gated ? 2 : 1), chunks = (q.K + 63) / 64 * q.phases;
     auto tiles = [&](int rows, int cols) { return (int64_t)((q.rows + rows - 1) / rows) * ((q.cols + cols - 1) / cols) * copies; };
     auto waves = [&](int64_t n, int64_t at_once) { return (double)((n + at_once - 1) / at_once); };
     const int64_t large = tiles(256, gated ? 128 : 256), small = tiles(128, gated ? 64 : 128);
-    double best = waves(large, ctx->num_sms / 2) * (double)chunks * 520.0 + 4500.0;
+    double best = waves(large, ctx->num_sms / 2) * (double)chunks * (q.w4 ? 690.0 : 520.0) + 4500.0;
     int splits  = 0;
-    for (int s = 1; s <= 8; s *= 2)
+    for (int s = 1, i = 0; s <= 8; s *= 2, i++)
     {
         if (s > 1 && (chunks < 4 * s || small * s > ctx->num_sms))
             break;
-        const double chunk = std::max(330.0, 700.0 * (double)std::min<int64_t>(small * s, ctx->num_sms) / ctx->num_sms);
-        const double cost  = waves(small * s, ctx->num_sms) * (double)((chunks + s - 1) / s) * chunk + 2500.0 + (s > 1 ? 2500.0 : 0.0);
+        const double chunk = q.w4 ? 490.0 : std::max(330.0, 700.0 * (double)std::min<int64_t>(small * s, ctx->num_sms) / ctx->num_sms);
+        double cost        = waves(small, ctx->num_sms) * (double)chunks * chunk + 2500.0;
+        if (s > 1)
+        {
+            // a share does one tile; clusters of four fill 132 of 148 SMs, of eight 120 (70 x 2048 x 2048 with 4-bit weights: 18 us, 10 by fours)
+            int at_once        = 0;
+            const tb200_status st = clusters_at_once(ctx, i - 1, s, &at_once);
+            if (st != TB200_OK)
+                return st;
+            cost = waves(small, at_once) * ((double)((chunks + s - 1) / s) * chunk + 2500.0) + 2500.0;
+        }
         if (cost < best)
         {
             best   = cost;
             splits = s;
         }
     }
-    const int forced = diag_env_int("TB200_FFN_SPLITS", -1);
-    if (forced >= 0)
-        splits = forced;
     return splits ? launch<false>(ctx, q, splits) : launch<true>(ctx, q, 1);
 }
 

@@ -130,68 +130,7 @@ __global__ void __launch_bounds__(kSmallThreads) row_copies_kernel(const __grid_
     }
 }
 
-// The values of a 4-bit matrix in 16 bits, rows [W][pitch], a value rounded once.  A warp takes 1024 elements of a row, a lane four runs of eight
-// (which share a group): it reads 128 bytes and writes 512 that follow one another at a time, all of a lane's loads on their way together
-// (32 neighbouring elements a thread, whose stores lay 64 bytes apart, took 19 us for 4096 x 4096; one run at a time 15 us).
-__global__ void __launch_bounds__(kSmallThreads) w4_dense_16_kernel(const W4Mat w0, const W4Mat w1, int C, int W, int group, bool bf16, uint16_t* out0,
-                                                                    uint16_t* out1, int64_t pitch, int* status)
-{
-    const W4Mat& w      = blockIdx.y ? w1 : w0;
-    uint16_t* const out = blockIdx.y ? out1 : out0;
-    ptx::dep_launch_trigger();
-    ptx::dep_launch_wait();
-    const int pieces    = (C + 1023) / 1024;    // of a row
-    const int64_t warps = (int64_t)gridDim.x * (kSmallThreads / 32), n = (int64_t)W * pieces;
-    const bool words    = w.pitch % 4 == 0;
-    bool bad            = false;
-    for (int64_t i = (int64_t)blockIdx.x * (kSmallThreads / 32) + (threadIdx.x >> 5); i < n; i += warps)
-    {
-        const int64_t row = i / pieces;
-        const int first   = (int)(i - row * pieces) * 1024 + (int)(threadIdx.x & 31) * 8;
-        const uint8_t* const src = w.data + row * w.pitch;
-        uint32_t b[4];
-        float s[4];
-        int z[4];
-#pragma unroll
-        for (int e = 0; e < 4; e++)
-        {
-            const int c0 = min(first + 256 * e, C - 1) & ~7;    // the last run, more than once, where the row ends
-            const int g  = (int)((uint32_t)c0 / (uint32_t)group);
-            s[e]         = load_fp(w.scale, (int64_t)g * W + row, w.scale_dt);
-            z[e]         = w.zero ? (int)w.zero[(int64_t)g * W + row] : 0;
-            if (words)
-                b[e] = *reinterpret_cast<const uint32_t*>(src + c0 / 2);
-            else
-            {
-                b[e] = 0;
-#pragma unroll
-                for (int j = 0; j < 4; j++)
-                    if (c0 + 2 * j < C)
-                        b[e] |= (uint32_t)src[c0 / 2 + j] << (8 * j);
-            }
-        }
-#pragma unroll
-        for (int e = 0; e < 4; e++)
-        {
-            const int c0 = first + 256 * e;
-            if (c0 >= C)
-                break;
-            bad |= z[e] < -8 || z[e] > 7;
-            uint32_t v[4];
-#pragma unroll
-            for (int j = 0; j < 4; j++)
-            {
-                const int lo = (int)(((b[e] >> (8 * j)) & 15) ^ 8) - 8 - z[e], hi = (int)(((b[e] >> (8 * j + 4)) & 15) ^ 8) - 8 - z[e];
-                v[j]         = pack2((float)lo * s[e], (float)hi * s[e], bf16);
-            }
-            *reinterpret_cast<uint4*>(out + row * pitch + c0) = make_uint4(v[0], v[1], v[2], v[3]);
-        }
-    }
-    if (bad)
-        atomicOr(status, TB200_DEV_UNPREDICTABLE);
-}
-
-// ... in fp32, [C][W]: a thread for 32 elements of a row, neighbouring threads on neighbouring columns
+// The values of a 4-bit matrix in fp32, [C][W]: a thread for 32 elements of a row, neighbouring threads on neighbouring columns
 __global__ void __launch_bounds__(kSmallThreads) w4_dense_32_kernel(const W4Mat w, int C, int W, int group, float* out, int* status)
 {
     const int64_t runs = (C + 31) / 32, n = runs * W;
@@ -243,7 +182,7 @@ __global__ void __launch_bounds__(kSmallThreads) grad_f32_kernel(float* __restri
     {
         float value, slope;
         act_slope(act, g[i], value, slope);
-        const float dg = d[i] * u[i] * slope, du = d[i] * value;
+        const float dg = d[i] * slope * u[i], du = d[i] * value;
         g[i]           = dg;
         u[i]           = du;
         if (both)
@@ -304,21 +243,12 @@ tb200_status row_copies_launch(tb200_ctx* ctx, const RowCopies& q)
     return post_launch(ctx, "row_copies");
 }
 
-tb200_status w4_dense_launch(tb200_ctx* ctx, const W4Mat* w, int mats, int C, int W, int group, tb200_dtype dt, void* const* out, int64_t pitch)
+tb200_status w4_dense_launch(tb200_ctx* ctx, const W4Mat* w, int mats, int C, int W, int group, void* const* out)
 {
-    if (dt == TB200_FP32)
-    {
-        for (int i = 0; i < mats; i++)
-            w4_dense_32_kernel<<<small_grid(ctx, (int64_t)((C + 31) / 32) * W), kSmallThreads, 0, ctx->stream>>>(w[i], C, W, group,
-                                                                                                             reinterpret_cast<float*>(out[i]), ctx->d_status);
-        return post_launch(ctx, "w4_dense", mats);
-    }
-    const cudaError_t e = launch_overlapped(ctx, w4_dense_16_kernel, dim3((unsigned)small_grid(ctx, (int64_t)((C + 1023) / 1024) * 32 * W), (unsigned)mats), w[0],
-                                            w[mats - 1], C, W, group, dt == TB200_BF16, reinterpret_cast<uint16_t*>(out[0]),
-                                            reinterpret_cast<uint16_t*>(out[mats - 1]), pitch, ctx->d_status);
-    if (e != cudaSuccess)
-        return fail(ctx, TB200_INTERNAL, "launch of w4_dense failed: %s", cudaGetErrorString(e));
-    return post_launch(ctx, "w4_dense");
+    for (int i = 0; i < mats; i++)
+        w4_dense_32_kernel<<<small_grid(ctx, (int64_t)((C + 31) / 32) * W), kSmallThreads, 0, ctx->stream>>>(w[i], C, W, group, reinterpret_cast<float*>(out[i]),
+                                                                                                         ctx->d_status);
+    return post_launch(ctx, "w4_dense", mats);
 }
 
 tb200_status gate_f32_launch(tb200_ctx* ctx, const float* g, const float* u, float* out, int64_t n, int act)

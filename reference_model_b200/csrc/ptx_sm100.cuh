@@ -66,6 +66,17 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity)
 
 // Bounded wait: gives up after `limit_cycles` SM clock cycles and returns false.  Every wait in the
 // tensor-core kernels goes through this so that a pipeline bug ends in an error status, not a hang.
+// whether the phase is complete, without waiting
+__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity)
+{
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.b32 %0, 1, 0, p;\n\t}"
+                 : "=r"(ok)
+                 : "r"(bar), "r"(parity)
+                 : "memory");
+    return ok != 0;
+}
+
 __device__ __forceinline__ bool mbar_wait_bounded(uint32_t bar, uint32_t parity, long long limit_cycles)
 {
     if (mbar_try_wait(bar, parity))
@@ -450,6 +461,13 @@ __device__ __forceinline__ uint32_t map_to_cta(uint32_t smem_addr, uint32_t rank
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_bar)
 {
     asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+}
+
+// The same behind writes to this CTA's own shared memory that the tensor cores read next (fence_proxy_async_smem first).  Each SM's
+// read its own memory, so the order within this CTA is enough; with .cluster scope the arrival took 2000 cycles.
+__device__ __forceinline__ void mbar_arrive_cluster_release(uint32_t cluster_bar)
+{
+    asm volatile("mbarrier.arrive.release.cta.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
 }
 
 // TMA tile load into this CTA's shared memory whose completion bytes are counted on an mbarrier of either CTA of the

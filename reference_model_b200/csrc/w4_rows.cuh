@@ -25,6 +25,7 @@
 #include "ffn.h"
 #include "ffn_math.cuh"
 #include "ptx_sm100.cuh"
+#include "w4_unpack.cuh"
 
 namespace tb200
 {
@@ -81,58 +82,6 @@ __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uin
                      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-__device__ __forceinline__ uint32_t fma2_bf16(uint32_t a, uint32_t b, uint32_t c)
-{
-    uint32_t d;
-    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
-    return d;
-}
-
-__device__ __forceinline__ uint32_t fma2_f16(uint32_t a, uint32_t b, uint32_t c)
-{
-    uint32_t d;
-    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
-    return d;
-}
-
-// (w & m) ^ x in one instruction
-__device__ __forceinline__ uint32_t and_xor(uint32_t w, uint32_t m, uint32_t x)
-{
-    uint32_t d;
-    asm("lop3.b32 %0, %1, %2, %3, 0x6A;" : "=r"(d) : "r"(w), "r"(m), "r"(x));
-    return d;
-}
-
-// Eight elements to four pairs (0,4), (1,5), (2,6), (3,7), minus their zero point; `base` holds -(136 + z) twice (fp16: -(1032 + z)).
-// One multiply-add by 1 takes it off (a bf16 subtraction of pairs is no instruction of its own: ncu counted five in its place).
-// fp16 reads every second pair four bits higher, as 1024 + 16 (8 + q), and scales by 1/16 in the same multiply-add: one shift in place of three.
-template <bool BF16>
-__device__ __forceinline__ void unpack8(uint32_t w, uint32_t base, uint32_t (&p)[4])
-{
-    if (BF16)
-    {
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-            p[i] = fma2_bf16(and_xor(w >> (4 * i), 0x000F000Fu, 0x43084308u), 0x3F803F80u, base);
-    }
-    else
-    {
-        const uint32_t high = fma2_f16(base, 0x3C003C00u, 0x63806380u);    // 960 - (1032 + z) = -(72 + z)
-        const uint32_t v    = w >> 8;
-        p[0]                = fma2_f16(and_xor(w, 0x000F000Fu, 0x64086408u), 0x3C003C00u, base);
-        p[1]                = fma2_f16(and_xor(w, 0x00F000F0u, 0x64806480u), 0x2C002C00u, high);
-        p[2]                = fma2_f16(and_xor(v, 0x000F000Fu, 0x64086408u), 0x3C003C00u, base);
-        p[3]                = fma2_f16(and_xor(v, 0x00F000F0u, 0x64806480u), 0x2C002C00u, high);
-    }
-}
-
-__device__ __forceinline__ uint4 lds128(uint32_t addr)
-{
-    uint4 v;
-    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
-    return v;
-}
-
 __device__ __forceinline__ uint32_t lds32(uint32_t addr)
 {
     uint32_t v;
@@ -184,7 +133,7 @@ __device__ __forceinline__ void run_scales(const RowsRun& r, int i, float (&scal
         int z = 0;
         if (r.has_zero)
             asm volatile("ld.shared.s8 %0, [%1];" : "=r"(z) : "r"(zat + (uint32_t)(q * 8)));
-        base[q] = (BF16 ? 0xC308C308u : 0xE408E408u) + (uint32_t)z * 0x10001u;
+        base[q] = unpack_base<BF16>(z);
     }
 }
 
@@ -332,7 +281,7 @@ __global__ void __launch_bounds__(kRowsThreads, rows_blocks_sm(NT)) w4_rows_kern
                         // a box behind the last element reads as zeros
                         for (int r = 0; r < units; r++)
                         {
-                            const int64_t at = min((int64_t)(group + r) * p.W + tile * kPer, (int64_t)0x7ffffff0);
+                            const int64_t at = min((int64_t)(group + r) * p.W + tile * kPer, (int64_t)0x7ffffff0);    // (may pass the last group)
                             ptx::tma_load_2d(sW + (uint32_t)(off + r * step), map, full, (int)(at & ~(int64_t)(flat - 1)), 0);
                         }
                     };
@@ -547,7 +496,6 @@ __global__ void __launch_bounds__(kRowsThreads, rows_blocks_sm(NT)) w4_rows_kern
         const bool share_first = n_first < S, share_last = tile_last > tile0 && n_last < S;
         if (tid == 0)
         {
-            // (the block's sums, which the barrier above has put before this, are published with the addition)
             __threadfence();    // the block's sums, which the barrier above has put before this
             const int first = share_first ? atomicAdd(p.counts + tile0, n_first) : 0, last = share_last ? atomicAdd(p.counts + tile_last, n_last) : 0;
             completes[0]    = share_first && first + n_first == S;

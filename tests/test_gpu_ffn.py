@@ -409,6 +409,32 @@ def test_backward_against_differences(ctx, act):
     assert abs(slope - want) <= (0.05 if act == "RELU" else 0.02) * size
 
 
+@pytest.mark.parametrize("policy", (0, 1))
+@pytest.mark.parametrize("dtype", ("bf16", "fp32"))
+@pytest.mark.parametrize("act", ("GELU_TANH", "RELU"))
+def test_backward_does_not_overflow_beside_a_zero(ctx, act, dtype, policy):
+    """Finite gradients stay finite where a square or a partial product on the way to them passes the type's largest number.  Powers
+    of two: every product and sum is exact."""
+    p = 2.0
+    up, d1 = (p ** -33, 1.0) if act == "GELU_TANH" else (p ** 60, p ** 50)
+    a, bg = torch.tensor([[[p ** 33]]]), torch.tensor([[[p ** 33, -p ** 33]]])
+    bu, d = torch.tensor([[[up, up]]]), torch.tensor([[[1.0, d1]]])
+    # G = (2^66, -2^66): values (G, 0), slopes (1, 0)
+    dg, du = p ** 33 * up, p ** 66
+    want = (dg * p ** 33 + du * up,), (p ** 33 * dg, 0.0), (p ** 33 * du, 0.0)
+    ops  = [put(ctx, t.to(TT[dtype])) for t in (a, bg, bu, d)]
+    outs = [blank(ctx, dtype, s) for s in ((1, 1, 1), (1, 1, 2), (1, 1, 2))]
+    old  = ctx.set_kernel_policy(policy)
+    try:
+        ctx.matmul_gated_backward(*ops, *outs, activation=act)
+    finally:
+        ctx.set_kernel_policy(old)
+    for t, w in zip(outs, want):
+        assert get(t).double().flatten().tolist() == list(w)
+    for t in ops + outs:
+        t.free()
+
+
 def test_gradients_that_are_not_asked_for(ctx):
     a, bg, bu, d = gated_inputs(1, 1, 70, 136, 72, "bf16")
     ts = [put(ctx, t) for t in (a, bg, bu, d)]
