@@ -75,8 +75,10 @@ void pad(RowCopies* copies, const void* data, const Matrix& m)
             return st__;                    \
     } while (0)
 
-// Rows up to which the kernels that stream the weights past a few rows serve.
-constexpr int64_t kFewRows = 64;
+// Rows up to which the kernels that stream the weights past a few rows serve; with more, 128-row tiles of the tensor cores are quicker for all their
+// padding (4-bit 4096 x 4096: 24 rows 11.7 against 13.0 us, 33 rows 14.6 against 13.1; 16-bit gated 2048 x 8192: 32 rows 14.3 against
+// 16.8, 33 rows 25.6 against 16.9).  fp32 rows against 4-bit weights, whose alternative is a pass over fp32 values: 64 of their parts.
+constexpr int64_t kFewRows = 32, kFewParts = 64;
 
 // 16-bit gated product on the tensor cores
 tb200_status gated_pair(tb200_ctx* ctx, const GatedProblem& q)
@@ -298,7 +300,7 @@ tb200_status w4_launch(tb200_ctx* ctx, const W4Problem& q)
     const int parts     = f32 ? 3 : 1;
     const int64_t xpitch = round_up(q.C, 8);
     const int64_t wpitch = round_up((q.C + 1) / 2, 16);
-    const bool few       = q.M * parts <= kFewRows;
+    const bool few       = f32 ? q.M * parts <= kFewParts : q.M <= kFewRows;
     const bool copy_x    = !f32 && q.C % 8 != 0;
     const int64_t n      = q.M * q.W;
     Carver c;

@@ -1,4 +1,4 @@
-// Gated product with up to 64 rows (a decoder's tokens), 16-bit weights: each weight meets only those rows, so the operator reads both
+// Gated product with up to 32 rows (a decoder's tokens), 16-bit weights: each weight meets only those rows, so the operator reads both
 // matrices once and nothing else counts.  Warp-level matrix instructions (m16n8k16) take sixteen output columns as their rows
 // and eight rows of `a` as their columns; a 256-row tile of the CTA-pair kernel would be padding.
 //
@@ -286,7 +286,7 @@ typedef void (*FewKern)(const FewParams);
 template <bool BF16>
 FewKern pick(int nt)
 {
-    return nt == 1 ? gated_rows_kernel<BF16, 1> : nt == 2 ? gated_rows_kernel<BF16, 2> : nt == 4 ? gated_rows_kernel<BF16, 4> : gated_rows_kernel<BF16, 8>;
+    return nt == 1 ? gated_rows_kernel<BF16, 1> : nt == 2 ? gated_rows_kernel<BF16, 2> : gated_rows_kernel<BF16, 4>;
 }
 
 }    // namespace
@@ -296,7 +296,7 @@ tb200_status gated_rows_launch(tb200_ctx* ctx, const PairProduct& q)
     FewParams p;
     memset(&p, 0, sizeof(p));
     const bool bf16 = q.dt == TB200_BF16;
-    const int nt    = q.rows <= 8 ? 1 : q.rows <= 16 ? 2 : q.rows <= 32 ? 4 : 8;
+    const int nt    = q.rows <= 8 ? 1 : q.rows <= 16 ? 2 : 4;
     tb200_status st = encode3d(ctx, &p.tmG, q.b[0], bf16, 64);
     if (st == TB200_OK)
         st = encode3d(ctx, &p.tmU, q.b[1], bf16, 64);
@@ -319,7 +319,7 @@ tb200_status gated_rows_launch(tb200_ctx* ctx, const PairProduct& q)
     const size_t red  = (size_t)8 * nt * kFewRedLd * sizeof(float);
     const size_t smem = std::max((size_t)p.num_stages * p.stage_bytes, red) + 1024;
     const FewKern kern = bf16 ? pick<true>(nt) : pick<false>(nt);
-    st = raise_smem_limit(ctx, 168 + (nt == 8 ? 3 : nt / 2) * 2 + (bf16 ? 1 : 0), reinterpret_cast<const void*>(kern), (int)smem);
+    st = raise_smem_limit(ctx, 168 + nt / 2 * 2 + (bf16 ? 1 : 0), reinterpret_cast<const void*>(kern), (int)smem);
     if (st != TB200_OK)
         return st;
     cudaLaunchConfig_t cfg = {};

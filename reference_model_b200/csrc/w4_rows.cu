@@ -76,7 +76,7 @@ size_t w4_rows_partial_bytes(const tb200_ctx* ctx, int64_t xrows)
 }
 
 // x: the rows in 16 bits (bf16 parts of fp32 rows), `x_pitch` elements apart, 16-byte aligned; the weights' pitch is a multiple of 16;
-// at most 64 of them.  partial: w4_rows_partial_bytes.
+// at most 32 of them (64 of the parts).  partial: w4_rows_partial_bytes.
 tb200_status w4_rows_launch(tb200_ctx* ctx, const W4Problem& q, const void* x, int64_t x_pitch, int parts, bool bf16, float* partial)
 {
     RowsParams p;
@@ -156,6 +156,8 @@ tb200_status w4_rows_launch(tb200_ctx* ctx, const W4Problem& q, const void* x, i
     const bool flat     = p.s_flat[0] || p.z_flat[0] || p.s_flat[1] || p.z_flat[1];
     const RowsKern kern = bf16 ? w4_rows_kernel_bf16(nt, q.mats, flat) : w4_rows_kernel_f16(nt, q.mats, flat);
     const int size_id   = nt <= 4 ? nt - 1 : nt / 2 + 1;
+    if (!kern)
+        return fail(ctx, TB200_INTERNAL, "no kernel for %d rows against 4-bit weights", xrows);
     st = raise_smem_limit(ctx, 192 + size_id * 8 + (flat ? 4 : 0) + (bf16 ? 2 : 0) + q.mats - 1, reinterpret_cast<const void*>(kern), (int)smem);
     if (st != TB200_OK)
         return st;

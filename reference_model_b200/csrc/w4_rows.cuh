@@ -1,4 +1,4 @@
-// Products with 4-bit weights, up to 64 rows: the weights are read once, straight from their bytes, and multiplied on the warp-level
+// Products with 4-bit weights, up to 32 rows (64 of fp32's parts): the weights are read once, straight from their bytes, and multiplied on the warp-level
 // matrix instruction (m16n8k16) with the output's columns as its sixteen rows and eight rows of `a` as its columns.  A 128-row
 // tensor-core tile would be padding, and CUDA cores cannot keep up: at the memory's rate an SM receives 46 weights a clock, which
 // leaves 2.8 lane instructions for each.
@@ -599,18 +599,22 @@ __global__ void __launch_bounds__(kRowsThreads, rows_blocks_sm(NT)) w4_rows_kern
 
 typedef void (*RowsKern)(const RowsParams);
 
+// (more than 32 rows are fp32's parts, in bf16)
 template <bool BF16, int MATS, bool FLAT>
 RowsKern pick(int nt)
 {
-    switch (nt)
+    if constexpr (BF16)
     {
-        case 1: return w4_rows_kernel<BF16, 1, MATS, FLAT>;
-        case 2: return w4_rows_kernel<BF16, 2, MATS, FLAT>;
-        case 3: return w4_rows_kernel<BF16, 3, MATS, FLAT>;
-        case 4: return w4_rows_kernel<BF16, 4, MATS, FLAT>;
-        case 6: return w4_rows_kernel<BF16, 6, MATS, FLAT>;
-        default: return w4_rows_kernel<BF16, 8, MATS, FLAT>;
+        if (nt == 6)
+            return w4_rows_kernel<BF16, 6, MATS, FLAT>;
+        if (nt == 8)
+            return w4_rows_kernel<BF16, 8, MATS, FLAT>;
     }
+    return nt == 1   ? w4_rows_kernel<BF16, 1, MATS, FLAT>
+           : nt == 2 ? w4_rows_kernel<BF16, 2, MATS, FLAT>
+           : nt == 3 ? w4_rows_kernel<BF16, 3, MATS, FLAT>
+           : nt == 4 ? w4_rows_kernel<BF16, 4, MATS, FLAT>
+                     : nullptr;
 }
 
 // w4_rows_f16.cu, w4_rows_bf16.cu: the kernel for `nt` tiles of eight rows

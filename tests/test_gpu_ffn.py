@@ -201,6 +201,51 @@ def check_gated(got, G, U, eg, eu, act, out):
     close(got, f * U, ef * U.abs() + f.abs() * eu + ef * eu + (f * U).abs() * 2.0 ** -23, out)
 
 
+@pytest.mark.parametrize("group", (32, 96, 197))
+@pytest.mark.parametrize("scales", ("fp16", "bf16"))
+@pytest.mark.parametrize("dtype", ("fp16", "bf16"))
+@pytest.mark.parametrize("h,w", ((70, 70), (700, 2060)))
+def test_w4_values_are_rounded_once(ctx, h, w, dtype, scales, group):
+    """More than 32 rows multiply the weights' values, rounded once to a's type (a whole number of at most 15 times a 16-bit scale is exact
+    in fp32).  What lies behind a row's last element counts for nothing; a scale that is not finite reaches its own column alone."""
+    c = 197
+    a = rand(11, dtype, 1.0, 1, h, c)
+    m = Four(ctx, 12, c, w, group, True, True, scales)
+    ta, to = put(ctx, a), blank(ctx, "fp32", (1, h, w))
+    ctx.matmul_w4(ta, m.op, to)
+    assert ctx.last_kernel() == "matmul_w4_pair"
+    values = m.dense.to(TT[dtype]).double()
+    got, a64 = get(to), a.double()
+    close(got, a64 @ values, acc(c, dtype) * (a64.abs() @ values.abs()), "fp32")
+    s = get(m.op.scale)
+    s[-1, 3] = math.inf
+    m.op.scale.upload(s.view(torch.uint16).numpy() if scales == "bf16" else s.numpy())
+    ctx.matmul_w4(ta, m.op, to)
+    again = get(to)
+    assert not torch.isfinite(again[..., 3]).any()
+    again[..., 3] = got[..., 3]
+    assert torch.equal(again, got)
+    for t in (ta, to):
+        t.free()
+    m.free()
+
+
+@pytest.mark.parametrize("rows", (15, 16, 21))
+def test_w4_parts_of_fp32_rows(ctx, rows):
+    """45 to 63 bf16 parts.  fp32 sums of exact products: as far off as 16-bit operands' (the parts' products are exact too)."""
+    c, w = 1001, 150
+    a = rand(13, "fp32", 1.0, 1, rows, c)
+    m = Four(ctx, 14, c, w, 64, True, True, "fp32")
+    ta, to = put(ctx, a), blank(ctx, "fp32", (1, rows, w))
+    ctx.matmul_w4(ta, m.op, to)
+    assert ctx.last_kernel() == "matmul_w4_rows"
+    a64 = a.double()
+    close(get(to), a64 @ m.dense, acc(3 * c, "fp16") * (a64.abs() @ m.dense.abs()), "fp32")
+    for t in (ta, to):
+        t.free()
+    m.free()
+
+
 def test_w4_extreme_values(ctx):
     """Lowest and highest elements, zero points at both ends, scales of both signs and zero."""
     c, w = 256, 64
@@ -649,23 +694,26 @@ def forms(ctx):
                      [dG @ bg.transpose(1, 2) + dU @ bu.transpose(1, 2), wg, wu]))
 
     gated("few rows, K over clusters", "gated_rows_f16", 1, 1, 3, 4000, 200)
-    gated("few rows, many columns", "gated_rows_f16", 2, 2, 40, 264, 12000)
+    gated("few rows, many columns", "gated_rows_f16", 2, 2, 30, 264, 12000)
     gated("pairs", "gated_pair_f16", 1, 1, 1500, 520, 2000)
     gated("single, K over clusters", "gated_pair_f16", 1, 1, 100, 4000, 72)
     gated("single", "gated_pair_f16", 3, 3, 150, 100, 300)
     four("few rows", "matmul_w4_rows", 1, 9000, 700, False)
     four("few rows, gated", "gated_w4_rows", 20, 3000, 333, True)
-    four("48 rows", "matmul_w4_rows", 45, 5000, 129, False)
+    four("30 rows", "matmul_w4_rows", 30, 5000, 129, False)
     four("many rows", "matmul_w4_pair", 200, 1000, 300, False)
     four("many rows, gated", "gated_w4_pair", 90, 2000, 200, True)
+    four("many rows, K over clusters", "matmul_w4_pair", 100, 4000, 300, False)
+    four("many rows, pairs", "matmul_w4_pair", 600, 700, 4100, False)
+    four("many rows, gated pairs", "gated_w4_pair", 700, 520, 2100, True)
     backward("small", "gated_backward_pair_f16", 2, 2, 130, 72, 200)
     backward("long K", "gated_backward_pair_f16", 1, 1, 2600, 64, 40)
     backward("large", "gated_backward_pair_f16", 1, 1, 700, 2100, 1290)
     return made
 
 
-FORMS = ["few rows, K over clusters", "few rows, many columns", "pairs", "single, K over clusters", "single", "few rows", "few rows, gated", "48 rows",
-         "many rows", "many rows, gated", "small", "long K", "large"]
+FORMS = ["few rows, K over clusters", "few rows, many columns", "pairs", "single, K over clusters", "single", "few rows", "few rows, gated", "30 rows",
+         "many rows", "many rows, gated", "many rows, K over clusters", "many rows, pairs", "many rows, gated pairs", "small", "long K", "large"]
 
 
 @pytest.fixture(scope="module")
