@@ -209,6 +209,7 @@ tb200_status gated_backward_pair(tb200_ctx* ctx, const GatedProblem& q)
             k.phases  = 1;
             k.NB      = q.NB;
             k.results = q.dgate && q.dup ? 2 : 1;
+            k.beside  = q.da != nullptr;
             if (!q.dgate)
                 k.b[0].data = dg + half;
             k.b[0].batches = (int64_t)q.NB * k.results;

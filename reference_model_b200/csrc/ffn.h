@@ -90,6 +90,7 @@ struct PairProduct
     int64_t ld;        // elements from one result row to the next
     const W4Mat* w4;   // in b's place: 4-bit matrices, rows a multiple of 16 bytes apart (PAIR_PLAIN and PAIR_GATED, NB and phases 1)
     int group;
+    bool beside;       // reads nothing that the launch of this kind directly before it writes: the two may run side by side
     const char* name;
 };
 tb200_status pair_launch(tb200_ctx* ctx, const PairProduct& q);

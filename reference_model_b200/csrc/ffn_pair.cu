@@ -67,6 +67,7 @@ struct Params
     int chunks, phases;    // K chunks of a phase
     int splits;            // CTAs of a cluster that share a tile's K (CTAs by themselves only)
     int NB;                // batches of A's and B's own
+    int beside;
     int act, bf16;
     tb200_dtype out_dt;
     uint32_t idesc;
@@ -475,7 +476,9 @@ __global__ void __launch_bounds__((Shape<PAIR, W4>::kThreads), 1) ffn_pair_kerne
         __syncthreads();
     // Everything a kernel before this one may have written is read behind this wait, and nothing is written before it.  Tensor memory
     // is taken behind it too, and the next kernel let in only then: neither kernel can keep the other from columns it waits for.
-    ptx::dep_launch_wait();
+    // A product beside the one before it reads what came before both: that one let this in behind its own wait, so it is there.
+    if (!p.beside)
+        ptx::dep_launch_wait();
     uint32_t tmem_base = 0;
     if (warp != 0)
     {
@@ -944,6 +947,9 @@ __global__ void __launch_bounds__((Shape<PAIR, W4>::kThreads), 1) ffn_pair_kerne
         else
             ptx::tmem_dealloc(tmem_base, S::kTmemCols);
     }
+    // whoever waits for this kernel waits for the one before it too
+    if (p.beside)
+        ptx::dep_launch_wait();
 }
 
 typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
@@ -1056,6 +1062,7 @@ tb200_status launch(tb200_ctx* ctx, const PairProduct& q, int splits)
     k.tiles_m           = (q.rows + S::kRows - 1) / S::kRows;
     k.tiles_n           = (q.cols + step_n - 1) / step_n;
     k.NB                = q.NB;
+    k.beside            = q.beside ? 1 : 0;
     const int64_t tiles = (int64_t)k.tiles_m * k.tiles_n * q.NB * (q.results == 2 && !gated ? 2 : 1);
     if (tiles > (1 << 30))
         return fail(ctx, TB200_ERROR, "a feed-forward product of %lld tiles is too large", (long long)tiles);
