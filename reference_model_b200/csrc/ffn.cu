@@ -268,17 +268,21 @@ tb200_status gated_backward_f32(tb200_ctx* ctx, const GatedProblem& q)
         }
     }
     const float *a = reinterpret_cast<const float*>(q.a), *gate = reinterpret_cast<const float*>(q.gate), *up = reinterpret_cast<const float*>(q.up);
+    Transposes t;
+    if (q.da)
+    {
+        t.add(gate, bt, q.NB, q.C, q.W, 2 * weights);
+        t.add(up, bt + weights, q.NB, q.C, q.W, 2 * weights);
+    }
+    if (weights_too)
+        t.add(a, at, q.NB, q.H, q.C, q.H * q.C);
+    TB200_TRY(transposes_f32_launch(ctx, t));
     TB200_TRY(projections_f32(ctx, q, g));
     TB200_TRY(grad_f32_launch(ctx, g, u, reinterpret_cast<const float*>(q.dout), q.da ? both : nullptr, rows, q.W, q.act));
     if (q.da)
-    {
-        TB200_TRY(transpose_f32_launch(ctx, gate, bt, q.NB, q.C, q.W, 2 * weights));
-        TB200_TRY(transpose_f32_launch(ctx, up, bt + weights, q.NB, q.C, q.W, 2 * weights));
         TB200_TRY(sgemm_f32_launch(ctx, both, bt, reinterpret_cast<float*>(q.da), q.NB, (int)q.H, 2 * q.W, q.C));
-    }
     if (weights_too)
     {
-        TB200_TRY(transpose_f32_launch(ctx, a, at, q.NB, q.H, q.C, q.H * q.C));
         float *const dgate = reinterpret_cast<float*>(q.dgate), *const dup = reinterpret_cast<float*>(q.dup);
         if (dgate && dup && q.NB == 1)
             TB200_TRY(sgemm_f32_two_launch(ctx, at, g, u, dgate, dup, q.C, (int)q.H, q.W));

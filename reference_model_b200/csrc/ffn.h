@@ -128,7 +128,20 @@ tb200_status w4_dense_launch(tb200_ctx* ctx, const W4Mat* w, int mats, int C, in
 tb200_status gate_f32_launch(tb200_ctx* ctx, const float* g, const float* u, float* out, int64_t n, int act);
 // g and u hold dG and dU afterwards, `both` (or null) the two side by side
 tb200_status grad_f32_launch(tb200_ctx* ctx, float* g, float* u, const float* d, float* both, int64_t rows, int W, int act);
-// [batches][R][C] to [batches][C][R], results `out_batch` elements apart
-tb200_status transpose_f32_launch(tb200_ctx* ctx, const float* in, float* out, int64_t batches, int64_t R, int64_t C, int64_t out_batch);
+// [batches][R][C] to [batches][C][R], results `out_batch` elements apart; up to three in a launch
+struct Transpose
+{
+    const float* in;
+    float* out;
+    int64_t R, C, out_batch;
+};
+struct Transposes
+{
+    Transpose job[3];
+    int64_t tiles[3];    // up to and with each
+    int n = 0;
+    void add(const float* in, float* out, int64_t batches, int64_t R, int64_t C, int64_t out_batch);
+};
+tb200_status transposes_f32_launch(tb200_ctx* ctx, const Transposes& q);
 }    // namespace ffn
 }    // namespace tb200

@@ -166,50 +166,96 @@ __global__ void __launch_bounds__(kSmallThreads) w4_dense_32_kernel(const W4Mat 
         atomicOr(status, TB200_DEV_UNPREDICTABLE);
 }
 
-// fp32 gated product behind its two projections
-__global__ void __launch_bounds__(kSmallThreads) gate_f32_kernel(const float* __restrict__ g, const float* __restrict__ u, float* __restrict__ out, int64_t n, int act)
+// fp32 gated product behind its two projections, four elements a thread where `n` allows
+__global__ void __launch_bounds__(kSmallThreads) gate_f32_kernel(const float* g, const float* u, float* out, int64_t n, int act)
 {
-    for (int64_t i = (int64_t)blockIdx.x * kSmallThreads + threadIdx.x; i < n; i += (int64_t)gridDim.x * kSmallThreads)
+    ptx::dep_launch_trigger();
+    ptx::dep_launch_wait();
+    const int64_t first = (int64_t)blockIdx.x * kSmallThreads + threadIdx.x, step = (int64_t)gridDim.x * kSmallThreads;
+    if (n % 4 == 0)
+    {
+        for (int64_t i = first; i < n / 4; i += step)
+        {
+            const float4 x = reinterpret_cast<const float4*>(g)[i], y = reinterpret_cast<const float4*>(u)[i];
+            reinterpret_cast<float4*>(out)[i] =
+                make_float4(act_value(act, x.x) * y.x, act_value(act, x.y) * y.y, act_value(act, x.z) * y.z, act_value(act, x.w) * y.w);
+        }
+        return;
+    }
+    for (int64_t i = first; i < n; i += step)
         out[i] = act_value(act, g[i]) * u[i];
 }
 
 // ... and its gradients: dG and dU in place of G and U, and side by side [rows][2 W] for the product with both matrices (where asked for)
-__global__ void __launch_bounds__(kSmallThreads) grad_f32_kernel(float* __restrict__ g, float* __restrict__ u, const float* __restrict__ d, float* __restrict__ both,
-                                                                 int64_t rows, int W, int act)
+__global__ void __launch_bounds__(kSmallThreads) grad_f32_kernel(float* g, float* u, const float* d, float* both, int64_t rows, int W, int act)
 {
-    const int64_t n = rows * W;
-    for (int64_t i = (int64_t)blockIdx.x * kSmallThreads + threadIdx.x; i < n; i += (int64_t)gridDim.x * kSmallThreads)
-    {
+    ptx::dep_launch_trigger();
+    ptx::dep_launch_wait();
+    const int64_t n = rows * W, first = (int64_t)blockIdx.x * kSmallThreads + threadIdx.x, step = (int64_t)gridDim.x * kSmallThreads;
+    auto gradients = [&](float G, float U, float D, float& dg, float& du) {
         float value, slope;
-        act_slope(act, g[i], value, slope);
-        const float dg = d[i] * slope * u[i], du = d[i] * value;
-        g[i]           = dg;
-        u[i]           = du;
+        act_slope(act, G, value, slope);
+        dg = D * slope * U;
+        du = D * value;
+    };
+    if (W % 4 == 0)
+    {
+        for (int64_t i = first; i < n / 4; i += step)
+        {
+            const float4 x = reinterpret_cast<const float4*>(g)[i], y = reinterpret_cast<const float4*>(u)[i], z = reinterpret_cast<const float4*>(d)[i];
+            float4 dg, du;
+            gradients(x.x, y.x, z.x, dg.x, du.x);
+            gradients(x.y, y.y, z.y, dg.y, du.y);
+            gradients(x.z, y.z, z.z, dg.z, du.z);
+            gradients(x.w, y.w, z.w, dg.w, du.w);
+            reinterpret_cast<float4*>(g)[i] = dg;
+            reinterpret_cast<float4*>(u)[i] = du;
+            if (both)
+            {
+                const int64_t r = i / (W / 4), c = i - r * (W / 4);
+                reinterpret_cast<float4*>(both)[r * 2 * (W / 4) + c]         = dg;
+                reinterpret_cast<float4*>(both)[(r * 2 + 1) * (W / 4) + c] = du;
+            }
+        }
+        return;
+    }
+    for (int64_t i = first; i < n; i += step)
+    {
+        float dg, du;
+        gradients(g[i], u[i], d[i], dg, du);
+        g[i] = dg;
+        u[i] = du;
         if (both)
         {
-            const int64_t r          = i / W, c = i - r * W;
-            both[r * 2 * W + c]      = dg;
-            both[r * 2 * W + W + c]  = du;
+            const int64_t r         = i / W, c = i - r * W;
+            both[r * 2 * W + c]     = dg;
+            both[r * 2 * W + W + c] = du;
         }
     }
 }
 
-// [batches][R][C] fp32 to [batches][C][R], tiles of 32 x 32 through shared memory; batches `out_batch` elements apart in the result
-__global__ void __launch_bounds__(256) transpose_f32_kernel(const float* __restrict__ in, float* __restrict__ out, int64_t R, int64_t C, int64_t out_batch,
-                                                            int64_t tiles_r, int64_t tiles_c, int64_t num_tiles)
+// [batches][R][C] fp32 to [batches][C][R], tiles of 32 x 32 through shared memory, all transposes of a call in one launch
+__global__ void __launch_bounds__(256) transposes_f32_kernel(const __grid_constant__ Transposes q)
 {
     __shared__ float t[32][33];
+    ptx::dep_launch_trigger();
+    ptx::dep_launch_wait();
     const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
-    for (int64_t i = blockIdx.x; i < num_tiles; i += gridDim.x)
+    for (int64_t i = blockIdx.x; i < q.tiles[q.n - 1]; i += gridDim.x)
     {
-        const int64_t b = i / (tiles_r * tiles_c), k = i - b * tiles_r * tiles_c, r0 = k / tiles_c * 32, c0 = k % tiles_c * 32;
-        for (int j = y; j < 32; j += 8)
-            if (r0 + j < R && c0 + x < C)
-                t[j][x] = in[(b * R + r0 + j) * C + c0 + x];
+        int job = 0;
+        while (i >= q.tiles[job])
+            job++;
+        const Transpose& j   = q.job[job];
+        const int64_t tile   = i - (job ? q.tiles[job - 1] : 0), tiles_c = (j.C + 31) / 32, per = (j.R + 31) / 32 * tiles_c;
+        const int64_t b = tile / per, k = tile - b * per, r0 = k / tiles_c * 32, c0 = k % tiles_c * 32;
+        for (int e = y; e < 32; e += 8)
+            if (r0 + e < j.R && c0 + x < j.C)
+                t[e][x] = j.in[(b * j.R + r0 + e) * j.C + c0 + x];
         __syncthreads();
-        for (int j = y; j < 32; j += 8)
-            if (c0 + j < C && r0 + x < R)
-                out[b * out_batch + (c0 + j) * R + r0 + x] = t[x][j];
+        for (int e = y; e < 32; e += 8)
+            if (c0 + e < j.C && r0 + x < j.R)
+                j.out[b * j.out_batch + (c0 + e) * j.R + r0 + x] = t[x][e];
         __syncthreads();
     }
 }
@@ -253,21 +299,33 @@ tb200_status w4_dense_launch(tb200_ctx* ctx, const W4Mat* w, int mats, int C, in
 
 tb200_status gate_f32_launch(tb200_ctx* ctx, const float* g, const float* u, float* out, int64_t n, int act)
 {
-    gate_f32_kernel<<<small_grid(ctx, n), kSmallThreads, 0, ctx->stream>>>(g, u, out, n, act);
+    const cudaError_t e = launch_overlapped(ctx, gate_f32_kernel, dim3((unsigned)small_grid(ctx, (n + 3) / 4)), g, u, out, n, act);
+    if (e != cudaSuccess)
+        return fail(ctx, TB200_INTERNAL, "launch of gate_f32 failed: %s", cudaGetErrorString(e));
     return post_launch(ctx, "gate_f32");
 }
 
 tb200_status grad_f32_launch(tb200_ctx* ctx, float* g, float* u, const float* d, float* both, int64_t rows, int W, int act)
 {
-    grad_f32_kernel<<<small_grid(ctx, rows * W), kSmallThreads, 0, ctx->stream>>>(g, u, d, both, rows, W, act);
+    const cudaError_t e = launch_overlapped(ctx, grad_f32_kernel, dim3((unsigned)small_grid(ctx, (rows * W + 3) / 4)), g, u, d, both, rows, W, act);
+    if (e != cudaSuccess)
+        return fail(ctx, TB200_INTERNAL, "launch of grad_f32 failed: %s", cudaGetErrorString(e));
     return post_launch(ctx, "grad_f32");
 }
 
-tb200_status transpose_f32_launch(tb200_ctx* ctx, const float* in, float* out, int64_t batches, int64_t R, int64_t C, int64_t out_batch)
+void Transposes::add(const float* in, float* out, int64_t batches, int64_t R, int64_t C, int64_t out_batch)
 {
-    const int64_t tr = (R + 31) / 32, tc = (C + 31) / 32, n = batches * tr * tc;
-    transpose_f32_kernel<<<(unsigned)std::min<int64_t>(n, (int64_t)ctx->num_sms * 8), 256, 0, ctx->stream>>>(in, out, R, C, out_batch, tr, tc, n);
-    return post_launch(ctx, "transpose_f32");
+    job[n]   = { in, out, R, C, out_batch };
+    tiles[n] = (n ? tiles[n - 1] : 0) + batches * ((R + 31) / 32) * ((C + 31) / 32);
+    n++;
+}
+
+tb200_status transposes_f32_launch(tb200_ctx* ctx, const Transposes& q)
+{
+    const cudaError_t e = launch_overlapped(ctx, transposes_f32_kernel, dim3((unsigned)std::min<int64_t>(q.tiles[q.n - 1], (int64_t)ctx->num_sms * 8)), q);
+    if (e != cudaSuccess)
+        return fail(ctx, TB200_INTERNAL, "launch of transposes_f32 failed: %s", cudaGetErrorString(e));
+    return post_launch(ctx, "transposes_f32");
 }
 
 }    // namespace ffn
