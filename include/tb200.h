@@ -319,7 +319,10 @@ extern "C"
      * groups = ceil(C / group); zero INT8 [groups, W] with values -8 .. 7 (another value is a failed REQUIRE:
      * TB200_UNPREDICTABLE at the next sync), or NULL for none.  group: a multiple of 32, or at least C (one scale per
      * column).  What a row holds behind its last element is not used.  Rows whose pitch is a multiple of 16 bytes are
-     * read as they are; others are copied into scratch first. */
+     * read as they are; others are copied into scratch first.
+     * Up to 32 rows of a (21 in FP32; N H of them) multiply element - zero exactly and scale the fp32 sum of a group.  More rows
+     * multiply the values scale * (element - zero), rounded once to a's type: in FP16 they overflow from 65520 on and lose
+     * places below 2^-14. */
     typedef struct tb200_w4
     {
         const tb200_tensor* data;

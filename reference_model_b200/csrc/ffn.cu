@@ -83,13 +83,14 @@ constexpr int64_t kFewRows = 32, kFewParts = 64;
 // 16-bit gated product on the tensor cores
 tb200_status gated_pair(tb200_ctx* ctx, const GatedProblem& q)
 {
+    const bool few = q.H <= kFewRows && q.NB <= 65535;    // (that kernel takes the matrices as they lie)
     Carver size, at;
     for (int pass = 0; pass < 2; pass++)
     {
         Carver& c     = pass ? at : size;
         void* const a = c.take(pad_bytes(q.C, q.NB * q.H));
-        void* const g = c.take(pad_bytes(q.W, (int64_t)q.NB * q.C));
-        void* const u = c.take(pad_bytes(q.W, (int64_t)q.NB * q.C));
+        void* const g = c.take(few ? 0 : pad_bytes(q.W, (int64_t)q.NB * q.C));
+        void* const u = c.take(few ? 0 : pad_bytes(q.W, (int64_t)q.NB * q.C));
         if (!pass)
         {
             if (size.used)
@@ -105,6 +106,11 @@ tb200_status gated_pair(tb200_ctx* ctx, const GatedProblem& q)
         k.a    = operand(q.a, q.C, q.H, q.NB, a);
         k.b[0] = operand(q.gate, q.W, q.C, q.NB, g);
         k.b[1] = operand(q.up, q.W, q.C, q.NB, u);
+        if (few)
+        {
+            k.b[0] = { q.gate, q.W, q.C, q.NB, q.W };
+            k.b[1] = { q.up, q.W, q.C, q.NB, q.W };
+        }
         RowCopies copies;
         pad(&copies, q.a, k.a);
         pad(&copies, q.gate, k.b[0]);
@@ -121,7 +127,7 @@ tb200_status gated_pair(tb200_ctx* ctx, const GatedProblem& q)
         k.out_dt[0] = k.out_dt[1] = q.out_dt;
         k.ld        = q.W;
         k.name      = "gated_pair_f16";
-        TB200_TRY(q.H <= kFewRows && q.NB <= 65535 ? gated_rows_launch(ctx, k) : pair_launch(ctx, k));
+        TB200_TRY(few ? gated_rows_launch(ctx, k) : pair_launch(ctx, k));
     }
     return TB200_OK;
 }

@@ -190,6 +190,26 @@ __device__ __forceinline__ void store_fp(void* p, int64_t i, tb200_dtype dt, flo
         reinterpret_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
 }
 
+// The sixteen bytes from byte `by` of two neighbouring sixteens
+__device__ __forceinline__ uint4 shifted_piece(const uint4& lo, const uint4& hi, int by)
+{
+    uint32_t w[8] = { lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w };
+    if (by & 4)
+    {
+#pragma unroll
+        for (int i = 0; i < 7; i++)
+            w[i] = w[i + 1];
+    }
+    if (by & 8)
+    {
+#pragma unroll
+        for (int i = 0; i < 6; i++)
+            w[i] = w[i + 2];
+    }
+    const int bits = (by & 3) * 8;
+    return make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits), __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits));
+}
+
 __device__ __forceinline__ uint32_t pack2(float lo, float hi, bool bf16)
 {
     if (bf16)

@@ -11,6 +11,16 @@
 // Tiles go in groups of `group_m` rows of tiles, rows fastest: a wave's tiles then share few columns of B and the group's A stays
 // in L2 while B streams by once per group.
 // Sums are fp32 in tensor memory; results are rounded once, where they are stored.
+//
+// 4-bit weights (W4): the ring's stages receive a chunk's nibbles (4 KB where its values take 16), and three groups of four warps make the values in
+// their place, a thread a row of 64 elements, chunk by chunk in turn; the tensor cores wait for those as for A's bytes.  Laid out in
+// memory by a pass before, the values cost 10 us for 4096 x 4096; made here they pass through shared memory once more (a chunk takes a
+// pair 690 cycles instead of 520), which evens out at about 2000 rows.  Two groups were 10 to 20 % slower.
+//
+// Measured: gated 4096 x 4096 x 8192 bf16 344 us (1600 TFLOP/s, the rate of the library's product for a short time; power holds the
+// clock down when it goes on), backward of the same 1105 us (1490); 777 x 4096 x 4096 with 4-bit weights 35 us (750: 64 of 74 pairs, a quarter of the rows
+// padding; tensor pipe 61 % busy); gated 788 x 1000 x 1416 fp16 14 us, its backward at 394 x 1024 x 2048 32 us (chains of launches
+// of a few chunks: latencies of set-up, first copies, epilogue and exchange).
 #include <algorithm>
 #include <cstring>
 #include <cuda.h>

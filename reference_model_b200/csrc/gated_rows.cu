@@ -7,6 +7,8 @@
 // transposing matrix loads as they lie, K across rows.  Blocks of a cluster share K out while the grid leaves SMs idle.  The sums
 // of a stage are added up in fp32 apart from the instruction's own; G and U meet in shared memory, in a fixed order, where the
 // activation and the product are taken.
+// One row, 4096 x 16384 bf16: 42 us for 268 MB, the rate of a plain copy (6.4 TB/s; DRAM 73 % of its peak).  2048 x 8192: 9.5 us for 67 MB.  Small
+// calls are latency: 4 us.  Columns that are no multiple of eight cost a copy of both matrices first (3248 x 3748: 35 us, 7 for 3752).
 #include <algorithm>
 #include <cstring>
 #include <cuda.h>
@@ -23,7 +25,11 @@ namespace
 {
 
 constexpr int kFewWarps     = 8;
-constexpr int kFewThreads   = 32 * (kFewWarps + 1);    // and the TMA warp
+constexpr int kFewLoaders   = 16;                      // warps that fetch matrices whose rows are not multiples of 16 bytes apart, in two groups
+constexpr int few_threads(bool shift)
+{
+    return 32 * (kFewWarps + 1 + (shift ? kFewLoaders : 0));    // and the TMA warp
+}
 constexpr int kFewCols      = 64;                      // output columns of a block
 constexpr int kFewStageK    = 128;
 constexpr int kFewWBytes    = 2 * kFewStageK * kFewCols * 2;    // gate and up: 32 KB
@@ -34,6 +40,8 @@ struct FewParams
 {
     CUtensorMap tmG, tmU;    // [NB][C][W], box 64 columns x 64 rows
     CUtensorMap tmX;         // [NB][H][C], box 64 x 8 NT
+    const uint8_t* w[2];     // without tmG and tmU: the matrices, and their bytes
+    int64_t w_bytes;
     int W, C, H;
     int act;
     int stages_total, splits, per_split, num_stages, stage_bytes;
@@ -69,8 +77,8 @@ __device__ __forceinline__ void few_mma(float (&c)[4], const uint32_t (&a)[4], u
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-template <bool BF16, int NT>
-__global__ void __launch_bounds__(kFewThreads) gated_rows_kernel(const __grid_constant__ FewParams p)
+template <bool BF16, int NT, bool SHIFT>
+__global__ void __launch_bounds__(few_threads(SHIFT)) gated_rows_kernel(const __grid_constant__ FewParams p)
 {
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t bar_full[kFewMaxStages];
@@ -89,12 +97,15 @@ __global__ void __launch_bounds__(kFewThreads) gated_rows_kernel(const __grid_co
     {
         for (int s = 0; s < p.num_stages; s++)
         {
-            ptx::mbar_init(ptx::smem_u32(&bar_full[s]), 1);
+            ptx::mbar_init(ptx::smem_u32(&bar_full[s]), 1 + (SHIFT ? kFewLoaders / 2 : 0));
             ptx::mbar_init(ptx::smem_u32(&bar_empty[s]), kFewWarps);
         }
         ptx::fence_barrier_init();
-        ptx::prefetch_tmap(&p.tmG);
-        ptx::prefetch_tmap(&p.tmU);
+        if (!SHIFT)
+        {
+            ptx::prefetch_tmap(&p.tmG);
+            ptx::prefetch_tmap(&p.tmU);
+        }
         ptx::prefetch_tmap(&p.tmX);
         gave_up = 0;
         ptx::dep_launch_trigger();
@@ -124,14 +135,17 @@ __global__ void __launch_bounds__(kFewThreads) gated_rows_kernel(const __grid_co
                 }
                 const uint32_t full = ptx::smem_u32(&bar_full[s]);
                 const uint32_t sW   = smem_base + (uint32_t)(s * p.stage_bytes), sX = sW + kFewWBytes;
-                ptx::mbar_arrive_expect_tx(full, (uint32_t)p.stage_bytes);
+                ptx::mbar_arrive_expect_tx(full, (uint32_t)(p.stage_bytes - (SHIFT ? kFewWBytes : 0)));
                 const int k = (first + i) * kFewStageK;
 #pragma unroll
                 for (int j = 0; j < 2; j++)
                 {
                     // 64 rows of K: the gate's columns, the up projection's, a's elements
-                    ptx::tma_load_3d(sW + (uint32_t)(j * 8192), &p.tmG, full, col0, k + j * 64, batch);
-                    ptx::tma_load_3d(sW + (uint32_t)(16384 + j * 8192), &p.tmU, full, col0, k + j * 64, batch);
+                    if (!SHIFT)
+                    {
+                        ptx::tma_load_3d(sW + (uint32_t)(j * 8192), &p.tmG, full, col0, k + j * 64, batch);
+                        ptx::tma_load_3d(sW + (uint32_t)(16384 + j * 8192), &p.tmU, full, col0, k + j * 64, batch);
+                    }
                     ptx::tma_load_3d(sX + (uint32_t)(j * 8 * NT * 128), &p.tmX, full, k + j * 64, row0, batch);
                 }
                 if (++s == p.num_stages)
@@ -148,6 +162,71 @@ __global__ void __launch_bounds__(kFewThreads) gated_rows_kernel(const __grid_co
                     ptx::mbar_wait_bounded(ptx::smem_u32(&bar_full[j % p.num_stages]), (uint32_t)(j / p.num_stages) & 1u, ptx::kDrainCycles);
             }
         }
+    }
+    else if (SHIFT && warp > kFewWarps)
+    {
+        // Matrix rows that start anywhere: a thread makes sixteen bytes of a stage's row from the two aligned sixteens that hold them, eight such
+        // pieces of every second stage, into the places where TMA would put them.
+        const int loader = warp - kFewWarps - 1, group = loader >> 3, thread = (loader & 7) * 32 + lane;
+        const int piece = thread & 7, row_in = thread >> 3, col = col0 + piece * 8;
+        bool ok = true;
+        int s = group;
+        uint32_t phase = 0;
+        for (int i = group; i < mine; i += 2)
+        {
+            ok = __all_sync(0xffffffffu, ptx::mbar_wait_bounded(ptx::smem_u32(&bar_empty[s]), phase ^ 1u, p.wait_limit));
+            if (!ok)
+                break;
+            const uint32_t sW = smem_base + (uint32_t)(s * p.stage_bytes);
+#pragma unroll
+            for (int m = 0; m < 2; m++)
+            {
+                uint4 lo[4], hi[4];
+                int64_t at[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                {
+                    const int k = (first + i) * kFewStageK + row_in + 32 * j;
+                    at[j]       = k < p.C && col < p.W ? (((int64_t)batch * p.C + k) * p.W + col) * 2 : -1;
+                    lo[j] = hi[j] = make_uint4(0, 0, 0, 0);
+                    const int64_t aligned = at[j] & ~(int64_t)15;
+                    if (at[j] >= 0 && aligned + 32 <= p.w_bytes)
+                    {
+                        lo[j] = *reinterpret_cast<const uint4*>(p.w[m] + aligned);
+                        hi[j] = *reinterpret_cast<const uint4*>(p.w[m] + aligned + 16);
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                {
+                    const int row = row_in + 32 * j;
+                    uint4 v       = shifted_piece(lo[j], hi[j], (int)(at[j] & 15));
+                    if (at[j] >= 0 && (at[j] & ~(int64_t)15) + 32 > p.w_bytes)
+                    {
+                        // the matrix's last elements
+                        uint16_t e[8];
+#pragma unroll
+                        for (int c = 0; c < 8; c++)
+                            e[c] = at[j] + 2 * c < p.w_bytes ? *reinterpret_cast<const uint16_t*>(p.w[m] + at[j] + 2 * c) : (uint16_t)0;
+                        v = make_uint4(e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16, e[4] | (uint32_t)e[5] << 16, e[6] | (uint32_t)e[7] << 16);
+                    }
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(sW + (uint32_t)(m * 16384 + row * 128 + ((piece ^ (row & 7)) << 4))), "r"(v.x),
+                                 "r"(v.y), "r"(v.z), "r"(v.w)
+                                 : "memory");
+                }
+            }
+            __syncwarp();
+            if (lane == 0)
+                ptx::mbar_arrive(ptx::smem_u32(&bar_full[s]));
+            s += 2;
+            if (s >= p.num_stages)
+            {
+                s -= p.num_stages;
+                phase ^= 1u;
+            }
+        }
+        if (!ok && lane == 0)
+            atomicOr(p.status, TB200_DEV_TIMEOUT);
     }
     else
     {
@@ -283,10 +362,10 @@ tb200_status encode3d(tb200_ctx* ctx, CUtensorMap* m, const Matrix& x, bool bf16
 
 typedef void (*FewKern)(const FewParams);
 
-template <bool BF16>
+template <bool BF16, bool SHIFT>
 FewKern pick(int nt)
 {
-    return nt == 1 ? gated_rows_kernel<BF16, 1> : nt == 2 ? gated_rows_kernel<BF16, 2> : gated_rows_kernel<BF16, 4>;
+    return nt == 1 ? gated_rows_kernel<BF16, 1, SHIFT> : nt == 2 ? gated_rows_kernel<BF16, 2, SHIFT> : gated_rows_kernel<BF16, 4, SHIFT>;
 }
 
 }    // namespace
@@ -297,9 +376,13 @@ tb200_status gated_rows_launch(tb200_ctx* ctx, const PairProduct& q)
     memset(&p, 0, sizeof(p));
     const bool bf16 = q.dt == TB200_BF16;
     const int nt    = q.rows <= 8 ? 1 : q.rows <= 16 ? 2 : 4;
-    tb200_status st = encode3d(ctx, &p.tmG, q.b[0], bf16, 64);
-    if (st == TB200_OK)
+    const bool shift = q.b[0].pitch % 8 != 0;    // rows that TMA cannot address
+    tb200_status st  = shift ? TB200_OK : encode3d(ctx, &p.tmG, q.b[0], bf16, 64);
+    if (st == TB200_OK && !shift)
         st = encode3d(ctx, &p.tmU, q.b[1], bf16, 64);
+    p.w[0]    = reinterpret_cast<const uint8_t*>(q.b[0].data);
+    p.w[1]    = reinterpret_cast<const uint8_t*>(q.b[1].data);
+    p.w_bytes = q.b[0].batches * q.b[0].outer * q.b[0].inner * 2;
     if (st == TB200_OK)
         st = encode3d(ctx, &p.tmX, q.a, bf16, (uint32_t)(8 * nt));
     if (st != TB200_OK)
@@ -312,19 +395,21 @@ tb200_status gated_rows_launch(tb200_ctx* ctx, const PairProduct& q)
     const int64_t tiles = (p.W + kFewCols - 1) / kFewCols, yb = (p.H + 8 * nt - 1) / (8 * nt);
     // K over a cluster while the blocks do not fill the SMs and a block keeps two stages
     p.splits = 1;
-    while (p.splits < 8 && p.stages_total / (2 * p.splits) >= 2 && tiles * yb * q.NB * p.splits < ctx->num_sms)
+    while (p.splits < 8 && p.stages_total / (2 * p.splits) >= 2 && tiles * yb * q.NB * p.splits * (shift ? 2 : 1) < ctx->num_sms + (shift ? 1 : 0))
         p.splits *= 2;
     p.per_split       = (p.stages_total + p.splits - 1) / p.splits;
-    p.num_stages      = std::max(2, std::min(std::min(kFewMaxStages, p.per_split), (104 * 1024) / p.stage_bytes));
+    p.num_stages      = std::max(2, std::min(std::min(kFewMaxStages, p.per_split), (shift ? 200 : 104) * 1024 / p.stage_bytes));
+    if (shift)
+        p.num_stages &= ~1;    // a group of loaders keeps to its stages
     const size_t red  = (size_t)8 * nt * kFewRedLd * sizeof(float);
     const size_t smem = std::max((size_t)p.num_stages * p.stage_bytes, red) + 1024;
-    const FewKern kern = bf16 ? pick<true>(nt) : pick<false>(nt);
-    st = raise_smem_limit(ctx, 168 + nt / 2 * 2 + (bf16 ? 1 : 0), reinterpret_cast<const void*>(kern), (int)smem);
+    const FewKern kern = bf16 ? (shift ? pick<true, true>(nt) : pick<true, false>(nt)) : shift ? pick<false, true>(nt) : pick<false, false>(nt);
+    st = raise_smem_limit(ctx, (shift ? 140 : 168) + nt / 2 * 2 + (bf16 ? 1 : 0), reinterpret_cast<const void*>(kern), (int)smem);
     if (st != TB200_OK)
         return st;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim            = dim3((unsigned)(tiles * p.splits), (unsigned)yb, (unsigned)q.NB);
-    cfg.blockDim           = dim3(kFewThreads);
+    cfg.blockDim           = dim3((unsigned)few_threads(shift));
     cfg.dynamicSmemBytes   = smem;
     cfg.stream             = ctx->stream;
     cudaLaunchAttribute at[2];

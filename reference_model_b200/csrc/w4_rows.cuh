@@ -16,8 +16,14 @@
 // number of consecutive stages, whatever tile they belong to, so that all SMs end together (whole tiles over 148 SMs left up to
 // half of them idle).  A tile that several blocks share goes through fp32 sums in scratch: the block whose stages complete it adds them
 // up, in block order, so results do not depend on which one that is.
-// Eight warps take 32 rows each and one half of every stage (with more rows of `a`, 16 and all of it).  One thread feeds a ring of stages by TMA (weights and rows of `a` with
-// 128-byte swizzle, so that both are read from shared memory without bank conflicts; scales and zero points as they lie).
+// Eight warps take 32 rows each and one half of every stage (with more rows of `a`, 16 and all of it).  One thread feeds a ring of stages
+// by TMA (weights and rows of `a` with 128-byte swizzle, so that both are read from shared memory without bank conflicts; scales and zero points
+// as they lie: threads that fetched them cost 5 us a call).
+//
+// Measured, bf16, one row, group 128 with zero points: 8192 x 8192 15.4 us (35 MB, 2.3 TB/s), gated 4096 x 16384 24.3 us (2.9 TB/s); 24 rows,
+// 4096 x 10250 fp16 21.9 us; 2048 x 1000 6.5 us.  What bounds it: instructions (78 to 100 for 1024 weights; 45 % of the issue slots over
+// the whole kernel, the integer pipe 39 %), and at either end latencies: 1.4 us from the start to the first stage, 1.5 to 4 us from a
+// shared tile's last sums to its results.
 #pragma once
 #include <cuda.h>
 #include <type_traits>

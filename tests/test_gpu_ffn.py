@@ -246,6 +246,30 @@ def test_w4_parts_of_fp32_rows(ctx, rows):
     m.free()
 
 
+@pytest.mark.parametrize("nb", (1, 3))
+@pytest.mark.parametrize("c", (1, 37, 300, 1500))
+@pytest.mark.parametrize("w", (1, 7, 203, 206, 212, 1001))
+@pytest.mark.parametrize("h", (1, 9, 30))
+def test_gated_rows_of_matrices_at_any_element(ctx, h, w, c, nb):
+    """Matrices whose rows do not start at multiples of sixteen bytes, on whole numbers: exact.  NaNs behind the last row and in the next
+    batch's rows count for nothing."""
+    a, bg, bu = whole(21, "bf16", -1, 2, nb, h, c), whole(22, "bf16", -1, 2, nb, c, w), whole(23, "bf16", -1, 2, nb, c, w)
+    out = blank(ctx, "fp32", (nb, h, w))
+    ts = [put(ctx, a)]
+    if nb > 1:
+        bg[1] = bu[1] = math.nan
+    ts += [put(ctx, bg), put(ctx, bu)]
+    ctx.matmul_gated(*ts, out, "RELU")
+    assert ctx.last_kernel() == "gated_rows_f16"
+    ref, got = (a.double() @ bg.double()).clamp(min=0) * (a.double() @ bu.double()), get(out).double()
+    if nb > 1:
+        assert torch.isnan(got[1]).all()
+        ref[1] = got[1] = 0
+    assert torch.equal(got, ref)
+    for t in ts + [out]:
+        t.free()
+
+
 def test_w4_extreme_values(ctx):
     """Lowest and highest elements, zero points at both ends, scales of both signs and zero."""
     c, w = 256, 64
@@ -695,6 +719,7 @@ def forms(ctx):
 
     gated("few rows, K over clusters", "gated_rows_f16", 1, 1, 3, 4000, 200)
     gated("few rows, many columns", "gated_rows_f16", 2, 2, 30, 264, 12000)
+    gated("few rows, odd columns", "gated_rows_f16", 2, 2, 3, 2000, 203)
     gated("pairs", "gated_pair_f16", 1, 1, 1500, 520, 2000)
     gated("single, K over clusters", "gated_pair_f16", 1, 1, 100, 4000, 72)
     gated("single", "gated_pair_f16", 3, 3, 150, 100, 300)
@@ -712,7 +737,7 @@ def forms(ctx):
     return made
 
 
-FORMS = ["few rows, K over clusters", "few rows, many columns", "pairs", "single, K over clusters", "single", "few rows", "few rows, gated", "30 rows",
+FORMS = ["few rows, K over clusters", "few rows, many columns", "few rows, odd columns", "pairs", "single, K over clusters", "single", "few rows", "few rows, gated", "30 rows",
          "many rows", "many rows, gated", "many rows, K over clusters", "many rows, pairs", "many rows, gated pairs", "small", "long K", "large"]
 
 
