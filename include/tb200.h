@@ -321,8 +321,8 @@ extern "C"
      * column).  What a row holds behind its last element is not used.  Rows whose pitch is a multiple of 16 bytes are
      * read as they are; others are copied into scratch first.
      * Up to 32 rows of a (21 in FP32; N H of them) multiply element - zero exactly and scale the fp32 sum of a group.  More rows
-     * multiply the values scale * (element - zero), rounded once to a's type: in FP16 they overflow from 65520 on and lose
-     * places below 2^-14. */
+     * multiply the values scale * (element - zero) in a's type: rounded once for tb200_matmul_w4, taken as two such numbers for
+     * tb200_matmul_gated_w4.  In FP16 they overflow from 65520 on and lose places below 2^-14. */
     typedef struct tb200_w4
     {
         const tb200_tensor* data;

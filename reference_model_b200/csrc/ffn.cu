@@ -303,7 +303,7 @@ tb200_status gated_backward_f32(tb200_ctx* ctx, const GatedProblem& q)
     return post_launch(ctx, "gated_backward_f32", 0);
 }
 
-// 4-bit weights: few rows multiply whole numbers and scale the sums; more take the weights' values, rounded to a's type as a tile needs them.  Many fp32
+// 4-bit weights: few rows multiply whole numbers and scale the sums; more take the weights' values in a's type, as a tile needs them.  Many fp32
 // rows go through fp32 values laid out in scratch.
 tb200_status w4_launch(tb200_ctx* ctx, const W4Problem& q)
 {

@@ -15,7 +15,9 @@
 // 4-bit weights (W4): the ring's stages receive a chunk's nibbles (4 KB where its values take 16), and three groups of four warps make the values in
 // their place, a thread a row of 64 elements, chunk by chunk in turn; the tensor cores wait for those as for A's bytes.  Laid out in
 // memory by a pass before, the values cost 10 us for 4096 x 4096; made here they pass through shared memory once more (a chunk takes a
-// pair 690 cycles instead of 520), which evens out at about 2000 rows.  Two groups were 10 to 20 % slower.
+// pair 690 cycles instead of 520), which evens out at about 2000 rows.  Two groups were 10 to 20 % slower.  The gated product carries what the
+// rounding of a value left as a second 16-bit number and a second MMA: rounded once, two projections' weights put 1.6 times the
+// output's own rounding into the result (100 x 2048 x 8192: 17.4 us so, 21.6 with both; 1000 rows 62 and 88).
 //
 // Measured: gated 4096 x 4096 x 8192 bf16 344 us (1600 TFLOP/s, the rate of the library's product for a short time; power holds the
 // clock down when it goes on), backward of the same 1105 us (1490); 777 x 4096 x 4096 with 4-bit weights 35 us (750: 64 of 74 pairs, a quarter of the rows
@@ -39,22 +41,22 @@ namespace
 {
 
 constexpr int kEpiWarps = 8;
-constexpr int kExpandGroups = 3;                  // of four warps: 4-bit weights to 16 bits
-constexpr int kExpandWarps = 4 * kExpandGroups;
 constexpr int kRawBytes    = 128 * 32;            // 128 rows x 64 elements of 4-bit weights
 constexpr int kChunk    = 16384;                  // 128 rows (or columns) x 64 elements of K
 
 // Pairs of CTAs (PAIR) with tiles of 256 rows and 256 accumulator columns, or CTAs by themselves with 128 x 128; one CTA to an SM.
-template <bool PAIR, bool W4 = false>
+// W4: 4-bit weights; LOW: their values as two 16-bit numbers each.
+template <bool PAIR, bool W4 = false, bool LOW = false>
 struct Shape
 {
-    static constexpr int kThreads = 64 + 32 * (kEpiWarps + (W4 ? kExpandWarps : 0));    // TMA warp, MMA warp, epilogue, and those
-    static constexpr int kStages = PAIR && !W4 ? 3 : 6;
-    static_assert(!W4 || kStages % kExpandGroups == 0, "a group keeps to its stages");
+    static constexpr int kGroups  = !W4 ? 0 : LOW ? 2 : 3;                   // of four warps that make the values
+    static constexpr int kThreads = 64 + 32 * (kEpiWarps + 4 * kGroups);     // TMA warp, MMA warp, epilogue, and those
+    static constexpr int kStages = LOW ? 4 : PAIR && !W4 ? 3 : 6;
+    static_assert(!W4 || kStages % kGroups == 0, "a group keeps to its stages");
     static constexpr int kCtas = PAIR ? 2 : 1;
     static constexpr int kRows = 128 * kCtas, kCols = PAIR ? 256 : 128;    // of a tile
     static constexpr int kSub  = PAIR && !W4 ? 2 : 1;                      // chunks per stage
-    static constexpr int kStage = 2 * kSub * kChunk;                       // each CTA holds 128 rows of A and 128 columns of B
+    static constexpr int kStage = (LOW ? 3 : 2 * kSub) * kChunk;           // each CTA holds 128 rows of A and 128 columns of B
     // (with the static part all of an SM's: a CTA that waits for tensor memory never shares an SM with another kernel's that holds some)
     static constexpr int kSmem  = 208 * 1024;
     static_assert(kStages * kStage + 1024 <= kSmem, "the ring fits");
@@ -361,7 +363,8 @@ __device__ __forceinline__ void load_zero(int& v, const int8_t* at, bool any)
 
 // A row's 64 elements of 4-bit weights (two sixteens of bytes) as 16-bit values in a chunk of B: 128 bytes, swizzled.  Values are rounded to the
 // operands' type, once: by scales of that type (SAME) as they are, by others in fp32.  TAIL: `left` elements up to the end of K.
-template <bool BF16, bool SAME, bool TAIL>
+// LOW: a chunk further, what the rounding left (exactly, for SAME): a value is then as good as never rounded.
+template <bool BF16, bool SAME, bool TAIL, bool LOW>
 __device__ __forceinline__ void expand_row(const uint4 (&raw)[2], const uint32_t (&bits)[2], tb200_dtype scale_dt, const int (&zero)[2], int left, uint32_t dst, int row)
 {
 #pragma unroll
@@ -379,15 +382,27 @@ __device__ __forceinline__ void expand_row(const uint4 (&raw)[2], const uint32_t
             o[1] = __byte_perm(v[2], v[3], 0x5410);
             o[2] = __byte_perm(v[0], v[1], 0x7632);
             o[3] = __byte_perm(v[2], v[3], 0x7632);
+            uint32_t low[4];
 #pragma unroll
             for (int j = 0; j < 4; j++)
             {
+                const uint32_t whole = o[j];
                 if (SAME)
-                    o[j] = BF16 ? fma2_bf16(o[j], s2, 0x80008000u) : fma2_f16(o[j], s2, 0x80008000u);
+                {
+                    o[j] = BF16 ? fma2_bf16(whole, s2, 0x80008000u) : fma2_f16(whole, s2, 0x80008000u);
+                    if (LOW)
+                        low[j] = BF16 ? fma2_bf16(whole, s2, o[j] ^ 0x80008000u) : fma2_f16(whole, s2, o[j] ^ 0x80008000u);
+                }
                 else
                 {
-                    const float2 f = unpack2(o[j], BF16);
-                    o[j]           = pack2(f.x * scale, f.y * scale, BF16);
+                    const float2 f = unpack2(whole, BF16);
+                    const float x = f.x * scale, y = f.y * scale;
+                    o[j]          = pack2(x, y, BF16);
+                    if (LOW)
+                    {
+                        const float2 h = unpack2(o[j], BF16);
+                        low[j]         = pack2(x - h.x, y - h.y, BF16);
+                    }
                 }
             }
             if (TAIL)
@@ -398,8 +413,14 @@ __device__ __forceinline__ void expand_row(const uint4 (&raw)[2], const uint32_t
                 {
                     const int at = h * 32 + i * 8 + j * 2;
                     o[j]         = at + 1 < left ? o[j] : at < left ? o[j] & 0xffffu : 0u;
+                    if (LOW)
+                        low[j] = at + 1 < left ? low[j] : at < left ? low[j] & 0xffffu : 0u;
                 }
             }
+            if (LOW)
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + (uint32_t)(kChunk + (((h * 4 + i) ^ (row & 7)) << 4))), "r"(low[0]), "r"(low[1]),
+                             "r"(low[2]), "r"(low[3])
+                             : "memory");
             asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + (uint32_t)(((h * 4 + i) ^ (row & 7)) << 4)), "r"(o[0]), "r"(o[1]), "r"(o[2]),
                          "r"(o[3])
                          : "memory");
@@ -408,10 +429,11 @@ __device__ __forceinline__ void expand_row(const uint4 (&raw)[2], const uint32_t
 }
 
 template <int EPI, bool A_MN, bool B_MN, bool PAIR, bool W4 = false>
-__global__ void __launch_bounds__((Shape<PAIR, W4>::kThreads), 1) ffn_pair_kernel(const __grid_constant__ Params p)
+__global__ void __launch_bounds__((Shape<PAIR, W4, W4 && EPI == EPI_GATED>::kThreads), 1) ffn_pair_kernel(const __grid_constant__ Params p)
 {
     static_assert(W4 || EPI == EPI_PLAIN || B_MN, "both projections' matrices have K across their rows");
-    using S               = Shape<PAIR, W4>;
+    constexpr bool LOW    = W4 && EPI == EPI_GATED;
+    using S               = Shape<PAIR, W4, LOW>;
     constexpr int kSub    = S::kSub, kStage = S::kStage, kHalf = S::kCols / 2, kStages = S::kStages, kThreads = S::kThreads;
     extern __shared__ uint8_t smem_raw[];
     // identical layout in both CTAs of a pair: remote signals address a barrier by its offset
@@ -671,6 +693,13 @@ __global__ void __launch_bounds__((Shape<PAIR, W4>::kThreads), 1) ffn_pair_kerne
                             else
                                 ptx::mma_f16_ss(d_tmem, ad, bd, p.idesc, accum);
                             accum = 1;
+                            if (LOW)
+                            {
+                                if (PAIR)
+                                    ptx::mma_f16_ss_pair(d_tmem, ad, bd + kChunk / 16, p.idesc, 1);
+                                else
+                                    ptx::mma_f16_ss(d_tmem, ad, bd + kChunk / 16, p.idesc, 1);
+                            }
                             // sixteen elements of K: 32 bytes inside the swizzled row, or sixteen rows of 128 bytes
                             ad += A_MN ? 128 : 2;
                             bd += B_MN ? 128 : 2;
@@ -767,8 +796,8 @@ __global__ void __launch_bounds__((Shape<PAIR, W4>::kThreads), 1) ffn_pair_kerne
                 zero[h]  = zero_next[h];
                 bad |= zero[h] < -8 || zero[h] > 7;
             }
-            c += kExpandGroups;
-            for (into += 2 * kExpandGroups; into >= p.group32; into -= p.group32)
+            c += S::kGroups;
+            for (into += 2 * S::kGroups; into >= p.group32; into -= p.group32)
                 first_group++;
             to_tile();
             if (tile < p.num_tiles)
@@ -786,11 +815,11 @@ __global__ void __launch_bounds__((Shape<PAIR, W4>::kThreads), 1) ffn_pair_kerne
             auto expand        = [&](auto bf16) {
                 constexpr bool kBf16 = decltype(bf16)::value;
                 if (left < 64)
-                    expand_row<kBf16, false, true>(raw, scale, p.scale_dt[mat], zero, left, dst, row);
+                    expand_row<kBf16, false, true, LOW>(raw, scale, p.scale_dt[mat], zero, left, dst, row);
                 else if (same)
-                    expand_row<kBf16, true, false>(raw, scale, p.scale_dt[mat], zero, left, dst, row);
+                    expand_row<kBf16, true, false, LOW>(raw, scale, p.scale_dt[mat], zero, left, dst, row);
                 else
-                    expand_row<kBf16, false, false>(raw, scale, p.scale_dt[mat], zero, left, dst, row);
+                    expand_row<kBf16, false, false, LOW>(raw, scale, p.scale_dt[mat], zero, left, dst, row);
             };
             if (p.bf16)
                 expand(std::true_type());
@@ -805,7 +834,7 @@ __global__ void __launch_bounds__((Shape<PAIR, W4>::kThreads), 1) ffn_pair_kerne
                 else
                     ptx::mbar_arrive(ptx::smem_u32(&bar_full[stage]));
             }
-            stage += kExpandGroups;
+            stage += S::kGroups;
             if (stage >= kStages)
             {
                 stage -= kStages;
@@ -1112,7 +1141,7 @@ tb200_status launch(tb200_ctx* ctx, const PairProduct& q, int splits)
     if (st != TB200_OK)
         return st;
     cudaLaunchConfig_t cfg = {};
-    cfg.blockDim           = dim3(q.w4 ? Shape<PAIR, true>::kThreads : S::kThreads);
+    cfg.blockDim           = dim3(!q.w4 ? S::kThreads : gated ? Shape<PAIR, true, true>::kThreads : Shape<PAIR, true>::kThreads);
     cfg.dynamicSmemBytes   = (size_t)S::kSmem;
     cfg.stream             = ctx->stream;
     cudaLaunchAttribute attr[2];
@@ -1174,13 +1203,13 @@ tb200_status pair_launch(tb200_ctx* ctx, const PairProduct& q)
     auto tiles = [&](int rows, int cols) { return (int64_t)((q.rows + rows - 1) / rows) * ((q.cols + cols - 1) / cols) * copies; };
     auto waves = [&](int64_t n, int64_t at_once) { return (double)((n + at_once - 1) / at_once); };
     const int64_t large = tiles(256, gated ? 128 : 256), small = tiles(128, gated ? 64 : 128);
-    double best = waves(large, ctx->num_sms / 2) * (double)chunks * (q.w4 ? 690.0 : 520.0) + 4500.0;
+    double best = waves(large, ctx->num_sms / 2) * (double)chunks * (!q.w4 ? 520.0 : gated ? 1100.0 : 690.0) + 4500.0;
     int splits  = 0;
     for (int s = 1, i = 0; s <= 8; s *= 2, i++)
     {
         if (s > 1 && (chunks < 4 * s || small * s > ctx->num_sms))
             break;
-        const double chunk = q.w4 ? 490.0 : std::max(330.0, 700.0 * (double)std::min<int64_t>(small * s, ctx->num_sms) / ctx->num_sms);
+        const double chunk = q.w4 ? (gated ? 700.0 : 490.0) : std::max(330.0, 700.0 * (double)std::min<int64_t>(small * s, ctx->num_sms) / ctx->num_sms);
         double cost        = waves(small, ctx->num_sms) * (double)chunks * chunk + 2500.0;
         if (s > 1)
         {

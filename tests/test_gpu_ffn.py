@@ -230,6 +230,28 @@ def test_w4_values_are_rounded_once(ctx, h, w, dtype, scales, group):
     m.free()
 
 
+@pytest.mark.parametrize("scales", ("fp16", "bf16", "fp32"))
+@pytest.mark.parametrize("dtype", ("fp16", "bf16"))
+@pytest.mark.parametrize("h,w", ((70, 70), (700, 2060)))
+def test_gated_w4_values_are_not_rounded(ctx, h, w, dtype, scales):
+    """The gated product takes a value as two numbers, each off by half a step: half a step's square of the value, or half the smallest
+    fp16 number (2^-25).  An fp32 scale's value is rounded to fp32 before (2^-24).  Sums have twice the terms."""
+    c = 197
+    a = rand(15, dtype, 1.0, 1, h, c)
+    g, u = Four(ctx, 16, c, w, 96, True, True, scales), Four(ctx, 17, c, w, 96, True, True, scales)
+    ta, to = put(ctx, a), blank(ctx, "fp32", (1, h, w))
+    ctx.matmul_gated_w4(ta, g.op, u.op, to, "SIGMOID")
+    assert ctx.last_kernel() == "gated_w4_pair"
+    a64 = a.double()
+    least = 2.0 ** -25 * a64.abs().sum(-1, keepdim=True) if dtype == "fp16" else 0.0
+    eg, eu = ((acc(2 * c, dtype) + HALF[dtype] ** 2 + 2.0 ** -24) * (a64.abs() @ m.dense.abs()) + least for m in (g, u))
+    check_gated(get(to), a64 @ g.dense, a64 @ u.dense, eg, eu, "SIGMOID", "fp32")
+    for t in (ta, to):
+        t.free()
+    g.free()
+    u.free()
+
+
 @pytest.mark.parametrize("rows", (15, 16, 21))
 def test_w4_parts_of_fp32_rows(ctx, rows):
     """45 to 63 bf16 parts.  fp32 sums of exact products: as far off as 16-bit operands' (the parts' products are exact too)."""
