@@ -373,6 +373,8 @@ __device__ __forceinline__ void expand_row(const uint4 (&raw)[2], const uint32_t
         const uint32_t w[4] = { raw[h].x, raw[h].y, raw[h].z, raw[h].w };
         const uint32_t base = unpack_base<BF16>(zero[h]), s2 = bits[h] * 0x10001u;
         const float scale   = SAME ? 0.f : bits_fp(bits[h], scale_dt);
+        // a value that overflows has no second number (infinity less infinity; SAME is not called where one may)
+        const uint32_t keep = fabsf(scale) * 15.f < (BF16 ? 3.38e38f : 65504.f) ? 0xffffffffu : 0u;
 #pragma unroll
         for (int i = 0; i < 4; i++)
         {
@@ -401,7 +403,7 @@ __device__ __forceinline__ void expand_row(const uint4 (&raw)[2], const uint32_t
                     if (LOW)
                     {
                         const float2 h = unpack2(o[j], BF16);
-                        low[j]         = pack2(x - h.x, y - h.y, BF16);
+                        low[j]         = keep & pack2(x - h.x, y - h.y, BF16);
                     }
                 }
             }
@@ -756,7 +758,8 @@ __global__ void __launch_bounds__((Shape<PAIR, W4, W4 && EPI == EPI_GATED>::kThr
         const bool with_zero     = p.zero[mat] != nullptr;
         const uint8_t* scale_at  = nullptr;    // of the thread's column, first group
         const int8_t* zero_at    = nullptr;
-        const int scale_step     = p.cols * (wide ? 4 : 2), last_group = p.groups - 1;
+        const int64_t scale_step = (int64_t)p.cols * (wide ? 4 : 2);
+        const int last_group     = p.groups - 1;
         auto to_column = [&]() {
             const int col = min(decode<EPI, PAIR>(p, tile).n0 + shift, p.cols - 1);
             scale_at      = reinterpret_cast<const uint8_t*>(p.scale[mat]) + (int64_t)col * (wide ? 4 : 2);
@@ -766,8 +769,8 @@ __global__ void __launch_bounds__((Shape<PAIR, W4, W4 && EPI == EPI_GATED>::kThr
         };
         auto fetch = [&]() {
             const int g0 = min(first_group, last_group), g1 = min(first_group + (into + 1 >= p.group32 ? 1 : 0), last_group);
-            load_bits(scale_next[0], scale_at + (int64_t)g0 * scale_step, wide);
-            load_bits(scale_next[1], scale_at + (int64_t)g1 * scale_step, wide);
+            load_bits(scale_next[0], scale_at + g0 * scale_step, wide);
+            load_bits(scale_next[1], scale_at + g1 * scale_step, wide);
             load_zero(zero_next[0], zero_at + (int64_t)g0 * p.cols, with_zero);
             load_zero(zero_next[1], zero_at + (int64_t)g1 * p.cols, with_zero);
         };
@@ -816,7 +819,7 @@ __global__ void __launch_bounds__((Shape<PAIR, W4, W4 && EPI == EPI_GATED>::kThr
                 constexpr bool kBf16 = decltype(bf16)::value;
                 if (left < 64)
                     expand_row<kBf16, false, true, LOW>(raw, scale, p.scale_dt[mat], zero, left, dst, row);
-                else if (same)
+                else if (same && (!LOW || max(scale[0] & 0x7fffu, scale[1] & 0x7fffu) < (kBf16 ? 0x7d88u : 0x6c44u)))    // the largest number over 15
                     expand_row<kBf16, true, false, LOW>(raw, scale, p.scale_dt[mat], zero, left, dst, row);
                 else
                     expand_row<kBf16, false, false, LOW>(raw, scale, p.scale_dt[mat], zero, left, dst, row);

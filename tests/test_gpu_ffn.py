@@ -252,6 +252,35 @@ def test_gated_w4_values_are_not_rounded(ctx, h, w, dtype, scales):
     u.free()
 
 
+@pytest.mark.parametrize("scales", ("same", "fp32"))
+@pytest.mark.parametrize("h", (5, 70))
+@pytest.mark.parametrize("dtype", ("fp16", "bf16"))
+def test_gated_w4_infinite_scales(ctx, h, dtype, scales):
+    """A group of one element under an infinite scale: the gate's sum is infinite, not a NaN; its sigmoid is 0 or 1."""
+    c, w = 33, 70
+    a = rand(18, dtype, 1.0, 1, h, c)
+    a[a == 0] = 1
+    scales = dtype if scales == "same" else scales
+    g, u = Four(ctx, 19, c, w, 32, True, True, scales), Four(ctx, 20, c, w, 32, True, True, scales)
+    s = get(g.op.scale)
+    whole_numbers = g.dense[32] * s[1].double().sign()    # their signs
+    s[1, :] = math.inf
+    g.op.scale.upload(s.view(torch.uint16).numpy() if scales == "bf16" else s.numpy())
+    ta, to = put(ctx, a), blank(ctx, "fp32", (1, h, w))
+    ctx.matmul_gated_w4(ta, g.op, u.op, to, "SIGMOID")
+    a64, last = a.double(), g.dense[32] != 0    # (zero times infinity is a NaN)
+    assert int(last.sum()) > w // 2
+    U, S = a64 @ u.dense, a64.abs() @ u.dense.abs()
+    one = (a64[..., 32:] * whole_numbers > 0).double()
+    got = get(to).double()
+    off = (got - one * U).abs() <= (acc(2 * c, dtype) + HALF[dtype] ** 2 + 2.0 ** -23) * S + 2.0 ** -24 * a64.abs().sum(-1, keepdim=True)
+    assert off[..., last].all() and torch.isnan(got[..., ~last]).all()
+    for t in (ta, to):
+        t.free()
+    g.free()
+    u.free()
+
+
 @pytest.mark.parametrize("rows", (15, 16, 21))
 def test_w4_parts_of_fp32_rows(ctx, rows):
     """45 to 63 bf16 parts.  fp32 sums of exact products: as far off as 16-bit operands' (the parts' products are exact too)."""
