@@ -241,9 +241,11 @@ tb200_status projections_f32(tb200_ctx* ctx, const GatedProblem& q, float* gu)
     return sgemm_f32_launch(ctx, a, up, gu + (int64_t)q.NB * q.H * q.W, q.NB, (int)q.H, q.C, q.W);
 }
 
-// fp32: the two projections by the fp32 product, then a pass over them
+// fp32: one row past streamed weights; more as the two projections by the fp32 product, then a pass over them
 tb200_status gated_f32(tb200_ctx* ctx, const GatedProblem& q)
 {
+    if (q.H == 1 && q.NB <= 65535)
+        return gated_rows_f32_launch(ctx, q);
     const int64_t n = q.NB * q.H * q.W;
     TB200_TRY(ensure_scratch(ctx, (size_t)n * 8));
     float* const gu = reinterpret_cast<float*>(ctx->scratch);

@@ -98,6 +98,9 @@ tb200_status pair_launch(tb200_ctx* ctx, const PairProduct& q);
 // ---- gated_rows.cu: PAIR_GATED with K across b's rows and few rows of a (weights read once)
 tb200_status gated_rows_launch(tb200_ctx* ctx, const PairProduct& q);
 
+// ---- gated_rows_f32.cu: the fp32 gated product of one row
+tb200_status gated_rows_f32_launch(tb200_ctx* ctx, const GatedProblem& q);
+
 // ---- w4_rows.cu: up to 32 16-bit rows against 4-bit weights
 // (64, where they are parts of fp32 rows.)
 // x: a's rows in 16 bits, `x_pitch` elements apart (a multiple of 8), 16-byte aligned; fp32 rows as three bf16 rows each (parts 3,

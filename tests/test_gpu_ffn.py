@@ -281,6 +281,28 @@ def test_gated_w4_infinite_scales(ctx, h, dtype, scales):
     u.free()
 
 
+@pytest.mark.parametrize("nb", (1, 3))
+@pytest.mark.parametrize("c", (1, 63, 300, 2000))
+@pytest.mark.parametrize("w", (1, 100, 129, 1002))
+def test_gated_f32_one_row(ctx, w, c, nb):
+    """Whole numbers, exact; a NaN in one batch's row stays there."""
+    h = 1
+    a, bg, bu = whole(31, "fp32", -3, 4, nb, h, c), whole(32, "fp32", -3, 4, nb, c, w), whole(33, "fp32", -3, 4, nb, c, w)
+    if nb > 1:
+        a[1, 0, c // 2] = math.nan
+    out = blank(ctx, "fp32", (nb, h, w))
+    ts  = [put(ctx, t) for t in (a, bg, bu)]
+    ctx.matmul_gated(*ts, out, "RELU")
+    assert ctx.last_kernel() == "gated_rows_f32"
+    a, got = a.double(), get(out).double()
+    if nb > 1:
+        assert torch.isnan(got[1]).all()
+        a[1], got[1] = 0, 0
+    assert torch.equal(got, (a @ bg.double()).clamp(min=0) * (a @ bu.double()))
+    for t in ts + [out]:
+        t.free()
+
+
 @pytest.mark.parametrize("rows", (15, 16, 21))
 def test_w4_parts_of_fp32_rows(ctx, rows):
     """45 to 63 bf16 parts.  fp32 sums of exact products: as far off as 16-bit operands' (the parts' products are exact too)."""
