@@ -3,8 +3,8 @@
 //
 // A block takes 128 columns of the gate and the same 128 of the up projection, a lane four of each; its eight warps take K's elements in turn,
 // sixteen loads of a lane on their way together.  Blocks of a cluster share K out while all run at once.  Sums of warps, then of blocks, are
-// added up in a fixed order.  4096 x 8192: 42.5 us, 6.3 TB/s, the rate of a plain copy (76 by the fp32 product's tiles and a pass over both
-// projections); 100 x 4000 4.0 us (7.3).  Two rows by the same code took 94 us, which leaves them to the tiles.
+// added up in a fixed order.  4096 x 8192: 57 us, 4.7 TB/s (76 by the fp32 product's tiles and a pass over both projections);
+// 100 x 4000 5.5 us (7.3).  What bounds it: a warp waits for all of its loads before it adds, two blocks to an SM.  Two rows by the same code took 94 us, which leaves them to the tiles.
 #include <algorithm>
 #include <cstring>
 
