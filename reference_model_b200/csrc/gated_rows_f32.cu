@@ -2,9 +2,10 @@
 // is an IEEE fp32 operation.
 //
 // A block takes 128 columns of the gate and the same 128 of the up projection, a lane four of each; its eight warps take K's elements in turn,
-// sixteen loads of a lane on their way together.  Blocks of a cluster share K out while all run at once.  Sums of warps, then of blocks, are
-// added up in a fixed order.  4096 x 8192: 57 us, 4.7 TB/s (76 by the fp32 product's tiles and a pass over both projections);
-// 100 x 4000 5.5 us (7.3).  What bounds it: a warp waits for all of its loads before it adds, two blocks to an SM.  Two rows by the same code took 94 us, which leaves them to the tiles.
+// eight loads of a lane on their way together, four blocks to an SM (sixteen loads and two blocks: 4096 x 8192 56 us).  Blocks of a cluster
+// share K out while all run at once.  Sums of warps, then of blocks, are added up in a fixed order.  4096 x 8192: 44 us, 6.1 TB/s, the rate of
+// a plain copy (76 by the fp32 product's tiles and a pass over both projections); 1480 x 7328 15 us (31); 100 x 4000 6.8 us (7.3).  Two rows by
+// the same code took 94 us, which leaves them to the tiles.
 #include <algorithm>
 #include <cstring>
 
@@ -19,7 +20,7 @@ namespace ffn
 namespace
 {
 
-constexpr int kF32Threads = 256, kF32Warps = 8, kF32Cols = 128, kF32Ahead = 8;    // elements of K whose weights are on their way
+constexpr int kF32Threads = 256, kF32Warps = 8, kF32Cols = 128, kF32Ahead = 4;    // elements of K whose weights are on their way
 
 struct FewF32Params
 {
@@ -50,7 +51,7 @@ __device__ __forceinline__ void weights4(const float* row, int col0, int lane, i
 }
 
 template <bool VEC>
-__global__ void __launch_bounds__(kF32Threads) gated_rows_f32_kernel(const __grid_constant__ FewF32Params p)
+__global__ void __launch_bounds__(kF32Threads, 4) gated_rows_f32_kernel(const __grid_constant__ FewF32Params p)
 {
     extern __shared__ float sums[];    // [warps][2][128]; the block's own in the first warp's place
     ptx::dep_launch_trigger();
@@ -150,9 +151,9 @@ tb200_status gated_rows_f32_launch(tb200_ctx* ctx, const GatedProblem& q)
     p.out  = reinterpret_cast<float*>(q.out);
     p.C = q.C; p.W = q.W; p.act = q.act;
     const int64_t tiles = (p.W + kF32Cols - 1) / kF32Cols;
-    // K over a cluster while all blocks run at once (two to an SM, less what clusters leave) and a warp keeps a batch of loads
+    // K over a cluster while all blocks run at once (four to an SM, less what clusters leave) and a warp keeps two batches of loads
     p.splits = 1;
-    while (p.splits < 8 && p.C >= 2 * p.splits * kF32Warps * kF32Ahead && tiles * q.NB * p.splits * 2 <= ctx->num_sms * 7 / 4)
+    while (p.splits < 8 && p.C >= 4 * p.splits * kF32Warps * kF32Ahead && tiles * q.NB * p.splits * 2 <= ctx->num_sms * 7 / 2)
         p.splits *= 2;
     p.per_split           = (p.C + p.splits - 1) / p.splits;
     const size_t smem     = (size_t)kF32Warps * 2 * kF32Cols * sizeof(float);
