@@ -81,7 +81,8 @@ template <bool BF16, int NT, bool SHIFT>
 __global__ void __launch_bounds__(few_threads(SHIFT)) gated_rows_kernel(const __grid_constant__ FewParams p)
 {
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t bar_full[kFewMaxStages];
+    __shared__ __align__(8) uint64_t bar_full[kFewMaxStages];                  // a stage's copies; SHIFT: its weights, made by the loaders
+    __shared__ __align__(8) uint64_t bar_rows[SHIFT ? kFewMaxStages : 1];      // SHIFT: the copies of a's rows
     __shared__ __align__(8) uint64_t bar_empty[kFewMaxStages];
     __shared__ int gave_up;
 
@@ -97,7 +98,9 @@ __global__ void __launch_bounds__(few_threads(SHIFT)) gated_rows_kernel(const __
     {
         for (int s = 0; s < p.num_stages; s++)
         {
-            ptx::mbar_init(ptx::smem_u32(&bar_full[s]), 1 + (SHIFT ? kFewLoaders / 2 : 0));
+            ptx::mbar_init(ptx::smem_u32(&bar_full[s]), SHIFT ? kFewLoaders / 2 : 1);
+            if (SHIFT)
+                ptx::mbar_init(ptx::smem_u32(&bar_rows[s]), 1);
             ptx::mbar_init(ptx::smem_u32(&bar_empty[s]), kFewWarps);
         }
         ptx::fence_barrier_init();
@@ -123,6 +126,7 @@ __global__ void __launch_bounds__(few_threads(SHIFT)) gated_rows_kernel(const __
     {
         if (lane == 0)
         {
+            uint64_t* const bar_copies = SHIFT ? bar_rows : bar_full;
             bool ok = true;
             int i = 0, s = 0;
             uint32_t phase = 0;
@@ -133,7 +137,7 @@ __global__ void __launch_bounds__(few_threads(SHIFT)) gated_rows_kernel(const __
                     ok = false;
                     break;
                 }
-                const uint32_t full = ptx::smem_u32(&bar_full[s]);
+                const uint32_t full = ptx::smem_u32(&bar_copies[s]);
                 const uint32_t sW   = smem_base + (uint32_t)(s * p.stage_bytes), sX = sW + kFewWBytes;
                 ptx::mbar_arrive_expect_tx(full, (uint32_t)(p.stage_bytes - (SHIFT ? kFewWBytes : 0)));
                 const int k = (first + i) * kFewStageK;
@@ -155,12 +159,11 @@ __global__ void __launch_bounds__(few_threads(SHIFT)) gated_rows_kernel(const __
                 }
             }
             if (!ok)
-            {
                 atomicOr(p.status, TB200_DEV_TIMEOUT);
-                // copies in flight land before the block leaves
-                for (int j = max(0, i - p.num_stages); j < i; j++)
-                    ptx::mbar_wait_bounded(ptx::smem_u32(&bar_full[j % p.num_stages]), (uint32_t)(j / p.num_stages) & 1u, ptx::kDrainCycles);
-            }
+            // Copies in flight land before the block leaves, whichever role may have given up on them.  (Nothing but copies counts on these
+            // barriers, and a block whose roles all go on waits for them anyway.)
+            for (int j = max(0, i - p.num_stages); j < i; j++)
+                ptx::mbar_wait_bounded(ptx::smem_u32(&bar_copies[j % p.num_stages]), (uint32_t)(j / p.num_stages) & 1u, ptx::kDrainCycles);
         }
     }
     else if (SHIFT && warp > kFewWarps)
@@ -238,7 +241,8 @@ __global__ void __launch_bounds__(few_threads(SHIFT)) gated_rows_kernel(const __
         uint32_t phase = 0;
         for (int i = 0; i < mine; i++)
         {
-            ok = ptx::mbar_wait_bounded(ptx::smem_u32(&bar_full[s]), phase, p.wait_limit);
+            ok = ptx::mbar_wait_bounded(ptx::smem_u32(&bar_full[s]), phase, p.wait_limit) &&
+                 (!SHIFT || ptx::mbar_wait_bounded(ptx::smem_u32(&bar_rows[s]), phase, p.wait_limit));
             ok = __all_sync(0xffffffffu, ok);
             if (!ok)
                 break;
