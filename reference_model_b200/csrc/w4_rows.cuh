@@ -307,12 +307,11 @@ __global__ void __launch_bounds__(kRowsThreads, rows_blocks_sm(NT)) w4_rows_kern
                 }
             }
             if (!ok)
-            {
                 atomicOr(p.status, TB200_DEV_TIMEOUT);
-                // copies in flight land before the block leaves
-                for (int j = max(0, i - p.num_stages); j < i; j++)
-                    ptx::mbar_wait_bounded(ptx::smem_u32(&bar_full[j % p.num_stages]), (uint32_t)(j / p.num_stages) & 1u, ptx::kDrainCycles);
-            }
+            // Copies in flight land before the block leaves, whichever role may have given up on them.  (A block whose roles all go on waits
+            // for them anyway.)
+            for (int j = max(0, i - p.num_stages); j < i; j++)
+                ptx::mbar_wait_bounded(ptx::smem_u32(&bar_full[j % p.num_stages]), (uint32_t)(j / p.num_stages) & 1u, ptx::kDrainCycles);
         }
     }
     else if (warp > kRowsWarps)

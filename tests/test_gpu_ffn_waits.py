@@ -46,6 +46,22 @@ def gated(ctx, kernel, nb, h, c, w):
     return Call(ctx, kernel, lambda: ctx.matmul_gated(*ts, out, "RELU"), [out], [ref], ts)
 
 
+def four(ctx, kernel, h, c, w, mats):
+    a = whole(4, "fp16", -1, 2, 1, h, c)
+    r = np.random.default_rng(5)
+    ops, projections, held = [], [], [put(ctx, a)]
+    for _ in range(mats):
+        d = r.integers(0, 256, size=(w, (c + 31) // 32 * 16)).astype(np.uint8)
+        q = torch.from_numpy(np.stack([d & 15, d >> 4], axis=2).reshape(w, -1)[:, :c].astype(np.float32))
+        projections.append(product64(a, torch.where(q > 7, q - 16, q).t()))
+        ops.append(tb.W4(ctx.from_numpy(d), put(ctx, torch.ones((-(-c // 64), w), dtype=torch.float16)), None, 64))
+        held += [ops[-1].data, ops[-1].scale]
+    out = blank(ctx, "fp32", (1, h, w))
+    if mats == 2:
+        return Call(ctx, kernel, lambda: ctx.matmul_gated_w4(held[0], *ops, out, "RELU"), [out], [(projections[0].clamp(min=0) * projections[1]).cpu()], held)
+    return Call(ctx, kernel, lambda: ctx.matmul_w4(held[0], ops[0], out), [out], [projections[0].cpu()], held)
+
+
 # More stages of K to a block than its ring holds, so that copies are asked for in the middle of a call, and fewer, so that all are on their way
 # before the first has been used.
 CALLS = {
@@ -53,6 +69,10 @@ CALLS = {
     "gated, few rows, a short ring": lambda ctx: gated(ctx, "gated_rows_f16", 1, 20, 200, 640),
     "gated, few rows at any element": lambda ctx: gated(ctx, "gated_rows_f16", 1, 3, 2500, 9601),
     "gated, few rows at any element, a short ring": lambda ctx: gated(ctx, "gated_rows_f16", 2, 9, 250, 203),
+    "4 bits, one row": lambda ctx: four(ctx, "matmul_w4_rows", 1, 8192, 12000, 1),
+    "4 bits, one row, a stage a block": lambda ctx: four(ctx, "matmul_w4_rows", 1, 2048, 1000, 1),
+    "4 bits, 30 rows": lambda ctx: four(ctx, "matmul_w4_rows", 30, 4096, 12000, 1),
+    "4 bits, gated": lambda ctx: four(ctx, "gated_w4_rows", 5, 4096, 6001, 2),
 }
 
 
