@@ -439,13 +439,15 @@ __global__ void __launch_bounds__((Shape<PAIR, W4, W4 && EPI == EPI_GATED>::kThr
     constexpr int kSub    = S::kSub, kStage = S::kStage, kHalf = S::kCols / 2, kStages = S::kStages, kThreads = S::kThreads;
     extern __shared__ uint8_t smem_raw[];
     // identical layout in both CTAs of a pair: remote signals address a barrier by its offset
-    __shared__ __align__(8) uint64_t bar_full[kStages];     // used in the first CTA: bytes of both CTAs, values of 4-bit weights in place
+    __shared__ __align__(8) uint64_t bar_full[kStages];     // used in the first CTA: bytes of both CTAs (4-bit weights: values in place)
     __shared__ __align__(8) uint64_t bar_empty[kStages];    // per CTA: stage consumed by the MMAs
     __shared__ __align__(8) uint64_t bar_tmem_full[2];         // per CTA: accumulator buffer complete
     __shared__ __align__(8) uint64_t bar_tmem_empty[2];        // first CTA: buffer drained by both CTAs' epilogues
     __shared__ __align__(8) uint64_t bar_ready;                // first CTA: tensor memory taken in both
     __shared__ __align__(8) uint64_t bar_drain;                // first CTA: MMAs in flight when the issuer gives up
-    __shared__ __align__(8) uint64_t bar_raw[W4 ? kStages : 1];         // per CTA: 4-bit weights of the stage
+    __shared__ __align__(8) uint64_t bar_raw[W4 ? kStages : 1];         // per CTA: 4-bit weights and rows of A of the stage
+    __shared__ int gave_up;                                    // a role of this CTA or of the pair's other one
+    __shared__ long long stages_issued;                        // per CTA: stages whose copies were asked for
     __shared__ uint32_t tmem_base_holder;
     __shared__ float stages[kEpiWarps][32 * 17];    // of the epilogue's warps
 
@@ -464,7 +466,7 @@ __global__ void __launch_bounds__((Shape<PAIR, W4, W4 && EPI == EPI_GATED>::kThr
     {
         for (int s = 0; s < kStages; s++)
         {
-            ptx::mbar_init(ptx::smem_u32(&bar_full[s]), 1 + (W4 ? 4 * S::kCtas : 0));    // (and a group's warps)
+            ptx::mbar_init(ptx::smem_u32(&bar_full[s]), W4 ? 4 * S::kCtas : 1);    // a group's warps of each CTA, or copies
             ptx::mbar_init(ptx::smem_u32(&bar_empty[s]), 1);
             if (W4)
                 ptx::mbar_init(ptx::smem_u32(&bar_raw[s]), 1);
@@ -476,6 +478,8 @@ __global__ void __launch_bounds__((Shape<PAIR, W4, W4 && EPI == EPI_GATED>::kThr
         }
         ptx::mbar_init(ptx::smem_u32(&bar_drain), 1);
         ptx::mbar_init(ptx::smem_u32(&bar_ready), S::kCtas);
+        gave_up       = 0;
+        stages_issued = 0;
         ptx::fence_barrier_init();
         ptx::prefetch_tmap(&p.tmA);
         ptx::prefetch_tmap(&p.tmB0);
@@ -513,6 +517,13 @@ __global__ void __launch_bounds__((Shape<PAIR, W4, W4 && EPI == EPI_GATED>::kThr
     // A product beside the one before it reads what came before both: that one let this in behind its own wait, so it is there.
     if (!p.beside)
         ptx::dep_launch_wait();
+    // a role that gives up says so in every CTA of the tile
+    auto give_up = [&]() {
+        atomicOr(p.status, TB200_DEV_TIMEOUT);
+        gave_up = 1;
+        if (PAIR)
+            asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(ptx::map_to_cta(ptx::smem_u32(&gave_up), rank ^ 1u)), "r"(1) : "memory");
+    };
     uint32_t tmem_base = 0;
     if (warp != 0)
     {
@@ -550,7 +561,7 @@ __global__ void __launch_bounds__((Shape<PAIR, W4, W4 && EPI == EPI_GATED>::kThr
             int stage      = 0;
             uint32_t phase = 0;
             bool ok        = true;
-            int64_t issued = 0;
+            long long issued = 0;
             for (int tile = cluster_id; tile < p.num_tiles && ok; tile += num_clusters)
             {
                 const Tile t          = decode<EPI, PAIR>(p, tile);
@@ -567,10 +578,13 @@ __global__ void __launch_bounds__((Shape<PAIR, W4, W4 && EPI == EPI_GATED>::kThr
                     }
                     const int nch             = min(kSub, left);
                     const uint32_t full_local = ptx::smem_u32(&bar_full[stage]);
-                    // the first CTA arms the barrier with the bytes of both CTAs; each CTA's copies report there
-                    if (rank == 0)
-                        ptx::mbar_arrive_expect_tx(full_local, (uint32_t)(nch * (W4 ? 1 : 2) * S::kCtas * kChunk));
-                    const uint32_t full_first = PAIR ? ptx::map_to_cta(full_local, 0) : full_local;
+                    // the first CTA arms the barrier with the bytes of both CTAs; each CTA's copies report there.  4-bit weights: copies report to
+                    // their own CTA, whose groups wait for them and then report.
+                    if (W4)
+                        ptx::mbar_arrive_expect_tx(ptx::smem_u32(&bar_raw[stage]), kChunk + kRawBytes);
+                    else if (rank == 0)
+                        ptx::mbar_arrive_expect_tx(full_local, (uint32_t)(nch * 2 * S::kCtas * kChunk));
+                    const uint32_t full_first = W4 ? ptx::smem_u32(&bar_raw[stage]) : PAIR ? ptx::map_to_cta(full_local, 0) : full_local;
                     const uint32_t sA         = smem_base + (uint32_t)(stage * kStage);
                     const uint32_t sB         = sA + (uint32_t)(kSub * kChunk);
                     for (int j = 0; j < nch; j++, c++)
@@ -579,7 +593,7 @@ __global__ void __launch_bounds__((Shape<PAIR, W4, W4 && EPI == EPI_GATED>::kThr
                         const int k       = (c - ph * p.chunks) * 64;
                         const uint32_t dA = sA + (uint32_t)(j * kChunk), dB = sB + (uint32_t)(j * kChunk);
                         auto load = [&](uint32_t dst, const CUtensorMap* m, int c0, int c1, int c2) {
-                            if (PAIR)
+                            if (PAIR && !W4)
                                 ptx::tma_load_3d_pair(dst, m, full_first, c0, c1, c2);
                             else
                                 ptx::tma_load_3d(dst, m, full_first, c0, c1, c2);
@@ -594,11 +608,9 @@ __global__ void __launch_bounds__((Shape<PAIR, W4, W4 && EPI == EPI_GATED>::kThr
                         if (W4)
                         {
                             // where their values will be
-                            const uint32_t raw = ptx::smem_u32(&bar_raw[stage]);
-                            ptx::mbar_arrive_expect_tx(raw, kRawBytes);
-                            ptx::tma_load_2d(dB, EPI != EPI_PLAIN && rank ? &p.tmB1 : &p.tmB0, raw, c * 32, n0);
+                            ptx::tma_load_2d(dB, EPI != EPI_PLAIN && rank ? &p.tmB1 : &p.tmB0, full_first, c * 32, n0);
                             if (EPI != EPI_PLAIN && !PAIR)
-                                ptx::tma_load_2d(dB + kRawBytes / 2, &p.tmB1, raw, c * 32, n0);
+                                ptx::tma_load_2d(dB + kRawBytes / 2, &p.tmB1, full_first, c * 32, n0);
                             continue;
                         }
                         if (EPI != EPI_PLAIN && !PAIR)
@@ -625,20 +637,9 @@ __global__ void __launch_bounds__((Shape<PAIR, W4, W4 && EPI == EPI_GATED>::kThr
                     }
                 }
             }
+            stages_issued = issued;
             if (!ok)
-            {
-                atomicOr(p.status, TB200_DEV_TIMEOUT);
-                // the pair's copies in flight land before either CTA leaves (all of them report to the first CTA, which may have given up on a
-                // stage that the second has asked for)
-                if (rank == 0)
-                    for (int64_t i = max((int64_t)0, issued - kStages); i < issued; i++)
-                        ptx::mbar_wait_bounded(ptx::smem_u32(&bar_full[i % kStages]), (uint32_t)(i / kStages) & 1u, ptx::kDrainCycles);
-                if (W4)
-                    for (int64_t i = max((int64_t)0, issued - kStages); i < issued; i++)
-                        ptx::mbar_wait_bounded(ptx::smem_u32(&bar_raw[i % kStages]), (uint32_t)(i / kStages) & 1u, ptx::kDrainCycles);
-                if (PAIR)
-                    ptx::settle();
-            }
+                give_up();
         }
     }
     else if (warp == 1)
@@ -726,14 +727,7 @@ __global__ void __launch_bounds__((Shape<PAIR, W4, W4 && EPI == EPI_GATED>::kThr
                     acc_phase ^= 1u;
             }
             if (!ok)
-            {
-                atomicOr(p.status, TB200_DEV_TIMEOUT);
-                if (PAIR)
-                    ptx::mma_commit_pair(ptx::smem_u32(&bar_drain), 1);
-                else
-                    ptx::mma_commit(ptx::smem_u32(&bar_drain));
-                ptx::mbar_wait_bounded(ptx::smem_u32(&bar_drain), 0, ptx::kDrainCycles);
-            }
+                give_up();
         }
     }
     else if (W4 && warp >= 2 + kEpiWarps)
@@ -845,7 +839,7 @@ __global__ void __launch_bounds__((Shape<PAIR, W4, W4 && EPI == EPI_GATED>::kThr
             }
         }
         if (!ok && lane == 0)
-            atomicOr(p.status, TB200_DEV_TIMEOUT);
+            give_up();
         if (bad)
             atomicOr(p.status, TB200_DEV_UNPREDICTABLE);
     }
@@ -926,7 +920,7 @@ __global__ void __launch_bounds__((Shape<PAIR, W4, W4 && EPI == EPI_GATED>::kThr
                 acc_phase ^= 1u;
         }
         if (!ok && lane == 0)
-            atomicOr(p.status, TB200_DEV_TIMEOUT);
+            give_up();
     }
 
     if (!PAIR && p.splits > 1)
@@ -981,6 +975,46 @@ __global__ void __launch_bounds__((Shape<PAIR, W4, W4 && EPI == EPI_GATED>::kThr
     __syncthreads();
     if (PAIR)
         ptx::cluster_sync();
+    if (gave_up)
+    {
+        // A role gave up (both CTAs of a pair know by now): MMAs and copies that are on their way are waited for, whoever has issued them.
+        if (warp == 1 && lane == 0 && rank == 0)
+        {
+            if (PAIR)
+                ptx::mma_commit_pair(ptx::smem_u32(&bar_drain), 1);
+            else
+                ptx::mma_commit(ptx::smem_u32(&bar_drain));
+            ptx::mbar_wait_bounded(ptx::smem_u32(&bar_drain), 0, ptx::kDrainCycles);
+        }
+        if (threadIdx.x == 0 && (W4 || rank == 0))
+        {
+            const long long mine = stages_issued;
+            long long all        = mine;
+            if (PAIR && !W4)
+            {
+                // One CTA may have asked for stages that the other has not.  Their barriers still count its bytes: armed for them where this
+                // CTA has not armed them, less the bytes that will not come where it has.
+                long long other;
+                asm volatile("ld.shared::cluster.b64 %0, [%1];" : "=l"(other) : "r"(ptx::map_to_cta(ptx::smem_u32(&stages_issued), 1)) : "memory");
+                all             = max(mine, other);
+                const int per   = (total + kSub - 1) / kSub;    // stages of a tile
+                for (long long i = min(mine, other); i < all; i++)
+                {
+                    const uint32_t full  = ptx::smem_u32(&bar_full[i % kStages]);
+                    const uint32_t bytes = (uint32_t)(min(kSub, total - (int)(i % per) * kSub) * 2 * kChunk);    // of one CTA
+                    if (other > mine)
+                        ptx::mbar_arrive_expect_tx(full, bytes);
+                    else
+                        ptx::mbar_complete_tx(full, bytes);
+                }
+            }
+            for (long long i = max(0LL, all - kStages); i < all; i++)
+                ptx::mbar_wait_bounded(ptx::smem_u32(W4 ? &bar_raw[i % kStages] : &bar_full[i % kStages]), (uint32_t)(i / kStages) & 1u, ptx::kDrainCycles);
+        }
+        __syncthreads();
+        if (PAIR)
+            ptx::cluster_sync();
+    }
     if (warp == 1)
     {
         ptx::tc_fence_after_sync();

@@ -93,13 +93,10 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint32_t bar, uint32_t parity,
 // What a role waits for after it has given up: copies and MMAs that are on their way land within microseconds, whatever the limit above is.
 constexpr long long kDrainCycles = 1 << 22;
 
-// ... and where their arrival cannot be seen (the other CTA's barrier): time in which they land
-__device__ __forceinline__ void settle()
+// Bytes that an mbarrier of this CTA waits for and no copy will bring
+__device__ __forceinline__ void mbar_complete_tx(uint32_t bar, uint32_t bytes)
 {
-    const long long t0 = clock64();
-    while (clock64() - t0 < (1 << 17))
-    {
-    }
+    asm volatile("mbarrier.complete_tx.relaxed.cluster.shared::cluster.b64 [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
 
 // ---------------------------------------------------------------- programmatic dependent launch

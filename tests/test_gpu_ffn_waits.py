@@ -62,6 +62,18 @@ def four(ctx, kernel, h, c, w, mats):
     return Call(ctx, kernel, lambda: ctx.matmul_w4(held[0], ops[0], out), [out], [projections[0].cpu()], held)
 
 
+def backward(ctx, nb, h, c, w):
+    # a few columns of `a`: dG and dU are whole numbers below 256, exact in bf16
+    a, bg, bu, d = whole(6, "bf16", 0, 2, nb, h, c), whole(7, "bf16", -1, 2, nb, c, w), whole(8, "bf16", -1, 2, nb, c, w), whole(9, "bf16", -1, 2, nb, h, w)
+    a[:, :, 8:] = 0
+    ts = [put(ctx, t) for t in (a, bg, bu, d)]
+    grads = [blank(ctx, "fp32", tuple(t.shape)) for t in (a, bg, bu)]
+    G, U = product64(a, bg), product64(a, bu)
+    dG, dU = d.cuda() * U * (G > 0), d.cuda() * G.clamp(min=0)
+    refs = [product64(dG, bg.transpose(1, 2)) + product64(dU, bu.transpose(1, 2)), product64(a.transpose(1, 2), dG), product64(a.transpose(1, 2), dU)]
+    return Call(ctx, "gated_backward_pair_f16", lambda: ctx.matmul_gated_backward(*ts, *grads, activation="RELU"), grads, [r.cpu() for r in refs], ts)
+
+
 # More stages of K to a block than its ring holds, so that copies are asked for in the middle of a call, and fewer, so that all are on their way
 # before the first has been used.
 CALLS = {
@@ -73,6 +85,16 @@ CALLS = {
     "4 bits, one row, a stage a block": lambda ctx: four(ctx, "matmul_w4_rows", 1, 2048, 1000, 1),
     "4 bits, 30 rows": lambda ctx: four(ctx, "matmul_w4_rows", 30, 4096, 12000, 1),
     "4 bits, gated": lambda ctx: four(ctx, "gated_w4_rows", 5, 4096, 6001, 2),
+    "pairs": lambda ctx: gated(ctx, "gated_pair_f16", 1, 1500, 2000, 2500),
+    "pairs, one stage": lambda ctx: gated(ctx, "gated_pair_f16", 1, 3000, 100, 2500),
+    "CTAs by themselves": lambda ctx: gated(ctx, "gated_pair_f16", 3, 150, 500, 300),
+    "K over clusters": lambda ctx: gated(ctx, "gated_pair_f16", 1, 100, 4000, 72),
+    "4 bits, pairs": lambda ctx: four(ctx, "matmul_w4_pair", 777, 4096, 4096, 1),
+    "4 bits, K over clusters": lambda ctx: four(ctx, "matmul_w4_pair", 100, 4000, 300, 1),
+    "4 bits, gated, pairs": lambda ctx: four(ctx, "gated_w4_pair", 700, 2000, 2100, 2),
+    "4 bits, gated, CTAs by themselves": lambda ctx: four(ctx, "gated_w4_pair", 90, 2000, 200, 2),
+    "gradients": lambda ctx: backward(ctx, 1, 1700, 1000, 1290),
+    "gradients, small": lambda ctx: backward(ctx, 2, 130, 72, 200),
 }
 
 
