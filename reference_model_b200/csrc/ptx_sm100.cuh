@@ -419,9 +419,11 @@ __device__ __forceinline__ uint32_t cluster_ctarank()
     return r;
 }
 
-// Full barrier over all threads of the cluster (release / acquire).
+// Full barrier over all threads of the cluster (release / acquire).  The aligned forms want the whole warp at the instruction together, which a branch or
+// a loop before it that only some lanes took does not give by itself.
 __device__ __forceinline__ void cluster_sync()
 {
+    __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
@@ -430,11 +432,13 @@ __device__ __forceinline__ void cluster_sync()
 // between them.
 __device__ __forceinline__ void cluster_arrive()
 {
+    __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
 }
 
 __device__ __forceinline__ void cluster_wait()
 {
+    __syncwarp();
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
