@@ -11,20 +11,44 @@ namespace tb200
 namespace ffn
 {
 
-// Value of the activation.  The logistic forms divide by 1 + exp(-x), which neither cancels nor overflows to NaN for a finite x;
-// the Gaussian one goes through erfc, whose relative error stays small in the left tail where 1 + erf would cancel.
+// The logistic forms go through e = exp(-|x|): s(x) = 1 / (1 + e) or e / (1 + e) and s(x) s(-x) = e / (1 + e)^2 neither cancel nor overflow on either
+// side (1 - s has no digits left from x = 17 on).  The Gaussian one goes through erfc, whose relative error stays small in the left tail where
+// 1 + erf would cancel.
+struct Logistic
+{
+    float s, product;    // s(x), s(x) s(-x)
+};
+
+__device__ __forceinline__ Logistic logistic(float x, float e, float reciprocal)
+{
+    return { (x < 0.f ? e : 1.f) * reciprocal, e * reciprocal * reciprocal };
+}
+
+__device__ __forceinline__ Logistic logistic(float x)
+{
+    const float e = expf(-fabsf(x));
+    return logistic(x, e, 1.f / (1.f + e));
+}
+
+// what GELU_TANH gives to it: (1 + tanh(y)) / 2 = s(2 y)
+__device__ __forceinline__ float tanh_argument(float g)
+{
+    return 1.5957691216057308f * (g + 0.044715f * g * g * g);
+}
+
+// Value of the activation.
 template <int ACT>
 __device__ __forceinline__ float act_value(float g)
 {
     if (ACT == TB200_ACT_SILU)
-        return g / (1.f + expf(-g));
+        return g * logistic(g).s;
     if (ACT == TB200_ACT_GELU)
         return 0.5f * g * erfcf(-0.70710678118654752f * g);
     if (ACT == TB200_ACT_GELU_TANH)
-        return g / (1.f + expf(-1.5957691216057308f * (g + 0.044715f * g * g * g)));    // (1 + tanh(y)) / 2 = 1 / (1 + exp(-2 y))
+        return g * logistic(tanh_argument(g)).s;
     if (ACT == TB200_ACT_RELU)
         return g < 0.f ? 0.f : g;    // a NaN stays one
-    return 1.f / (1.f + expf(-g));
+    return logistic(g).s;
 }
 
 // 1 + 3 * 0.044715 g^2 of GELU_TANH's derivative.  Where s (1 - s) has long been 0 the square must not overflow beside it.
@@ -34,27 +58,27 @@ __device__ __forceinline__ float tanh_growth(float g)
     return 1.f + 0.134145f * c * c;
 }
 
+// Value and derivative of a logistic form
+template <int ACT>
+__device__ __forceinline__ void logistic_slope(float g, const Logistic& l, float& value, float& slope)
+{
+    value = ACT == TB200_ACT_SIGMOID ? l.s : g * l.s;
+    slope = ACT == TB200_ACT_SIGMOID ? l.product
+            : ACT == TB200_ACT_SILU  ? l.s + g * l.product
+                                     : l.s + g * l.product * 1.5957691216057308f * tanh_growth(g);
+}
+
 // Value and derivative.
 template <int ACT>
 __device__ __forceinline__ void act_slope(float g, float& value, float& slope)
 {
-    if (ACT == TB200_ACT_SILU || ACT == TB200_ACT_SIGMOID)
-    {
-        const float s = 1.f / (1.f + expf(-g));
-        value         = ACT == TB200_ACT_SILU ? g * s : s;
-        slope         = ACT == TB200_ACT_SILU ? s * (1.f + g * (1.f - s)) : s * (1.f - s);
-    }
+    if (ACT == TB200_ACT_SILU || ACT == TB200_ACT_SIGMOID || ACT == TB200_ACT_GELU_TANH)
+        logistic_slope<ACT>(g, logistic(ACT == TB200_ACT_GELU_TANH ? tanh_argument(g) : g), value, slope);
     else if (ACT == TB200_ACT_GELU)
     {
         const float p = 0.5f * erfcf(-0.70710678118654752f * g);
         value         = g * p;
         slope         = p + g * (0.39894228040143268f * expf(-0.5f * g * g));
-    }
-    else if (ACT == TB200_ACT_GELU_TANH)
-    {
-        const float s = 1.f / (1.f + expf(-1.5957691216057308f * (g + 0.044715f * g * g * g)));
-        value         = g * s;
-        slope         = s + g * s * (1.f - s) * 1.5957691216057308f * tanh_growth(g);
     }
     else
     {
@@ -72,15 +96,21 @@ __device__ __forceinline__ float erfc_positive(float x, float e)
     return t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f) * e;
 }
 
+__device__ __forceinline__ Logistic logistic_16(float x)
+{
+    const float e = __expf(-fabsf(x));
+    return logistic(x, e, __fdividef(1.f, 1.f + e));
+}
+
 template <int ACT>
 __device__ __forceinline__ float act_value_16(float g)
 {
     if (ACT == TB200_ACT_SILU)
-        return __fdividef(g, 1.f + __expf(-g));
+        return g * logistic_16(g).s;
     if (ACT == TB200_ACT_GELU_TANH)
-        return __fdividef(g, 1.f + __expf(-1.5957691216057308f * (g + 0.044715f * g * g * g)));
+        return g * logistic_16(tanh_argument(g)).s;
     if (ACT == TB200_ACT_SIGMOID)
-        return __fdividef(1.f, 1.f + __expf(-g));
+        return logistic_16(g).s;
     if (ACT == TB200_ACT_GELU)
     {
         const float tail = 0.5f * erfc_positive(0.70710678118654752f * fabsf(g), __expf(-0.5f * g * g));
@@ -92,12 +122,8 @@ __device__ __forceinline__ float act_value_16(float g)
 template <int ACT>
 __device__ __forceinline__ void act_slope_16(float g, float& value, float& slope)
 {
-    if (ACT == TB200_ACT_SILU || ACT == TB200_ACT_SIGMOID)
-    {
-        const float s = __fdividef(1.f, 1.f + __expf(-g));
-        value         = ACT == TB200_ACT_SILU ? g * s : s;
-        slope         = ACT == TB200_ACT_SILU ? s * (1.f + g * (1.f - s)) : s * (1.f - s);
-    }
+    if (ACT == TB200_ACT_SILU || ACT == TB200_ACT_SIGMOID || ACT == TB200_ACT_GELU_TANH)
+        logistic_slope<ACT>(g, logistic_16(ACT == TB200_ACT_GELU_TANH ? tanh_argument(g) : g), value, slope);
     else if (ACT == TB200_ACT_GELU)
     {
         const float e    = __expf(-0.5f * g * g);
@@ -105,12 +131,6 @@ __device__ __forceinline__ void act_slope_16(float g, float& value, float& slope
         const float p    = g < 0.f ? tail : 1.f - tail;
         value            = g * p;
         slope            = p + g * (0.39894228040143268f * e);
-    }
-    else if (ACT == TB200_ACT_GELU_TANH)
-    {
-        const float s = __fdividef(1.f, 1.f + __expf(-1.5957691216057308f * (g + 0.044715f * g * g * g)));
-        value         = g * s;
-        slope         = s + g * s * (1.f - s) * 1.5957691216057308f * tanh_growth(g);
     }
     else
         act_slope<ACT>(g, value, slope);
