@@ -88,12 +88,22 @@ __device__ __forceinline__ void act_slope(float g, float& value, float& slope)
 }
 
 // The same for results that are rounded to 16 bits: exp by the hardware's power of two (relative error about 2^-21 |x|), quotients by its
-// reciprocal, and the Gaussian's tail by Abramowitz and Stegun's 7.1.26, erfc(x) = t (a1 + t (a2 + ...)) exp(-x^2), t = 1 / (1 + p x), within 1.5e-7.
+// reciprocal, and the Gaussian's tail by a polynomial: erfc(x) = t (c0 + c1 t + ... + c7 t^7) exp(-x^2) with t = 1 / (1 + 0.44 x), the coefficients
+// fitted to erfc(x) exp(x^2) / t over all x >= 0 by weighted least squares (Lawson's iteration).  Within 3.2e-8 of erfc for small x and 6.2e-6 of its value
+// for all, which a bound on the difference alone does not give: f(-6) is 1e-9, and the next factor may be large.
 // An epilogue of the CTA-pair kernel took 9000 cycles for 64 values a thread with the functions above, 2100 to 2900 with these.
 __device__ __forceinline__ float erfc_positive(float x, float e)
 {
-    const float t = __fdividef(1.f, fmaf(0.3275911f, x, 1.f));
-    return t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f) * e;
+    const float t = __fdividef(1.f, fmaf(0.44f, x, 1.f));
+    float c       = 0.0631131908f;
+    c             = fmaf(c, t, -0.244836184f);
+    c             = fmaf(c, t, 0.241915805f);
+    c             = fmaf(c, t, 0.0266969014f);
+    c             = fmaf(c, t, 0.193881295f);
+    c             = fmaf(c, t, 0.222735351f);
+    c             = fmaf(c, t, 0.24824873f);
+    c             = fmaf(c, t, 0.248244942f);
+    return t * c * e;
 }
 
 __device__ __forceinline__ Logistic logistic_16(float x)

@@ -84,7 +84,7 @@ def terms(act, g):
     return p + (s - p).abs()
 
 
-@pytest.mark.parametrize("act", [a for a in ACTS if a != "GELU"])
+@pytest.mark.parametrize("act", ACTS)
 @pytest.mark.parametrize("c", (2, 1032))
 @pytest.mark.parametrize("rows", (32, 600))
 @pytest.mark.parametrize("dtype,out", (("bf16", "bf16"), ("fp16", "fp16"), ("bf16", "fp32"), ("fp16", "fp32"), ("fp32", "fp32")))
@@ -103,7 +103,7 @@ def test_values(ctx, act, c, rows, dtype, out, policy):    # noqa: F811
         t.free()
 
 
-@pytest.mark.parametrize("act", [a for a in ACTS if a != "GELU"])
+@pytest.mark.parametrize("act", ACTS)
 @pytest.mark.parametrize("c", (2, 1032))
 @pytest.mark.parametrize("dtype", ("bf16", "fp16", "fp32"))
 @pytest.mark.parametrize("policy", (0, 1))
