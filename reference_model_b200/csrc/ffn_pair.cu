@@ -178,6 +178,12 @@ __device__ __forceinline__ void gate_run(const uint32_t (&g)[16], const uint32_t
         o[i] = act_value_16<ACT>(__uint_as_float(g[i])) * __uint_as_float(u[i]);
 }
 
+// Results that stay in fp32 take CUDA's functions.  A call, so that sixteen copies of them do not cost the other results' code its registers.
+__device__ __noinline__ float act_value_32(int act, float g)
+{
+    return act_value(act, g);
+}
+
 template <int ACT>
 __device__ __forceinline__ void grad_run(const uint32_t (&g)[16], const uint32_t (&u)[16], const float (&d)[16], float (&dg)[16], float (&du)[16])
 {
@@ -250,14 +256,21 @@ __device__ __forceinline__ void finish_run(const Params& p, const Tile& t, int r
     else if (EPI == EPI_GATED)
     {
         float v[16];
-        switch (p.act)
+        if (p.out_dt == TB200_FP32)
         {
-            case TB200_ACT_SILU: gate_run<TB200_ACT_SILU>(g, u, v); break;
-            case TB200_ACT_GELU: gate_run<TB200_ACT_GELU>(g, u, v); break;
-            case TB200_ACT_GELU_TANH: gate_run<TB200_ACT_GELU_TANH>(g, u, v); break;
-            case TB200_ACT_RELU: gate_run<TB200_ACT_RELU>(g, u, v); break;
-            default: gate_run<TB200_ACT_SIGMOID>(g, u, v); break;
+#pragma unroll
+            for (int i = 0; i < 16; i++)
+                v[i] = act_value_32(p.act, __uint_as_float(g[i])) * __uint_as_float(u[i]);
         }
+        else
+            switch (p.act)
+            {
+                case TB200_ACT_SILU: gate_run<TB200_ACT_SILU>(g, u, v); break;
+                case TB200_ACT_GELU: gate_run<TB200_ACT_GELU>(g, u, v); break;
+                case TB200_ACT_GELU_TANH: gate_run<TB200_ACT_GELU_TANH>(g, u, v); break;
+                case TB200_ACT_RELU: gate_run<TB200_ACT_RELU>(g, u, v); break;
+                default: gate_run<TB200_ACT_SIGMOID>(g, u, v); break;
+            }
         emit(p.out0, p.out_dt, v);
     }
     else
@@ -326,7 +339,7 @@ __device__ __forceinline__ void finish_quad(const Params& p, const Tile& t, int 
         float v[4];
 #pragma unroll
         for (int i = 0; i < 4; i++)
-            v[i] = act_value_16(p.act, g[i]) * u[i];
+            v[i] = (p.out_dt == TB200_FP32 ? act_value_32(p.act, g[i]) : act_value_16(p.act, g[i])) * u[i];
         store_quad(p.out0, orow, p.out_dt, n, p.vec, v);
     }
     else
