@@ -344,7 +344,9 @@ extern "C"
      * evaluated again: with G = a x gate, U = a x up, dG = grad_output * U * activation'(G), dU = grad_output * activation(G),
      *   grad_a = dG x gate^T + dU x up^T, grad_gate = a^T x dG, grad_up = a^T x dU,
      * the last two summed over the batches where the weights are shared.  Each gradient has its operand's shape, the operands'
-     * type or FP32, and may be NULL.  In the 16-bit types dG and dU are rounded to that type between the products. */
+     * type or FP32, and may be NULL.  In the 16-bit types dG and dU are rounded to that type between the products, whatever type a
+     * gradient has; in FP16 all of a call's under one power of two where the largest of them is 65520 or more or below 2^-8, so that only
+     * values below 2^-39 of the largest are lost (2^-17 where it lies between). */
     TB200_API tb200_status tb200_matmul_gated_backward(tb200_ctx* ctx, const tb200_tensor* a, const tb200_tensor* gate,
                                                        const tb200_tensor* up, const tb200_tensor* grad_output,
                                                        int32_t activation, tb200_tensor* grad_a, tb200_tensor* grad_gate,

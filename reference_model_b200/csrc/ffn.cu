@@ -132,7 +132,8 @@ tb200_status gated_pair(tb200_ctx* ctx, const GatedProblem& q)
     return TB200_OK;
 }
 
-// Its gradients: dG and dU into scratch (rounded to the operands' type), then one product for grad_a and one for both weights'.
+// Its gradients: dG and dU into scratch (rounded to the operands' type, in FP16 under a power of two where their size calls for one: a second launch sees to
+// that), then one product for grad_a and one for both weights'.
 tb200_status gated_backward_pair(tb200_ctx* ctx, const GatedProblem& q)
 {
     const int64_t Wp  = round_up(q.W, 16);
@@ -145,6 +146,9 @@ tb200_status gated_backward_pair(tb200_ctx* ctx, const GatedProblem& q)
         void* const pg      = c.take(pad_bytes(q.W, (int64_t)q.NB * q.C));
         void* const pu      = c.take(pad_bytes(q.W, (int64_t)q.NB * q.C));
         uint8_t* const dg   = reinterpret_cast<uint8_t*>(c.take(2 * half));
+        const bool f16      = q.dt == TB200_FP16;
+        float* const peaks  = reinterpret_cast<float*>(c.take(f16 ? (size_t)pair_peaks(ctx) * sizeof(float) : 0));
+        float* const undo   = reinterpret_cast<float*>(c.take(f16 ? sizeof(float) : 0));
         if (!pass)
         {
             TB200_TRY(ensure_scratch(ctx, size.used));
@@ -178,7 +182,15 @@ tb200_status gated_backward_pair(tb200_ctx* ctx, const GatedProblem& q)
         k.out_dt[0] = k.out_dt[1] = q.dt;
         k.ld      = Wp;
         k.name    = "gated_backward_pair_f16";
+        k.peaks   = f16 ? peaks : nullptr;
         TB200_TRY(pair_launch(ctx, k));
+        if (f16)
+        {
+            k.peaks = nullptr;
+            k.seen  = peaks;
+            k.undo  = undo;
+            TB200_TRY(pair_launch(ctx, k));
+        }
         const Matrix d = { dg, q.W, q.H, 2 * (int64_t)q.NB, Wp };
         if (q.da)
         {
@@ -196,6 +208,7 @@ tb200_status gated_backward_pair(tb200_ctx* ctx, const GatedProblem& q)
             k.results   = 1;
             k.out[0]    = q.da;
             k.out_dt[0] = q.da_dt;
+            k.undo      = f16 ? undo : nullptr;
             k.ld        = q.C;
             k.name      = "gated_backward_pair_f16";
             TB200_TRY(pair_launch(ctx, k));
@@ -223,6 +236,7 @@ tb200_status gated_backward_pair(tb200_ctx* ctx, const GatedProblem& q)
             k.out_dt[0] = q.dgate ? q.dgate_dt : q.dup_dt;
             k.out[1]    = k.results == 2 ? q.dup : nullptr;
             k.out_dt[1] = q.dup_dt;
+            k.undo      = f16 ? undo : nullptr;
             k.ld        = q.W;
             k.name      = "gated_backward_pair_f16";
             TB200_TRY(pair_launch(ctx, k));

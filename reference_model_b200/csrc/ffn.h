@@ -91,9 +91,13 @@ struct PairProduct
     const W4Mat* w4;   // in b's place: 4-bit matrices, rows a multiple of 16 bytes apart (PAIR_PLAIN and PAIR_GATED, NB and phases 1)
     int group;
     bool beside;       // reads nothing that the launch of this kind directly before it writes: the two may run side by side
+    float* peaks;        // PAIR_GRAD in FP16: where the launch leaves what its values reach (pair_peaks of them)
+    const float* seen;   // ... a second launch of the same product, which looks at them and evaluates again where they call for a power of two,
+    float* undo;         // ... and leaves what takes it back; PAIR_PLAIN: what results are multiplied by (or null)
     const char* name;
 };
 tb200_status pair_launch(tb200_ctx* ctx, const PairProduct& q);
+int64_t pair_peaks(const tb200_ctx* ctx);
 
 // ---- gated_rows.cu: PAIR_GATED with K across b's rows and few rows of a (weights read once)
 tb200_status gated_rows_launch(tb200_ctx* ctx, const PairProduct& q);

@@ -97,9 +97,33 @@ struct Params
     tb200_dtype scale_dt[2];
     int K, groups;
     uint32_t group32;      // of 32 elements
+    // The power of two under which fp16 holds dG and dU (range_scale).  Gradients, first launch: where each warp leaves the largest it has met;
+    // second: those, and where the other products find what takes the power back.
+    float* peaks;
+    const float* seen;
+    float* undo;
     long long wait_limit;
     int* status;
 };
+
+// fp16 has five bits of exponent: from 65520 on dG and dU would be infinite, and below 2^-14 they lose places.  Where the largest of a call is outside of
+// what fp16 holds well, all are held under the power of two that brings it to 2^14 .. 2^15.  Sums of products with values that small are
+// exact in the power, so gradients come out as if dG and dU had a float's exponent, but for values below 2^-39 of the largest (2^-17 where
+// no power is taken), which become 0.
+__device__ __forceinline__ float range_scale(float peak)
+{
+    if (!(peak >= 65520.f || (peak > 0.f && peak < 0x1p-8f)))
+        return 1.f;
+    const int exponent = max((int)(__float_as_uint(peak) >> 23) - 127, -106);
+    return __uint_as_float((uint32_t)(14 - exponent + 127) << 23);
+}
+
+// (what is not finite stays so under any power)
+__device__ __forceinline__ void note_peak(float& peak, float x)
+{
+    const float v = fabsf(x);
+    peak          = v <= 3.402823466e38f ? fmaxf(peak, v) : peak;
+}
 
 struct Tile
 {
@@ -185,15 +209,15 @@ __device__ __noinline__ float act_value_32(int act, float g)
 }
 
 template <int ACT>
-__device__ __forceinline__ void grad_run(const uint32_t (&g)[16], const uint32_t (&u)[16], const float (&d)[16], float (&dg)[16], float (&du)[16])
+__device__ __forceinline__ void grad_run(const uint32_t (&g)[16], const uint32_t (&u)[16], const float (&d)[16], float scale, float (&dg)[16], float (&du)[16])
 {
 #pragma unroll
     for (int i = 0; i < 16; i++)
     {
         float value, slope;
         act_slope_16<ACT>(__uint_as_float(g[i]), value, slope);
-        dg[i] = d[i] * slope * __uint_as_float(u[i]);    // (the slope is 1.13 at most: only the result itself can overflow)
-        du[i] = d[i] * value;
+        dg[i] = d[i] * slope * __uint_as_float(u[i]) * scale;    // (the slope is 1.13 at most: in fp32 only the product itself can overflow)
+        du[i] = d[i] * value * scale;
     }
 }
 
@@ -202,7 +226,8 @@ __device__ __forceinline__ void grad_run(const uint32_t (&g)[16], const uint32_t
 // of the warp's own) and out sixteen neighbouring columns of two rows at a time (a row a lane, one element at a time, touched 32 sectors with every
 // store: gradients of 6 x 280 x 2758 took 150 us).
 template <int EPI>
-__device__ __forceinline__ void finish_run(const Params& p, const Tile& t, int row, int run, const uint32_t (&g)[16], const uint32_t (&u)[16], float* stage)
+__device__ __forceinline__ void finish_run(const Params& p, const Tile& t, int row, int run, const uint32_t (&g)[16], const uint32_t (&u)[16], float* stage,
+                                           float scale, float& peak)
 {
     const int m = t.m0 + row, col = t.n0 + run, n = min(16, p.cols - col);
     const bool valid = m < p.rows, together = p.vec == 0;
@@ -250,7 +275,7 @@ __device__ __forceinline__ void finish_run(const Params& p, const Tile& t, int r
         float v[16];
 #pragma unroll
         for (int i = 0; i < 16; i++)
-            v[i] = __uint_as_float(g[i]);
+            v[i] = __uint_as_float(g[i]) * scale;
         emit(t.idx < p.NB ? p.out0 : p.out1, t.idx < p.NB ? p.out_dt : p.out1_dt, v);
     }
     else if (EPI == EPI_GATED)
@@ -297,11 +322,20 @@ __device__ __forceinline__ void finish_run(const Params& p, const Tile& t, int r
         }
         switch (p.act)
         {
-            case TB200_ACT_SILU: grad_run<TB200_ACT_SILU>(g, u, d, dg, du); break;
-            case TB200_ACT_GELU: grad_run<TB200_ACT_GELU>(g, u, d, dg, du); break;
-            case TB200_ACT_GELU_TANH: grad_run<TB200_ACT_GELU_TANH>(g, u, d, dg, du); break;
-            case TB200_ACT_RELU: grad_run<TB200_ACT_RELU>(g, u, d, dg, du); break;
-            default: grad_run<TB200_ACT_SIGMOID>(g, u, d, dg, du); break;
+            case TB200_ACT_SILU: grad_run<TB200_ACT_SILU>(g, u, d, scale, dg, du); break;
+            case TB200_ACT_GELU: grad_run<TB200_ACT_GELU>(g, u, d, scale, dg, du); break;
+            case TB200_ACT_GELU_TANH: grad_run<TB200_ACT_GELU_TANH>(g, u, d, scale, dg, du); break;
+            case TB200_ACT_RELU: grad_run<TB200_ACT_RELU>(g, u, d, scale, dg, du); break;
+            default: grad_run<TB200_ACT_SIGMOID>(g, u, d, scale, dg, du); break;
+        }
+        if (p.peaks)
+        {
+#pragma unroll
+            for (int i = 0; i < 16; i++)
+            {
+                note_peak(peak, dg[i]);
+                note_peak(peak, du[i]);
+            }
         }
         emit(p.out0, p.out_dt, dg);
         emit(p.out1, p.out_dt, du);
@@ -327,13 +361,16 @@ __device__ __forceinline__ void store_quad(void* base, int64_t at, tb200_dtype d
 
 // The same for four columns, whichever thread has them.
 template <int EPI>
-__device__ __forceinline__ void finish_quad(const Params& p, const Tile& t, int row, int run, const float (&g)[4], const float (&u)[4])
+__device__ __forceinline__ void finish_quad(const Params& p, const Tile& t, int row, int run, const float (&g)[4], const float (&u)[4], float scale, float& peak)
 {
     const int m = t.m0 + row, col = t.n0 + run, n = min(4, p.cols - col);
     const int batch    = t.idx < p.NB ? t.idx : t.idx - p.NB;
     const int64_t orow = ((int64_t)batch * p.rows + m) * p.ld + col;
     if (EPI == EPI_PLAIN)
-        store_quad(t.idx < p.NB ? p.out0 : p.out1, orow, t.idx < p.NB ? p.out_dt : p.out1_dt, n, p.vec, g);
+    {
+        const float v[4] = { g[0] * scale, g[1] * scale, g[2] * scale, g[3] * scale };
+        store_quad(t.idx < p.NB ? p.out0 : p.out1, orow, t.idx < p.NB ? p.out_dt : p.out1_dt, n, p.vec, v);
+    }
     else if (EPI == EPI_GATED)
     {
         float v[4];
@@ -352,8 +389,13 @@ __device__ __forceinline__ void finish_quad(const Params& p, const Tile& t, int 
             const float d = i < n ? load_fp(p.dout, at + i, p.bf16 ? TB200_BF16 : TB200_FP16) : 0.f;
             float value, slope;
             act_slope_16(p.act, g[i], value, slope);
-            dg[i] = d * slope * u[i];
-            du[i] = d * value;
+            dg[i] = d * slope * u[i] * scale;
+            du[i] = d * value * scale;
+            if (p.peaks)
+            {
+                note_peak(peak, dg[i]);
+                note_peak(peak, du[i]);
+            }
         }
         store_quad(p.out0, orow, p.out_dt, n, p.vec, dg);
         store_quad(p.out1, orow, p.out_dt, n, p.vec, du);
@@ -475,6 +517,28 @@ __global__ void __launch_bounds__((Shape<PAIR, W4, W4 && EPI == EPI_GATED>::kThr
     const uint32_t smem_base = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
     float* const red         = reinterpret_cast<float*>(smem_raw + (smem_base - ptx::smem_u32(smem_raw)));    // a share's sums of a tile
 
+    float scale = 1.f, peak = 0.f;
+    if (EPI == EPI_GRAD && p.seen)
+    {
+        // The second launch: nothing is left to do where the first one's values are held well (394 x 1024 x 2048: 2.5 us of 34.8).
+        constexpr int kWarps = kThreads / 32;
+        float* const most    = &stages[0][0];
+        ptx::dep_launch_wait();
+        for (int i = threadIdx.x; i < (int)gridDim.x * kWarps; i += kThreads)
+            peak = fmaxf(peak, __ldcg(p.seen + i));
+        peak = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(peak)));    // (none is negative)
+        if (lane == 0)
+            most[warp] = peak;
+        __syncthreads();
+        for (int i = 0; i < kWarps; i++)
+            peak = fmaxf(peak, most[i]);
+        __syncthreads();
+        scale = range_scale(peak);
+        if (blockIdx.x == 0 && threadIdx.x == 0)
+            *p.undo = 1.f / scale;
+        if (scale == 1.f)
+            return;
+    }
     if (threadIdx.x == 0)
     {
         for (int s = 0; s < kStages; s++)
@@ -530,6 +594,8 @@ __global__ void __launch_bounds__((Shape<PAIR, W4, W4 && EPI == EPI_GATED>::kThr
     // A product beside the one before it reads what came before both: that one let this in behind its own wait, so it is there.
     if (!p.beside)
         ptx::dep_launch_wait();
+    if (EPI == EPI_PLAIN && !W4 && p.undo)
+        scale = __ldcg(p.undo);
     // a role that gives up says so in every CTA of the tile
     auto give_up = [&]() {
         atomicOr(p.status, TB200_DEV_TIMEOUT);
@@ -901,7 +967,7 @@ __global__ void __launch_bounds__((Shape<PAIR, W4, W4 && EPI == EPI_GATED>::kThr
                     uint32_t g[16];
                     ptx::tmem_ld_32x32b_x16(taddr + (uint32_t)(c * 16), g);
                     ptx::tmem_ld_wait_x16(g);
-                    finish_run<EPI>(p, t, (int)rank * 128 + row, c * 16, g, g, stage);
+                    finish_run<EPI>(p, t, (int)rank * 128 + row, c * 16, g, g, stage, scale, peak);
                 }
             }
             else
@@ -915,7 +981,7 @@ __global__ void __launch_bounds__((Shape<PAIR, W4, W4 && EPI == EPI_GATED>::kThr
                     ptx::tmem_ld_32x32b_x16(taddr + (uint32_t)(kHalf + c * 16), u);
                     ptx::tmem_ld_wait_x16(g);
                     ptx::tmem_ld_wait_x16(u);
-                    finish_run<EPI>(p, t, (int)rank * 128 + row, c * 16, g, u, stage);
+                    finish_run<EPI>(p, t, (int)rank * 128 + row, c * 16, g, u, stage, scale, peak);
                 }
             }
             // this warp has read its part of the buffer: one arrival per warp on the first CTA's barrier
@@ -977,7 +1043,7 @@ __global__ void __launch_bounds__((Shape<PAIR, W4, W4 && EPI == EPI_GATED>::kThr
             sum(col, g);
             if (EPI != EPI_PLAIN)
                 sum(kHalf + col, u);
-            finish_quad<EPI>(p, t, r, col, g, u);
+            finish_quad<EPI>(p, t, r, col, g, u, scale, peak);
         }
         ptx::cluster_sync();    // nobody leaves while another share may still read its sums
     }
@@ -986,6 +1052,12 @@ __global__ void __launch_bounds__((Shape<PAIR, W4, W4 && EPI == EPI_GATED>::kThr
     // Neither CTA may leave (or free its TMEM) while the other can still signal it or read its shared memory.
     ptx::tc_fence_before_sync();
     __syncthreads();
+    if (EPI == EPI_GRAD && p.peaks)
+    {
+        peak = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(peak)));
+        if (lane == 0)
+            p.peaks[blockIdx.x * (kThreads / 32) + warp] = peak;
+    }
     if (PAIR)
         ptx::cluster_sync();
     if (gave_up)
@@ -1181,6 +1253,9 @@ tb200_status launch(tb200_ctx* ctx, const PairProduct& q, int splits)
     k.b_desc_hi  = q.b_mn ? ptx::make_smem_desc_hi(8192, 1024, 2) : ptx::make_smem_desc_hi(16, 1024, 2);
     const uint32_t fmt = bf16 ? 1u : 0u;
     k.idesc      = ptx::make_idesc(1u, fmt, fmt, q.a_mn ? 1u : 0u, q.b_mn ? 1u : 0u, (uint32_t)S::kRows, (uint32_t)S::kCols);
+    k.peaks      = q.peaks;
+    k.seen       = q.seen;
+    k.undo       = q.undo;
     k.wait_limit = ctx->wait_limit_cycles;
     k.status     = ctx->d_status;
     int bit      = 0;
@@ -1242,6 +1317,12 @@ tb200_status clusters_at_once(tb200_ctx* ctx, int which, int size, int* n)
 }
 
 }    // namespace
+
+// A warp of a grid each, which has no more CTAs than the device SMs (gradients' launches: no 4-bit weights).
+int64_t pair_peaks(const tb200_ctx* ctx)
+{
+    return (int64_t)std::max(2, ctx->num_sms) * (Shape<true>::kThreads / 32);
+}
 
 tb200_status pair_launch(tb200_ctx* ctx, const PairProduct& q)
 {
