@@ -398,12 +398,6 @@ tb200_status w4_launch(tb200_ctx* ctx, const W4Problem& q)
     return pair_launch(ctx, k);
 }
 
-// The tiled kernels' 32-bit indexes step past the last element, by less than a tile.
-bool tiles_reach(int64_t rows, int64_t C, int64_t W)
-{
-    return rows <= (1 << 30) && C <= (1 << 30) && W <= (1 << 29);
-}
-
 // A sum over nothing is zero in every type.
 tb200_status write_zeros(tb200_ctx* ctx, const tb200_tensor* t)
 {
@@ -444,7 +438,7 @@ tb200_status w4_entry(tb200_ctx* ctx, const char* op, const tb200_tensor* a, con
     }
     // (scales of any width are read as one row, whose elements have 32-bit coordinates)
     const int64_t groups = ((int64_t)q.C + q.group - 1) / q.group;
-    const bool tiled     = ctx->policy == 0 && tiles_reach(q.M, q.C, q.W) && groups * q.W < (1LL << 31) - 256;
+    const bool tiled     = ctx->policy == 0 && tiles_reach(1, q.M, q.C, q.W, false) && groups * q.W < (1LL << 31) - 256;
     return tiled ? w4_launch(ctx, q) : w4_direct_launch(ctx, q);
 }
 
@@ -504,7 +498,7 @@ extern "C" tb200_status tb200_matmul_gated(tb200_ctx* ctx, const tb200_tensor* a
         GatedProblem q = gated_problem(a, gate, up, activation);
         q.out          = output->data;
         q.out_dt       = output->dtype;
-        if (ctx->policy == 0 && tiles_reach(q.H, q.C, q.W))
+        if (ctx->policy == 0 && tiles_reach(q.NB, q.H, q.C, q.W, false))
             return q.dt == TB200_FP32 ? gated_f32(ctx, q) : gated_pair(ctx, q);
         return gated_direct_launch(ctx, q);
     });
@@ -553,7 +547,7 @@ extern "C" tb200_status tb200_matmul_gated_backward(tb200_ctx* ctx, const tb200_
             q.dup    = grad_up->data;
             q.dup_dt = grad_up->dtype;
         }
-        if (ctx->policy == 0 && tiles_reach(q.H, q.C, q.W))
+        if (ctx->policy == 0 && tiles_reach(q.NB, q.H, q.C, q.W, true))
             return q.dt == TB200_FP32 ? gated_backward_f32(ctx, q) : gated_backward_pair(ctx, q);
         const size_t each     = (size_t)q.NB * q.H * q.W * sizeof(float);
         const tb200_status st = ensure_scratch(ctx, 2 * each);

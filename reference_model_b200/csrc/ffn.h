@@ -53,6 +53,9 @@ std::string check_gated_output(const char* op, const tb200_tensor* a, const tb20
 std::string check_gated_grads(const char* op, const tb200_tensor* a, const tb200_tensor* gate, const tb200_tensor* up, const tb200_tensor* dout,
                               const tb200_tensor* da, const tb200_tensor* dgate, const tb200_tensor* dup);
 
+// whether the tiled kernels' 32-bit indexes serve a product of these sizes (or its gradients)
+bool tiles_reach(int64_t batches, int64_t rows, int64_t C, int64_t W, bool gradients);
+
 // ---- ffn_direct.cu: one thread per result, any type and size
 tb200_status w4_direct_launch(tb200_ctx* ctx, const W4Problem& q);
 tb200_status gated_direct_launch(tb200_ctx* ctx, const GatedProblem& q);

@@ -126,6 +126,16 @@ std::string check_gated_output(const char* op, const tb200_tensor* a, const tb20
     return std::string();
 }
 
+// Indexes step past the last element, by less than a tile; tiles, of 128 rows and 64 columns of a gated product (128 of another) at least, are
+// counted in 32 bits with room for a grid's step.
+bool tiles_reach(int64_t batches, int64_t rows, int64_t C, int64_t W, bool gradients)
+{
+    auto tiles = [](int64_t n, int64_t size) { return (double)((n + size - 1) / size); };
+    const double most = 1 << 30;
+    return rows <= (1 << 30) && C <= (1 << 30) && W <= (1 << 29) && batches * tiles(rows, 128) * tiles(W, 64) <= most &&
+           (!gradients || (batches * tiles(rows, 128) * tiles(C, 128) <= most && 2 * batches * tiles(C, 128) * tiles(W, 128) <= most));
+}
+
 std::string check_gated_grads(const char* op, const tb200_tensor* a, const tb200_tensor* gate, const tb200_tensor* up, const tb200_tensor* dout,
                               const tb200_tensor* da, const tb200_tensor* dgate, const tb200_tensor* dup)
 {

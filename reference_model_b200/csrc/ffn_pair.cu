@@ -1224,10 +1224,7 @@ tb200_status launch(tb200_ctx* ctx, const PairProduct& q, int splits)
     k.tiles_n           = (q.cols + step_n - 1) / step_n;
     k.NB                = q.NB;
     k.beside            = q.beside ? 1 : 0;
-    const int64_t tiles = (int64_t)k.tiles_m * k.tiles_n * q.NB * (q.results == 2 && !gated ? 2 : 1);
-    if (tiles > (1 << 30))
-        return fail(ctx, TB200_ERROR, "a feed-forward product of %lld tiles is too large", (long long)tiles);
-    k.num_tiles = (int)tiles;
+    k.num_tiles         = k.tiles_m * k.tiles_n * q.NB * (q.results == 2 && !gated ? 2 : 1);    // (2^30 at most: tiles_reach)
     // A's rows of a group, about 32 MB, stay in L2
     const int64_t a_tile = (int64_t)S::kRows * q.K * q.phases * 2;
     k.group_m  = (int)std::max<int64_t>(1, std::min<int64_t>(k.tiles_m, (32LL << 20) / std::max<int64_t>(1, a_tile)));
