@@ -46,8 +46,8 @@ def gated(ctx, kernel, nb, h, c, w):
     return Call(ctx, kernel, lambda: ctx.matmul_gated(*ts, out, "RELU"), [out], [ref], ts)
 
 
-def four(ctx, kernel, h, c, w, mats):
-    a = whole(4, "fp16", -1, 2, 1, h, c)
+def four(ctx, kernel, h, c, w, mats, dtype="fp16"):
+    a = whole(4, dtype, -1, 2, 1, h, c)
     r = np.random.default_rng(5)
     ops, projections, held = [], [], [put(ctx, a)]
     for _ in range(mats):
@@ -85,6 +85,8 @@ CALLS = {
     "4 bits, one row, a stage a block": lambda ctx: four(ctx, "matmul_w4_rows", 1, 2048, 1000, 1),
     "4 bits, 30 rows": lambda ctx: four(ctx, "matmul_w4_rows", 30, 4096, 12000, 1),
     "4 bits, gated": lambda ctx: four(ctx, "gated_w4_rows", 5, 4096, 6001, 2),
+    "4 bits, fp32 rows": lambda ctx: four(ctx, "matmul_w4_rows", 21, 8192, 12000, 1, "fp32"),
+    "4 bits, gated, fp32 rows": lambda ctx: four(ctx, "gated_w4_rows", 21, 4096, 12001, 2, "fp32"),
     "pairs": lambda ctx: gated(ctx, "gated_pair_f16", 1, 1500, 2000, 2500),
     "pairs, one stage": lambda ctx: gated(ctx, "gated_pair_f16", 1, 3000, 100, 2500),
     "CTAs by themselves": lambda ctx: gated(ctx, "gated_pair_f16", 3, 150, 500, 300),
@@ -100,9 +102,10 @@ CALLS = {
 
 @pytest.mark.parametrize("name", list(CALLS))
 def test_waits_that_give_up_leave_others_alone(two, name):
-    """One context under the shortest limit, another beside it under its usual one.  A short call may well finish within the time that a
-    barrier waits by itself."""
+    """One context under the shortest limit, another beside it under its usual one, and copies that keep the memory busy, so that waits are long.  A
+    short call may well finish within the time that a barrier waits by itself (few rows against 4-bit weights mostly do)."""
     limited, other = (CALLS[name](c) for c in two)
+    copies, side = torch.empty((2, 1 << 29), dtype=torch.uint8, device="cuda"), torch.cuda.Stream()
     for x in (limited, other):
         x.run()
         assert x.ctx.last_kernel() == x.kernel
@@ -112,13 +115,17 @@ def test_waits_that_give_up_leave_others_alone(two, name):
         for _ in range(5):
             for o in other.outs:
                 o.upload(np.full(o.shape, np.nan, np.float32))
-            for _ in range(4):
+            with torch.cuda.stream(side):
+                for _ in range(8):
+                    copies[1].copy_(copies[0])
+            for _ in range(10):
                 limited.run()
                 other.run()
             other.check()
             assert limited.ctx.sync(check=False) in (tb.Status.OK, tb.Status.INTERNAL)
     finally:
         limited.ctx.set_wait_limit(DEFAULT)
+        side.synchronize()
     for _ in range(2):
         limited.run()
         limited.check()
