@@ -312,7 +312,8 @@ __global__ void __launch_bounds__(kSplitThreads, 1) sgemm_split_kernel(const __g
         const int row     = quarter * 32 + lane;
         const uint32_t t0 = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * 64);
         float* const st   = reinterpret_cast<float*>(sm + kOutOff) + warp * 32 * kStagePitch;
-        const bool v8 = (p.N & 7) == 0 && (reinterpret_cast<uintptr_t>(p.out) & 31) == 0;
+        // (two products of one launch: results as far apart as a caller's tensors lie)
+        const bool v8 = (p.N & 7) == 0 && (p.o_batch & 7) == 0 && (reinterpret_cast<uintptr_t>(p.out) & 31) == 0;
         // The stage's MMAs, by the first lane of the first of these warps: issuing takes as long as the MMAs before take to make
         // room in the unit's short queue, so a splitting warp must not do it (the two then take turns: 5 600 cycles a stage), and a warp of its own, the seventeenth, would leave 96 registers per thread instead of 128.
         // These warps have time: a stage's sums take about a third of its MMAs.
