@@ -1,5 +1,5 @@
 // 16-bit products of the feed-forward operators on CTA pairs (tcgen05 cta_group::2): the gated product of two projections, the
-// gradients of its projections, and the plain products of the backward pass and of 4-bit weights laid out in 16 bits.
+// gradients of its projections, the plain products of the backward pass, and both forms with 4-bit weights.
 //
 // A pair owns a 256-row tile of 256 accumulator columns.  Each CTA loads its own 128 rows of A and its own 128 columns of B per 64
 // elements of K; the tensor cores of both read B from both.  For the gated product the first CTA's 128 columns are the gate's and
@@ -202,10 +202,12 @@ __device__ __forceinline__ void gate_run(const uint32_t (&g)[16], const uint32_t
         o[i] = act_value_16<ACT>(__uint_as_float(g[i])) * __uint_as_float(u[i]);
 }
 
-// Results that stay in fp32 take CUDA's functions.  A call, so that sixteen copies of them do not cost the other results' code its registers.
-__device__ __noinline__ float act_value_32(int act, float g)
+template <int ACT>
+__device__ __forceinline__ void gate_run_32(const uint32_t (&g)[16], const uint32_t (&u)[16], float (&o)[16])
 {
-    return act_value(act, g);
+#pragma unroll
+    for (int i = 0; i < 16; i++)
+        o[i] = act_value_32<ACT>(__uint_as_float(g[i])) * __uint_as_float(u[i]);
 }
 
 template <int ACT>
@@ -283,11 +285,17 @@ __device__ __forceinline__ void finish_run(const Params& p, const Tile& t, int r
         float v[16];
         if (p.out_dt == TB200_FP32)
         {
-#pragma unroll
-            for (int i = 0; i < 16; i++)
-                v[i] = act_value_32(p.act, __uint_as_float(g[i])) * __uint_as_float(u[i]);
+            switch (p.act)
+            {
+                case TB200_ACT_SILU: gate_run_32<TB200_ACT_SILU>(g, u, v); break;
+                case TB200_ACT_GELU: gate_run_32<TB200_ACT_GELU>(g, u, v); break;
+                case TB200_ACT_GELU_TANH: gate_run_32<TB200_ACT_GELU_TANH>(g, u, v); break;
+                case TB200_ACT_RELU: gate_run_32<TB200_ACT_RELU>(g, u, v); break;
+                default: gate_run_32<TB200_ACT_SIGMOID>(g, u, v); break;
+            }
         }
         else
+        {
             switch (p.act)
             {
                 case TB200_ACT_SILU: gate_run<TB200_ACT_SILU>(g, u, v); break;
@@ -296,6 +304,7 @@ __device__ __forceinline__ void finish_run(const Params& p, const Tile& t, int r
                 case TB200_ACT_RELU: gate_run<TB200_ACT_RELU>(g, u, v); break;
                 default: gate_run<TB200_ACT_SIGMOID>(g, u, v); break;
             }
+        }
         emit(p.out0, p.out_dt, v);
     }
     else
