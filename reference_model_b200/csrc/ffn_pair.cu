@@ -21,7 +21,7 @@
 //
 // Measured: gated 4096 x 4096 x 8192 bf16 344 us (1600 TFLOP/s, the rate of the library's product for a short time; power holds the
 // clock down when it goes on), backward of the same 1105 us (1490); 777 x 4096 x 4096 with 4-bit weights 35 us (750: 64 of 74 pairs, a quarter of the rows
-// padding; tensor pipe 61 % busy); gated 788 x 1000 x 1416 fp16 14 us, its backward at 394 x 1024 x 2048 32 us (chains of launches
+// padding; tensor pipe 61 % busy); gated 788 x 1000 x 1416 fp16 14.5 us, its backward at 394 x 1024 x 2048 34 us (chains of launches
 // of a few chunks: latencies of set-up, first copies, epilogue and exchange).
 #include <algorithm>
 #include <cstring>

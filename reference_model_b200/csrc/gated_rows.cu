@@ -7,8 +7,10 @@
 // transposing matrix loads as they lie, K across rows.  Blocks of a cluster share K out while the grid leaves SMs idle.  The sums
 // of a stage are added up in fp32 apart from the instruction's own; G and U meet in shared memory, in a fixed order, where the
 // activation and the product are taken.
-// One row, 4096 x 16384 bf16: 42 us for 268 MB, the rate of a plain copy (6.4 TB/s; DRAM 73 % of its peak).  2048 x 8192: 9.5 us for 67 MB.  Small
-// calls are latency: 4 us.  Columns that are no multiple of eight cost a copy of both matrices first (3248 x 3748: 35 us, 7 for 3752).
+// One row, 4096 x 16384 bf16: 42 us for 268 MB, the rate of a plain copy (6.4 TB/s; DRAM 73 % of its peak).  2048 x 8192: 14.2 us for 67 MB that come from
+// memory (six sets of operands in turn), 9.2 where a call finds much of them in L2 (the same operands again).  Small calls are latency: 4.3 us.
+// Matrices whose rows are not multiples of sixteen bytes apart, which TMA cannot address, are read as they lie by warps of their own (SHIFT):
+// 3248 x 3748 27.2 us from memory, 18.5 again, where 3752 columns take 12.1 and 10.5; a copy of both matrices first took 35 again.
 #include <algorithm>
 #include <cstring>
 #include <cuda.h>

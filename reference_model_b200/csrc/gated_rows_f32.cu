@@ -4,7 +4,7 @@
 // A block takes 128 columns of the gate and the same 128 of the up projection, a lane four of each; its eight warps take K's elements in turn,
 // eight loads of a lane on their way together, four blocks to an SM (sixteen loads and two blocks: 4096 x 8192 56 us).  Blocks of a cluster
 // share K out while all run at once.  Sums of warps, then of blocks, are added up in a fixed order.  4096 x 8192: 44 us, 6.1 TB/s, the rate of
-// a plain copy (76 by the fp32 product's tiles and a pass over both projections); 1480 x 7328 15 us (31); 100 x 4000 6.8 us (7.3).  Two rows by
+// a plain copy (76 by the fp32 product's tiles and a pass over both projections); 1480 x 7328 17 us from memory, 15 again (31); 100 x 4000 4.5 us.  Two rows by
 // the same code took 94 us, which leaves them to the tiles.
 #include <algorithm>
 #include <cstring>

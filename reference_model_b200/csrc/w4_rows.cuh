@@ -21,9 +21,11 @@
 // as they lie: threads that fetched them cost 5 us a call).
 //
 // Measured, bf16, one row, group 128 with zero points: 8192 x 8192 15.4 us (35 MB, 2.3 TB/s), gated 4096 x 16384 24.3 us (2.9 TB/s); 24 rows,
-// 4096 x 10250 fp16 21.9 us; 2048 x 1000 6.5 us.  What bounds it: instructions (78 to 100 for 1024 weights; 45 % of the issue slots over
-// the whole kernel, the integer pipe 39 %), and at either end latencies: 1.4 us from the start to the first stage, 1.5 to 4 us from a
-// shared tile's last sums to its results.
+// 4096 x 10250 fp16 21.9 us; 2048 x 1000 6.5 us.  What bounds it: no single thing.  Instructions, 78 to 100 for 1024 weights, are 5 to 6 us of issue time for
+// the first, 9 to 11 for the second, 3 to 3.5 for the third (45 % of the issue slots and 39 % of the integer pipe over the whole kernel).  Shared memory:
+// with three tiles of eight rows each of eight warps reads all of `a` for its sixteen matrix rows, 98 KB a stage beside 16 KB of weights, about 4 us, and
+// permutes it again.  Latencies at either end, paid for 4 to 14 stages a block: 1.4 us from the start to the first stage, 1.5 to 4 us
+// from a shared tile's last sums to its results.
 #pragma once
 #include <cuda.h>
 #include <type_traits>
