@@ -107,9 +107,8 @@ struct Params
 };
 
 // fp16 has five bits of exponent: from 65520 on dG and dU would be infinite, and below 2^-14 they lose places.  Where the largest of a call is outside of
-// what fp16 holds well, all are held under the power of two that brings it to 2^14 .. 2^15.  Sums of products with values that small are
-// exact in the power, so gradients come out as if dG and dU had a float's exponent, but for values below 2^-39 of the largest (2^-17 where
-// no power is taken), which become 0.
+// what fp16 holds well, all are held under the power of two that brings it to 2^14 .. 2^15, and the products' fp32 sums are divided by it again, which
+// rounds nothing.  Values below 2^-39 of the largest become 0 (2^-17 where no power is taken and the largest is near 2^-8).
 __device__ __forceinline__ float range_scale(float peak)
 {
     if (!(peak >= 65520.f || (peak > 0.f && peak < 0x1p-8f)))
